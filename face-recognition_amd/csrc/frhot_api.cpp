@@ -5,6 +5,7 @@
 #include <dlfcn.h>
 
 #include <atomic>
+#include <climits>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -108,6 +109,8 @@ struct IndexPin {
     bool pending = false;
 };
 
+struct frhot_head;
+
 struct frhot_ctx {
     int device = 0;
     hipStream_t stream = nullptr;
@@ -161,6 +164,12 @@ struct frhot_ctx {
     void* xq = nullptr; size_t xq_cap = 0;           // every rank's queries, fp16 [world*B, D]
     int32_t* xk = nullptr; size_t xk_cap = 0;        // every rank's keys [world*B]
     int64_t* xblk = nullptr; size_t xblk_cap = 0;    // this shard's answer block, then the world's blocks (int64 words)
+    // descriptor heads: scratch of the linear kernels (allocated with the first layer), the attached head
+    void* lin_ws = nullptr; LinearWork lin{};
+    frhot_head* head = nullptr;
+    // page-locked item lists of the page calls, taken in turn (a list is free again once the stream has passed its call)
+    IndexPin page_pin[4]; unsigned page_next = 0;
+    int32_t* page_off = nullptr; size_t page_off_cap = 0;    // compact: live rows in front of every tile
     // timing: per stage a ring of (begin, end) event pairs; n[i] counts recorded pairs
     bool timing = false;
     static constexpr int kRing = 128;
@@ -179,6 +188,27 @@ struct frhot_ctx {
 };
 
 static void dist_release(frhot_ctx* c);
+
+// One layer of a descriptor head: weights in fragment order, padded bias.
+struct frhot_linear {
+    frhot_ctx* ctx = nullptr;
+    int N = 0, K = 0, dtype = 0;
+    void* wt = nullptr;
+    float* bias = nullptr;
+    int heads = 0;              // heads that hold this layer
+};
+
+struct frhot_head {
+    frhot_ctx* ctx = nullptr;
+    struct Layer { frhot_linear* lin; int act; bool residual; };
+    std::vector<Layer> layers;
+    int din = 0, dout = 0;
+    int64_t rows = 0;           // rows one pass of the layers takes (longer inputs go through in runs of this many)
+    void* in16 = nullptr;       // fp16 [rows, din]: gallery rows brought out for a residual of the first layer
+    void* mid[2] = {};          // fp16 [rows, widest inner layer], in turn
+    float* y = nullptr;         // fp32 [rows, dout]: the last layer's output, in front of its norm
+    void* desc = nullptr;       // fp16 [max_batch, 4096]: descriptors of an embed call, while the head is attached
+};
 
 struct frhot_gallery {
     frhot_ctx* ctx = nullptr;
@@ -262,6 +292,42 @@ int upload(void** dst, const void* src, size_t n) {
 }
 
 constexpr int kSplitMin = 32;   // batches from this size on run their conv stack as two halves on two streams
+
+// The layers of a head over M fp16 rows of din values (`x`: rows ldx apart, or, `tiled`, the start of a tile of a gallery of
+// dimension din), the last layer's rows brought to unit length into `o` (its row0 counts on with the runs).  Inner layers
+// round to fp16 between layers, as every activation of the library does; the last one stays fp32 up to the norm.
+int head_enqueue(frhot_head* h, const void* x, int64_t ldx, bool tiled, int64_t M, UnitOut o) {
+    frhot_ctx* c = h->ctx;
+    hipStream_t s = c->stream;
+    const int nl = (int)h->layers.size();
+    for (int64_t m0 = 0; m0 < M; m0 += h->rows) {
+        const int64_t n = M - m0 < h->rows ? M - m0 : h->rows;
+        const void* in = tiled ? (const char*)x + (size_t)m0 * h->din * 2 : (const char*)x + (size_t)m0 * ldx * 2;
+        int64_t ld = ldx;
+        bool t = tiled;
+        for (int l = 0; l < nl; ++l) {
+            const frhot_head::Layer& L = h->layers[l];
+            if (t && L.residual) {          // the residual is added from rows in plain order
+                HIP_TRY(launch_page_rows(in, h->in16, n, h->din, s));
+                in = h->in16; ld = h->din; t = false;
+            }
+            LinearCall q{};
+            q.x = in; q.ldx = ld; q.tiled = t ? 1 : 0; q.bf16 = 0;
+            q.wt = L.lin->wt; q.bias = L.lin->bias; q.M = n; q.N = L.lin->N; q.K = L.lin->K;
+            const bool last = l == nl - 1;
+            q.out.out = last ? (void*)h->y : h->mid[l & 1];
+            q.out.ldo = q.N; q.out.otype = last ? kF32 : kF16; q.out.act = L.act;
+            if (L.residual) { q.out.res = in; q.out.ldr = ld; q.out.rtype = kF16; }
+            HIP_TRY(launch_linear(q, c->lin, s));
+            in = q.out.out; ld = q.N; t = false;
+        }
+        UnitOut u = o;
+        if (o.gallery) u.row0 = o.row0 + m0;
+        else u.out = (char*)o.out + (size_t)m0 * o.ldo * 2;
+        HIP_TRY(launch_unit_rows(h->y, kF32, h->dout, n, h->dout, u, s));
+    }
+    return FRHOT_OK;
+}
 
 // What embed_enqueue asks before it enqueues the second half of a batch: a host call whose crops
 // are still being packed and uploaded lets the first half start on the GPU meanwhile.
@@ -371,7 +437,14 @@ int embed_enqueue(frhot_ctx* c, const void* crops_dev, const int64_t* offsets, c
     HIP_TRY(launch_fc_splitk(c->act[kNumConv - 1], c->w6, c->partial, B, kFcN, kFc6K, kFc6Split, s));
     HIP_TRY(launch_fc_reduce_relu(c->partial, c->b6, c->fc6_out, B, kFcN, kFc6Split, s));
     HIP_TRY(launch_fc_splitk(c->fc6_out, c->w7, c->partial, B, kFcN, kFcN, kFc7Split, s));
-    HIP_TRY(launch_fc_reduce_relu_l2(c->partial, c->b7, out_f32, out_q, out_q ? Dq : kFcN, B, kFcN, kFc7Split, s));
+    if (out_q && c->head && Dq == c->head->dout) {
+        // queries of the attached head's width: the whole descriptor in fp16, then the head
+        HIP_TRY(launch_fc_reduce_relu_l2(c->partial, c->b7, out_f32, c->head->desc, kFcN, B, kFcN, kFc7Split, s));
+        const int rc = head_enqueue(c->head, c->head->desc, kFcN, false, B, UnitOut{out_q, Dq, 0, 0, nullptr, nullptr});
+        if (rc) return rc;
+    } else {
+        HIP_TRY(launch_fc_reduce_relu_l2(c->partial, c->b7, out_f32, out_q, out_q ? Dq : kFcN, B, kFcN, kFc7Split, s));
+    }
     if (c->stage_end(2)) return fail(FRHOT_EHIP, "event record failed");
     return FRHOT_OK;
 }
@@ -1012,6 +1085,7 @@ int frhot_ctx_create(int device_id, void* stream, int max_batch, frhot_ctx** out
     if (strncmp(prop.gcnArchName, "gfx950", 6) != 0)
         return fail(FRHOT_EHIP, "device %d is %s; this library holds gfx950 code only", device_id, prop.gcnArchName);
     HIP_TRY(kernels_init());
+    HIP_TRY(linear_kernels_init());
     frhot_ctx* c = new frhot_ctx();
     c->device = device_id;
     c->max_batch = max_batch;
@@ -1064,6 +1138,12 @@ int frhot_ctx_destroy(frhot_ctx* c) {
             if (c->ev_b[i][j]) (void)hipEventDestroy(c->ev_b[i][j]);
             if (c->ev_e[i][j]) (void)hipEventDestroy(c->ev_e[i][j]);
         }
+    if (c->lin_ws) (void)hipFree(c->lin_ws);
+    if (c->page_off) (void)hipFree(c->page_off);
+    for (auto& ip : c->page_pin) {
+        if (ip.p) (void)hipHostFree(ip.p);
+        if (ip.copied) (void)hipEventDestroy(ip.copied);
+    }
     if (c->own_stream && c->stream) (void)hipStreamDestroy(c->stream);
     delete c;
     return FRHOT_OK;
@@ -2246,6 +2326,579 @@ int frhot_det_debug_read(frhot_detector* d, const char* name, int B, void* host_
     DeviceGuard dg(d->ctx->device);
     HIP_TRY(hipStreamSynchronize(d->ctx->stream));
     HIP_TRY(hipMemcpy(host_out, it->second.p, need, hipMemcpyDeviceToHost));
+    return FRHOT_OK;
+    });
+}
+
+}  // extern "C"
+
+// ---- descriptor heads ---------------------------------------------------------------------------
+namespace {
+
+bool linear_type_ok(int t) { return t == kF16 || t == kF32 || t == kBF16; }
+size_t type_size(int t) { return t == kF32 ? 4 : 2; }
+
+// Bytes from the first to the last value of M rows of n values ld apart.
+size_t span_bytes(int64_t M, int64_t n, int64_t ld, int type) { return ((size_t)(M - 1) * (size_t)ld + (size_t)n) * type_size(type); }
+bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+    return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
+
+constexpr int kMaxWidth = 65536;            // N and K of a layer
+constexpr int64_t kMaxRows = 0x7fffff00LL;  // rows of one call
+constexpr size_t kSlabBytes = 64u << 20, kPackBytes = 34u << 20;
+
+// The linear kernels' scratch of a context: partial sums of K slices, rows packed for the 16-byte loads, zeros.
+int linear_scratch(frhot_ctx* c) {
+    if (c->lin_ws) return FRHOT_OK;
+    const size_t total = kSlabBytes + kPackBytes + 256;
+    HIP_TRY(hipMalloc(&c->lin_ws, total));
+    hipError_t e = hipMemset((char*)c->lin_ws + kSlabBytes + kPackBytes, 0, 256);
+    if (e != hipSuccess) {
+        (void)free_null(c->lin_ws);
+        return fail(FRHOT_EHIP, "clearing the linear scratch failed: %s", hipGetErrorString(e));
+    }
+    c->lin = LinearWork{(float*)c->lin_ws, kSlabBytes, (char*)c->lin_ws + kSlabBytes, kPackBytes, (char*)c->lin_ws + kSlabBytes + kPackBytes};
+    return FRHOT_OK;
+}
+
+int check_rows_args(const char* what, const void* p, int64_t ld, int64_t M, int64_t n, int type) {
+    if (!p) return fail(FRHOT_EINVAL, "%s is null", what);
+    if (!linear_type_ok(type)) return fail(FRHOT_EINVAL, "%s: element type %d is not FRHOT_F16 / _F32 / _BF16", what, type);
+    if (ld < n) return fail(FRHOT_EINVAL, "%s: rows of %lld values are %lld apart", what, (long long)n, (long long)ld);
+    if (M > 1 && ld > (int64_t)1 << 40) return fail(FRHOT_EINVAL, "%s: row distance %lld", what, (long long)ld);
+    if ((uintptr_t)p % type_size(type)) return fail(FRHOT_EINVAL, "%s is not aligned to its elements", what);
+    return FRHOT_OK;
+}
+
+void head_free(frhot_head* h) {
+    void* ptrs[] = {h->in16, h->mid[0], h->mid[1], h->y, h->desc};
+    for (void* p : ptrs) if (p) (void)hipFree(p);
+    for (auto& L : h->layers) --L.lin->heads;
+    delete h;
+}
+
+}  // namespace
+
+extern "C" {
+
+int frhot_linear_create(frhot_ctx* c, const void* w, const float* bias, int N, int K, int dtype, frhot_linear** out) {
+    return guarded([&]() -> int {
+    if (!out) return fail(FRHOT_EINVAL, "out is null");
+    *out = nullptr;
+    if (!c || !w) return fail(FRHOT_EINVAL, "null argument");
+    if (N <= 0 || K <= 0 || N > kMaxWidth || K > kMaxWidth) return fail(FRHOT_EINVAL, "layer of %d x %d outside 1..%d", N, K, kMaxWidth);
+    if (dtype != kF16 && dtype != kBF16) return fail(FRHOT_EINVAL, "weights of type %d: FRHOT_F16 or FRHOT_BF16", dtype);
+    std::lock_guard<std::mutex> lk(c->mu);
+    DeviceGuard dg(c->device);
+    if (!dg.ok) return fail(FRHOT_EHIP, "cannot select device %d", c->device);
+    int rc = linear_scratch(c);
+    if (rc) return rc;
+    std::unique_ptr<frhot_linear> l(new frhot_linear());
+    l->ctx = c; l->N = N; l->K = K; l->dtype = dtype;
+    std::vector<float> b((size_t)linear_npad(N), 0.f);
+    if (bias) memcpy(b.data(), bias, (size_t)N * 4);
+    void* raw = nullptr;
+    hipError_t e = hipMalloc(&raw, (size_t)N * K * 2);
+    if (e == hipSuccess) e = hipMemcpy(raw, w, (size_t)N * K * 2, hipMemcpyHostToDevice);
+    if (e == hipSuccess) e = hipMalloc(&l->wt, linear_layout_bytes(N, K));
+    if (e == hipSuccess) e = hipMalloc((void**)&l->bias, b.size() * 4);
+    if (e == hipSuccess) e = hipMemcpy(l->bias, b.data(), b.size() * 4, hipMemcpyHostToDevice);
+    if (e == hipSuccess) e = launch_linear_layout(raw, l->wt, N, K, c->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(c->stream);
+    if (raw) (void)hipFree(raw);
+    if (e != hipSuccess) {
+        if (l->wt) (void)hipFree(l->wt);
+        if (l->bias) (void)hipFree(l->bias);
+        return fail(FRHOT_EHIP, "loading a layer of %d x %d failed: %s", N, K, hipGetErrorString(e));
+    }
+    *out = l.release();
+    return FRHOT_OK;
+    });
+}
+
+int frhot_linear_destroy(frhot_linear* l) {
+    return guarded([&]() -> int {
+    if (!l) return FRHOT_OK;
+    std::lock_guard<std::mutex> lk(l->ctx->mu);
+    if (l->heads) return fail(FRHOT_ESTATE, "the layer belongs to %d head(s)", l->heads);
+    DeviceGuard dg(l->ctx->device);
+    (void)hipStreamSynchronize(l->ctx->stream);
+    (void)hipFree(l->wt);
+    (void)hipFree(l->bias);
+    delete l;
+    return FRHOT_OK;
+    });
+}
+
+int frhot_linear_dev(frhot_linear* l, const void* x_dev, int64_t ldx, int64_t M, int act, const void* residual_dev, int64_t ldr,
+                     int residual_dtype, void* out_dev, int64_t ldo, int out_dtype) {
+    return guarded([&]() -> int {
+    if (!l) return fail(FRHOT_EINVAL, "layer is null");
+    if (M < 0 || M > kMaxRows) return fail(FRHOT_EINVAL, "%lld rows outside 0..%lld", (long long)M, (long long)kMaxRows);
+    if (act < kActNone || act > kActGeluTanh) return fail(FRHOT_EINVAL, "activation %d is not one of FRHOT_ACT_*", act);
+    if (M == 0) return FRHOT_OK;
+    int rc = check_rows_args("x", x_dev, ldx, M, l->K, l->dtype);
+    if (!rc) rc = check_rows_args("out", out_dev, ldo, M, l->N, out_dtype);
+    if (!rc && residual_dev) rc = check_rows_args("residual", residual_dev, ldr, M, l->N, residual_dtype);
+    if (rc) return rc;
+    const size_t out_bytes = span_bytes(M, l->N, ldo, out_dtype);
+    if (overlap(out_dev, out_bytes, x_dev, span_bytes(M, l->K, ldx, l->dtype))) return fail(FRHOT_EINVAL, "out overlaps x");
+    if (residual_dev && overlap(out_dev, out_bytes, residual_dev, span_bytes(M, l->N, ldr, residual_dtype)) &&
+        !(out_dev == residual_dev && ldo == ldr && type_size(out_dtype) == type_size(residual_dtype)))
+        return fail(FRHOT_EINVAL, "out overlaps the residual without being it");
+    frhot_ctx* c = l->ctx;
+    std::lock_guard<std::mutex> lk(c->mu);
+    DeviceGuard dg(c->device);
+    LinearCall q{};
+    q.x = x_dev; q.ldx = ldx; q.bf16 = l->dtype == kBF16; q.wt = l->wt; q.bias = l->bias; q.M = M; q.N = l->N; q.K = l->K;
+    q.out.out = out_dev; q.out.ldo = ldo; q.out.otype = out_dtype; q.out.act = act;
+    q.out.res = residual_dev; q.out.ldr = residual_dev ? ldr : 0; q.out.rtype = residual_dev ? residual_dtype : kF16;
+    HIP_TRY(launch_linear(q, c->lin, c->stream));
+    return FRHOT_OK;
+    });
+}
+
+int frhot_unit_rows_dev(frhot_ctx* c, const void* x_dev, int dtype, int64_t ldx, int64_t M, int N, void* out_f16_dev, int64_t ldo) {
+    return guarded([&]() -> int {
+    if (!c) return fail(FRHOT_EINVAL, "ctx is null");
+    if (M < 0 || M > kMaxRows) return fail(FRHOT_EINVAL, "%lld rows outside 0..%lld", (long long)M, (long long)kMaxRows);
+    if (N <= 0 || N > kMaxWidth) return fail(FRHOT_EINVAL, "rows of %d values outside 1..%d", N, kMaxWidth);
+    if (M == 0) return FRHOT_OK;
+    int rc = check_rows_args("x", x_dev, ldx, M, N, dtype);
+    if (!rc) rc = check_rows_args("out", out_f16_dev, ldo, M, N, kF16);
+    if (rc) return rc;
+    if (overlap(out_f16_dev, span_bytes(M, N, ldo, kF16), x_dev, span_bytes(M, N, ldx, dtype))) return fail(FRHOT_EINVAL, "out overlaps x");
+    std::lock_guard<std::mutex> lk(c->mu);
+    DeviceGuard dg(c->device);
+    HIP_TRY(launch_unit_rows(x_dev, dtype, ldx, M, N, UnitOut{out_f16_dev, ldo, 0, 0, nullptr, nullptr}, c->stream));
+    return FRHOT_OK;
+    });
+}
+
+int frhot_head_create(frhot_ctx* c, frhot_linear* const* layers, const int32_t* acts, const int32_t* residuals, int n, frhot_head** out) {
+    return guarded([&]() -> int {
+    if (!out) return fail(FRHOT_EINVAL, "out is null");
+    *out = nullptr;
+    if (!c || !layers || !acts) return fail(FRHOT_EINVAL, "null argument");
+    if (n <= 0 || n > 16) return fail(FRHOT_EINVAL, "%d layers outside 1..16", n);
+    int widest = 0;
+    for (int i = 0; i < n; ++i) {
+        if (!layers[i] || layers[i]->ctx != c) return fail(FRHOT_EINVAL, "layer %d is null or belongs to another context", i);
+        if (layers[i]->dtype != kF16) return fail(FRHOT_EINVAL, "layer %d: a head takes fp16 layers (descriptors and gallery rows are fp16)", i);
+        if (acts[i] < kActNone || acts[i] > kActGeluTanh) return fail(FRHOT_EINVAL, "layer %d: activation %d is not one of FRHOT_ACT_*", i, acts[i]);
+        if (i && layers[i]->K != layers[i - 1]->N)
+            return fail(FRHOT_EINVAL, "layer %d takes %d values, layer %d gives %d", i, layers[i]->K, i - 1, layers[i - 1]->N);
+        if (residuals && residuals[i] && layers[i]->K != layers[i]->N)
+            return fail(FRHOT_EINVAL, "layer %d of %d x %d cannot add its input", i, layers[i]->N, layers[i]->K);
+        if (i < n - 1 && layers[i]->N > widest) widest = layers[i]->N;
+    }
+    const int din = layers[0]->K, dout = layers[n - 1]->N;
+    if (din % 64 || dout % 64) return fail(FRHOT_EINVAL, "a head takes and gives multiples of 64 values (%d -> %d)", din, dout);
+    std::lock_guard<std::mutex> lk(c->mu);
+    DeviceGuard dg(c->device);
+    std::unique_ptr<frhot_head, void (*)(frhot_head*)> h(new frhot_head(), head_free);
+    h->ctx = c; h->din = din; h->dout = dout;
+    for (int i = 0; i < n; ++i) {
+        h->layers.push_back({layers[i], acts[i], residuals && residuals[i]});
+        ++layers[i]->heads;
+    }
+    // As many rows a pass as fill the GPU with tiles and keep the intermediates inside the 256 MiB Infinity Cache
+    // (32,768 rows of a 512-wide fp32 output: 64 MiB).
+    const bool bring_out = h->layers[0].residual;
+    const size_t per_row = (size_t)dout * 4 + (size_t)widest * 2 * (n > 2 ? 2 : 1) + (bring_out ? (size_t)din * 2 : 0);
+    int64_t rows = (int64_t)((192u << 20) / per_row) / 256 * 256;
+    h->rows = rows < 2048 ? 2048 : (rows > 32768 ? 32768 : rows);
+    hipError_t e = hipMalloc((void**)&h->y, (size_t)h->rows * dout * 4);
+    if (e == hipSuccess && n > 1) e = hipMalloc(&h->mid[0], (size_t)h->rows * widest * 2);
+    if (e == hipSuccess && n > 2) e = hipMalloc(&h->mid[1], (size_t)h->rows * widest * 2);
+    if (e == hipSuccess && bring_out) e = hipMalloc(&h->in16, (size_t)h->rows * din * 2);
+    if (e != hipSuccess) return fail(FRHOT_EHIP, "head scratch for %lld rows failed: %s", (long long)h->rows, hipGetErrorString(e));
+    *out = h.release();
+    return FRHOT_OK;
+    });
+}
+
+int frhot_head_destroy(frhot_head* h) {
+    return guarded([&]() -> int {
+    if (!h) return FRHOT_OK;
+    frhot_ctx* c = h->ctx;
+    std::lock_guard<std::mutex> lk(c->mu);
+    DeviceGuard dg(c->device);
+    (void)hipStreamSynchronize(c->stream);
+    if (c->head == h) c->head = nullptr;
+    head_free(h);
+    return FRHOT_OK;
+    });
+}
+
+int frhot_head_dev(frhot_head* h, const void* x_f16_dev, int64_t ldx, int64_t M, void* out_f16_dev, int64_t ldo) {
+    return guarded([&]() -> int {
+    if (!h) return fail(FRHOT_EINVAL, "head is null");
+    if (M < 0 || M > kMaxRows) return fail(FRHOT_EINVAL, "%lld rows outside 0..%lld", (long long)M, (long long)kMaxRows);
+    if (M == 0) return FRHOT_OK;
+    int rc = check_rows_args("x", x_f16_dev, ldx, M, h->din, kF16);
+    if (!rc) rc = check_rows_args("out", out_f16_dev, ldo, M, h->dout, kF16);
+    if (rc) return rc;
+    if (overlap(out_f16_dev, span_bytes(M, h->dout, ldo, kF16), x_f16_dev, span_bytes(M, h->din, ldx, kF16)))
+        return fail(FRHOT_EINVAL, "out overlaps x");
+    std::lock_guard<std::mutex> lk(h->ctx->mu);
+    DeviceGuard dg(h->ctx->device);
+    return head_enqueue(h, x_f16_dev, ldx, false, M, UnitOut{out_f16_dev, ldo, 0, 0, nullptr, nullptr});
+    });
+}
+
+int frhot_ctx_head(frhot_ctx* c, frhot_head* h) {
+    return guarded([&]() -> int {
+    if (!c) return fail(FRHOT_EINVAL, "ctx is null");
+    if (h && h->ctx != c) return fail(FRHOT_EINVAL, "head belongs to another context");
+    if (h && h->din != kFcN) return fail(FRHOT_EINVAL, "a head of %d inputs does not take descriptors of %d", h->din, kFcN);
+    if (h && h->dout > kFcN) return fail(FRHOT_EINVAL, "a head of %d outputs: queries have at most %d components", h->dout, kFcN);
+    std::lock_guard<std::mutex> lk(c->mu);
+    DeviceGuard dg(c->device);
+    if (h && !h->desc) HIP_TRY(hipMalloc(&h->desc, (size_t)c->max_batch * kFcN * 2));
+    c->head = h;
+    return FRHOT_OK;
+    });
+}
+
+}  // extern "C"
+
+// ---- pages of a gallery -------------------------------------------------------------------------
+namespace {
+
+struct PageRun { int64_t src, dst; int32_t n, key; };
+
+// Runs [first[i], first[i] + counts[i]) inside [0, limit), counts null = 1 each; the sum of the lengths goes to *total.
+int page_check_runs(const char* what, const int64_t* first, const int32_t* counts, int nruns, int64_t limit, int64_t* total) {
+    int64_t sum = 0;
+    for (int i = 0; i < nruns; ++i) {
+        const int64_t n = counts ? counts[i] : 1;
+        if (n <= 0) return fail(FRHOT_EINVAL, "%s run %d has %lld rows", what, i, (long long)n);
+        if (first[i] < 0 || first[i] > limit - n)
+            return fail(FRHOT_ECAPACITY, "%s rows [%lld,%lld) outside capacity %lld", what, (long long)first[i], (long long)(first[i] + n), (long long)limit);
+        sum += n;
+    }
+    *total = sum;
+    return FRHOT_OK;
+}
+
+// No row twice among the runs (a row written by two runs would end with either's content).
+int page_check_disjoint(const int64_t* first, const int32_t* counts, int nruns, std::vector<std::pair<int64_t, int64_t>>& sorted) {
+    sorted.resize((size_t)nruns);
+    bool ascending = true;
+    for (int i = 0; i < nruns; ++i) {
+        sorted[i] = {first[i], first[i] + (counts ? counts[i] : 1)};
+        ascending = ascending && (i == 0 || sorted[i - 1].first <= sorted[i].first);
+    }
+    if (!ascending) std::sort(sorted.begin(), sorted.end());
+    for (int i = 1; i < nruns; ++i)
+        if (sorted[i].first < sorted[i - 1].second)
+            return fail(FRHOT_EINVAL, "row %lld is a destination twice", (long long)sorted[i].first);
+    return FRHOT_OK;
+}
+
+// Page-locked memory for a page call of the stream; mark behind the launch that reads it.
+int page_pin_take(frhot_ctx* c, size_t words, IndexPin** out) {
+    // a captured launch would read the list at every replay, long after another call has taken the memory
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    HIP_TRY(hipStreamIsCapturing(c->stream, &st));
+    if (st != hipStreamCaptureStatusNone) return fail(FRHOT_ESTATE, "row lists cannot be captured into a graph");
+    IndexPin& ip = c->page_pin[c->page_next++ & 3];
+    const int rc = index_pin_grow(ip, words);
+    *out = &ip;
+    return rc;
+}
+int page_pin_mark(frhot_ctx* c, IndexPin* ip) {
+    HIP_TRY(hipEventRecord(ip->copied, c->stream));
+    ip->pending = true;
+    return FRHOT_OK;
+}
+
+// Runs -> items of at most kPageRows rows in page-locked memory, moved by one launch.  A null side's `first` counts from 0 on.
+int page_move_enqueue(frhot_ctx* c, const PageSide& src, const int64_t* src_first, const PageSide& dst, const int64_t* dst_first,
+                      const int32_t* counts, const int32_t* keys, int nruns, int D) {
+    size_t items = 0;
+    for (int i = 0; i < nruns; ++i) items += (size_t)((counts ? counts[i] : 1) + kPageRows - 1) / kPageRows;
+    if (items > 0x7fffffffu) return fail(FRHOT_ECAPACITY, "%zu row runs in one call", items);
+    IndexPin* ip = nullptr;
+    int rc = page_pin_take(c, items * (sizeof(PageItem) / 4) + 2, &ip);
+    if (rc) return rc;
+    PageItem* it = (PageItem*)ip->p;
+    int64_t dense = 0;
+    size_t k = 0;
+    for (int i = 0; i < nruns; ++i) {
+        const int32_t n = counts ? counts[i] : 1;
+        const int64_t s0 = src_first ? src_first[i] : dense, d0 = dst_first ? dst_first[i] : dense;
+        for (int32_t at = 0; at < n; at += kPageRows)
+            it[k++] = PageItem{s0 + at, d0 + at, n - at < kPageRows ? n - at : kPageRows, keys ? keys[i] : kKeepKey};
+        dense += n;
+    }
+    HIP_TRY(launch_page_move(src, dst, it, (int)items, D, c->stream));
+    return page_pin_mark(c, ip);
+}
+
+// What a gallery's host-side tables know after the runs were written: `sorted` ascending destination runs, keys per run (in the
+// caller's order, `first` / `counts`) or null: keys that only the device knows.
+void page_note_writes(frhot_gallery* g, const std::vector<std::pair<int64_t, int64_t>>& sorted, const int64_t* first, const int32_t* counts,
+                      const int32_t* keys, int nruns, bool all_live) {
+    int64_t end = g->nrows;
+    bool dense = g->dense && all_live;
+    for (const auto& r : sorted) {
+        if (r.first > end) dense = false;
+        if (r.second > end) end = r.second;
+    }
+    g->dense = dense;
+    g->nrows = end;
+    if (!keys) { g->key_tiles_valid = false; return; }
+    for (int i = 0; i < nruns; ++i) {
+        if (keys[i] < 0) continue;
+        const int64_t last = first[i] + (counts ? counts[i] : 1) - 1;
+        for (int64_t r = first[i]; r <= last; r = ((r >> 8) + 1) << 8) key_tiles_add(g, &r, &keys[i], 1);
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+int frhot_gallery_copy(frhot_gallery* src, const int64_t* src_rows, frhot_gallery* dst, const int64_t* dst_rows, const int32_t* counts,
+                       const int32_t* keys, int nruns) {
+    return guarded([&]() -> int {
+    if (!src || !dst || !src_rows || !dst_rows) return fail(FRHOT_EINVAL, "null argument");
+    if (nruns <= 0) return fail(FRHOT_EINVAL, "nruns must be positive");
+    if (src->ctx != dst->ctx) return fail(FRHOT_EINVAL, "the galleries belong to two contexts");
+    if (src->D != dst->D) return fail(FRHOT_EINVAL, "rows of %d components do not fit a gallery of %d", src->D, dst->D);
+    if (keys)
+        for (int i = 0; i < nruns; ++i)
+            if (keys[i] < 0) return fail(FRHOT_EINVAL, "key %d must be non-negative", keys[i]);
+    frhot_ctx* c = src->ctx;
+    std::lock_guard<std::mutex> lk(c->mu);
+    int64_t total = 0;
+    int rc = page_check_runs("source", src_rows, counts, nruns, src->capacity, &total);
+    if (!rc) rc = page_check_runs("destination", dst_rows, counts, nruns, dst->capacity, &total);
+    std::vector<std::pair<int64_t, int64_t>> to;
+    if (!rc) rc = page_check_disjoint(dst_rows, counts, nruns, to);
+    if (rc) return rc;
+    bool inside = true;             // every source row was written once
+    for (int i = 0; i < nruns; ++i) inside = inside && src_rows[i] + (counts ? counts[i] : 1) <= src->nrows;
+    if (src == dst) {
+        // a row that is read and written in one call would be copied before or after its change
+        for (int i = 0; i < nruns; ++i) {
+            const int64_t lo = src_rows[i], hi = lo + (counts ? counts[i] : 1);
+            auto it = std::upper_bound(to.begin(), to.end(), std::make_pair(lo, INT64_MAX));
+            if ((it != to.begin() && std::prev(it)->second > lo) || (it != to.end() && it->first < hi))
+                return fail(FRHOT_EINVAL, "rows [%lld,%lld) are read and written by one call", (long long)lo, (long long)hi);
+        }
+    }
+    DeviceGuard dg(c->device);
+    rc = page_move_enqueue(c, PageSide{src->rows, src->keys, 0}, src_rows, PageSide{dst->rows, dst->keys, 0}, dst_rows, counts, keys, nruns, src->D);
+    if (rc) return rc;
+    page_note_writes(dst, to, dst_rows, counts, keys, nruns, keys ? true : (src->dense && inside));
+    return FRHOT_OK;
+    });
+}
+
+int frhot_gallery_read_dev(frhot_gallery* g, const int64_t* rows, const int32_t* counts, int nruns, void* out_f16_dev, int32_t* out_keys_dev) {
+    return guarded([&]() -> int {
+    if (!g || !rows || !out_f16_dev) return fail(FRHOT_EINVAL, "null argument");
+    if (nruns <= 0) return fail(FRHOT_EINVAL, "nruns must be positive");
+    if ((uintptr_t)out_f16_dev % 16) return fail(FRHOT_EINVAL, "out is not 16-byte aligned");
+    frhot_ctx* c = g->ctx;
+    std::lock_guard<std::mutex> lk(c->mu);
+    int64_t total = 0;
+    int rc = page_check_runs("source", rows, counts, nruns, g->capacity, &total);
+    if (rc) return rc;
+    DeviceGuard dg(c->device);
+    return page_move_enqueue(c, PageSide{g->rows, g->keys, 0}, rows, PageSide{out_f16_dev, out_keys_dev, 1}, nullptr, counts, nullptr, nruns, g->D);
+    });
+}
+
+int frhot_gallery_write_dev(frhot_gallery* g, const void* rows_f16_dev, const int64_t* rows, const int32_t* counts, const int32_t* keys, int nruns) {
+    return guarded([&]() -> int {
+    if (!g || !rows_f16_dev || !rows || !keys) return fail(FRHOT_EINVAL, "null argument");
+    if (nruns <= 0) return fail(FRHOT_EINVAL, "nruns must be positive");
+    if ((uintptr_t)rows_f16_dev % 16) return fail(FRHOT_EINVAL, "the rows are not 16-byte aligned");
+    bool live = true;
+    for (int i = 0; i < nruns; ++i) {
+        if (keys[i] < FRHOT_KEY_DEAD) return fail(FRHOT_EINVAL, "key %d is not a row key", keys[i]);
+        live = live && keys[i] >= 0;
+    }
+    frhot_ctx* c = g->ctx;
+    std::lock_guard<std::mutex> lk(c->mu);
+    int64_t total = 0;
+    int rc = page_check_runs("destination", rows, counts, nruns, g->capacity, &total);
+    std::vector<std::pair<int64_t, int64_t>> to;
+    if (!rc) rc = page_check_disjoint(rows, counts, nruns, to);
+    if (rc) return rc;
+    DeviceGuard dg(c->device);
+    rc = page_move_enqueue(c, PageSide{const_cast<void*>(rows_f16_dev), nullptr, 1}, nullptr, PageSide{g->rows, g->keys, 0}, rows, counts, keys, nruns, g->D);
+    if (rc) return rc;
+    page_note_writes(g, to, rows, counts, keys, nruns, live);
+    return FRHOT_OK;
+    });
+}
+
+int frhot_gallery_free_keys(frhot_gallery* g, const int32_t* keys, int nkeys, int64_t* freed) {
+    return guarded([&]() -> int {
+    if (freed) *freed = 0;
+    if (!g || !keys) return fail(FRHOT_EINVAL, "null argument");
+    if (nkeys <= 0) return fail(FRHOT_EINVAL, "nkeys must be positive");
+    std::vector<int32_t> want(keys, keys + nkeys);
+    std::sort(want.begin(), want.end());
+    want.erase(std::unique(want.begin(), want.end()), want.end());
+    if (want.front() < 0) return fail(FRHOT_EINVAL, "key %d must be non-negative", want.front());
+    frhot_ctx* c = g->ctx;
+    std::lock_guard<std::mutex> lk(c->mu);
+    DeviceGuard dg(c->device);
+    if (g->nrows == 0) return FRHOT_OK;
+    if (!g->key_tiles_off && !g->key_tiles_valid) {
+        const int rc = key_tiles_rebuild(g);
+        if (rc) return rc;
+    }
+    // only the tiles that may hold one of the keys are looked at (all of them once the lists were given up)
+    std::vector<int32_t> tiles;
+    const bool listed = !g->key_tiles_off;
+    if (listed) {
+        for (int32_t k : want) {
+            const auto it = g->key_tiles.find(k);
+            if (it != g->key_tiles.end()) tiles.insert(tiles.end(), it->second.begin(), it->second.end());
+        }
+        if (want.size() > 1) {
+            std::sort(tiles.begin(), tiles.end());
+            tiles.erase(std::unique(tiles.begin(), tiles.end()), tiles.end());
+        }
+        if (tiles.empty()) return FRHOT_OK;
+    }
+    const size_t nt = listed ? tiles.size() : (size_t)((g->nrows + 255) / 256);
+    IndexPin* ip = nullptr;
+    int rc = page_pin_take(c, nt + want.size() + (listed ? nt : 0), &ip);
+    if (rc) return rc;
+    int32_t *counts = ip->p, *wk = ip->p + nt, *tl = wk + want.size();
+    memcpy(wk, want.data(), want.size() * 4);
+    if (listed) memcpy(tl, tiles.data(), nt * 4);
+    HIP_TRY(launch_page_free(g->keys, listed ? tl : nullptr, (int)nt, wk, (int)want.size(), counts, c->stream));
+    rc = page_pin_mark(c, ip);
+    if (rc) return rc;
+    HIP_TRY(hipEventSynchronize(ip->copied));
+    ip->pending = false;
+    int64_t n = 0;
+    for (size_t i = 0; i < nt; ++i) n += counts[i];
+    if (n) g->dense = false;
+    if (listed)
+        for (int32_t k : want) {
+            const auto it = g->key_tiles.find(k);
+            if (it != g->key_tiles.end()) { g->key_tiles_entries -= it->second.size(); g->key_tiles.erase(it); }
+        }
+    if (freed) *freed = n;
+    return FRHOT_OK;
+    });
+}
+
+int frhot_gallery_compact(frhot_gallery* src, frhot_gallery* dst, int64_t* new_rows_dev, int64_t* live_out) {
+    return guarded([&]() -> int {
+    if (live_out) *live_out = 0;
+    if (!src) return fail(FRHOT_EINVAL, "gallery is null");
+    if (dst == src) dst = nullptr;
+    if (dst && dst->ctx != src->ctx) return fail(FRHOT_EINVAL, "the galleries belong to two contexts");
+    if (dst && dst->D != src->D) return fail(FRHOT_EINVAL, "rows of %d components do not fit a gallery of %d", src->D, dst->D);
+    if (new_rows_dev && (uintptr_t)new_rows_dev % 8) return fail(FRHOT_EINVAL, "new_rows is not aligned to its elements");
+    frhot_ctx* c = src->ctx;
+    std::lock_guard<std::mutex> lk(c->mu);
+    DeviceGuard dg(c->device);
+    hipStream_t s = c->stream;
+    frhot_gallery* g = dst ? dst : src;
+    int64_t live = 0;
+    if (src->nrows == 0) {
+        HIP_TRY(launch_page_kill(g->keys, 0, g->nrows, s));
+    } else {
+        const size_t ntiles = (size_t)((src->nrows + 255) / 256);
+        if (ntiles + 1 > c->page_off_cap) {
+            HIP_TRY(hipStreamSynchronize(s));
+            c->page_off_cap = 0;
+            HIP_TRY(free_null(c->page_off));
+            const size_t cap = ntiles + ntiles / 2 + 64;
+            HIP_TRY(hipMalloc((void**)&c->page_off, cap * 4));
+            c->page_off_cap = cap;
+        }
+        IndexPin* ip = nullptr;
+        int rc = page_pin_take(c, 16, &ip);
+        if (rc) return rc;
+        if (dst && dst->capacity < src->nrows) {
+            // the rows must fit, and only the device knows how many there are: count first
+            HIP_TRY(launch_page_count(src->keys, src->nrows, c->page_off, ip->p, s));
+            rc = page_pin_mark(c, ip);
+            if (rc) return rc;
+            HIP_TRY(hipEventSynchronize(ip->copied));
+            ip->pending = false;
+            if (ip->p[0] > dst->capacity)
+                return fail(FRHOT_ECAPACITY, "%d live rows, capacity %lld", ip->p[0], (long long)dst->capacity);
+        }
+        void* rows = g->rows;
+        int32_t* keys = g->keys;
+        int64_t old_rows = g->nrows;
+        if (!dst) {
+            // in place: into fresh buffers, which take the old ones' place once everything has landed
+            const size_t padded = ((size_t)src->capacity + 255) & ~(size_t)255;
+            rows = nullptr; keys = nullptr; old_rows = 0;
+            hipError_t e = hipMalloc(&rows, padded * src->D * 2);
+            if (e == hipSuccess) e = hipMalloc((void**)&keys, padded * 4);
+            if (e == hipSuccess) e = hipMemsetAsync(rows, 0, padded * src->D * 2, s);
+            if (e == hipSuccess) e = hipMemsetAsync(keys, 0xFF, padded * 4, s);
+            if (e != hipSuccess) {
+                if (rows) (void)hipFree(rows);
+                if (keys) (void)hipFree(keys);
+                return fail(FRHOT_ECAPACITY, "no room for a second copy of the gallery: %s", hipGetErrorString(e));
+            }
+        }
+        hipError_t e = launch_page_compact(src->rows, src->keys, src->nrows, rows, keys, old_rows, src->D, c->page_off, new_rows_dev, ip->p, s);
+        if (e == hipSuccess) e = hipEventRecord(ip->copied, s);
+        if (e == hipSuccess) e = hipEventSynchronize(ip->copied);
+        if (e != hipSuccess) {
+            if (!dst) { (void)hipFree(rows); (void)hipFree(keys); }
+            return fail(FRHOT_EHIP, "compacting failed: %s", hipGetErrorString(e));
+        }
+        live = ip->p[0];
+        if (!dst) {
+            (void)hipFree(src->rows);
+            (void)hipFree(src->keys);
+            src->rows = rows;
+            src->keys = keys;
+        }
+    }
+    g->nrows = live;
+    g->dense = true;
+    std::unordered_map<int32_t, std::vector<int32_t>>().swap(g->key_tiles);
+    g->key_tiles_entries = 0;
+    g->key_tiles_off = false;
+    g->key_tiles_valid = live == 0;     // (else read back from the keys when a by-key search next needs them)
+    if (live_out) *live_out = live;
+    return FRHOT_OK;
+    });
+}
+
+int frhot_gallery_reproject(frhot_gallery* src, frhot_head* h, frhot_gallery* dst) {
+    return guarded([&]() -> int {
+    if (!src || !h || !dst) return fail(FRHOT_EINVAL, "null argument");
+    if (src->ctx != h->ctx || dst->ctx != h->ctx) return fail(FRHOT_EINVAL, "galleries and head belong to different contexts");
+    if (src == dst) return fail(FRHOT_EINVAL, "a gallery cannot be reprojected into itself");
+    if (src->D != h->din || dst->D != h->dout)
+        return fail(FRHOT_EINVAL, "a head of %d -> %d between galleries of %d and %d", h->din, h->dout, src->D, dst->D);
+    frhot_ctx* c = h->ctx;
+    std::lock_guard<std::mutex> lk(c->mu);
+    if (dst->capacity < src->nrows) return fail(FRHOT_ECAPACITY, "%lld rows, capacity %lld", (long long)src->nrows, (long long)dst->capacity);
+    DeviceGuard dg(c->device);
+    if (src->nrows > 0) {
+        const int rc = head_enqueue(h, src->rows, 0, true, src->nrows, UnitOut{dst->rows, 0, 1, 0, src->keys, dst->keys});
+        if (rc) return rc;
+    }
+    HIP_TRY(launch_page_kill(dst->keys, src->nrows, dst->nrows, c->stream));
+    dst->nrows = src->nrows;
+    dst->dense = src->dense;
+    dst->key_tiles = src->key_tiles;
+    dst->key_tiles_entries = src->key_tiles_entries;
+    dst->key_tiles_off = src->key_tiles_off;
+    dst->key_tiles_valid = src->key_tiles_valid;
     return FRHOT_OK;
     });
 }

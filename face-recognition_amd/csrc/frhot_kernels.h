@@ -153,6 +153,59 @@ hipError_t launch_topk_final(const float* cand_s, const int64_t* cand_r, int nli
                              int64_t stride_s = 0, int64_t stride_r = 0);   // elements between consecutive lists' blocks
                                                                             // in cand_s / cand_r (0: Bq * kin, back to back)
 
+// ---- descriptor heads: matrix product with an epilogue, unit rows (frhot_linear.hip) ----
+enum { kF16 = 0, kF32 = 1, kBF16 = 2 };                                             // element types (FRHOT_F16 ...)
+enum { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActGeluTanh = 4 };  // activations (FRHOT_ACT_*)
+inline int linear_npad(int N) { return (N + 31) / 32 * 32; }    // rows / columns of the laid-out weights and of the bias
+inline int linear_kpad(int K) { return (K + 63) / 64 * 64; }
+struct LinearOut {
+    void* out; int64_t ldo; int otype;
+    const void* res; int64_t ldr; int rtype;        // residual added after the activation, or null
+    int act, N, vec_out, vec_res;                   // (N and vec_*: filled in by launch_linear)
+};
+struct LinearIn {
+    const void* x; int64_t ldx; size_t xtile; int tiled, xstep;
+    const void* wt; const float* bias; const void* zeros; float* slab;
+    int M, K, npad, panels, ksteps, ksteps_per_split, mtiles, ntiles, m_fast;
+};
+struct LinearCall {
+    const void* x; int64_t ldx;     // [M, K] fp16 or bf16 rows ldx elements apart; tiled: rows 0.. of a gallery of dimension K (x = a tile's start)
+    int tiled, bf16;
+    const void* wt; const float* bias;      // launch_linear_layout's result; linear_npad(N) floats
+    int64_t M; int N, K;
+    LinearOut out;
+};
+// Device scratch of the linear kernels.  Calls that use one such scratch must be ordered among themselves.
+struct LinearWork { float* slabs; size_t slab_bytes; void* pack; size_t pack_bytes; const void* zeros; };   // zeros: 128 bytes of 0
+size_t linear_layout_bytes(int N, int K);
+hipError_t launch_linear_layout(const void* w, void* wt, int N, int K, hipStream_t s);
+hipError_t launch_linear(const LinearCall& q, const LinearWork& ws, hipStream_t s);
+struct UnitOut {
+    void* out; int64_t ldo;         // fp16 rows, or
+    int gallery; int64_t row0;      // rows row0 .. of a gallery of dimension N whose rows start at `out`
+    const int32_t* keys_src; int32_t* keys_dst;     // gallery: keys copied beside the rows (or null)
+};
+hipError_t launch_unit_rows(const void* x, int type, int64_t ldx, int64_t M, int N, const UnitOut& o, hipStream_t s);
+hipError_t linear_kernels_init();
+
+// ---- pages of a gallery (frhot_pages.hip) ----
+constexpr int32_t kKeepKey = INT32_MIN;
+struct PageItem { int64_t src, dst; int32_t n, key; };     // n <= kPageRows rows src.. -> dst..; key: the new key or kKeepKey
+constexpr int kPageRows = 64;
+struct PageSide { void* rows; int32_t* keys; int dense; };  // a gallery's rows and keys, or a dense [n, D] buffer and its keys (or null)
+// `items` may lie in page-locked host memory (each is read once)
+hipError_t launch_page_move(const PageSide& src, const PageSide& dst, const PageItem* items, int n, int D, hipStream_t s);
+// Rows of the listed tiles (null: tiles 0 .. ntiles-1) whose key is one of keys[0..nkeys) (ascending) die; counts[i] = how many in tile i.
+hipError_t launch_page_free(int32_t* g_keys, const int32_t* tiles, int ntiles, const int32_t* keys, int nkeys, int32_t* counts, hipStream_t s);
+// Live rows of src to the front of dst in order; dst's rows behind them (up to dst_rows) die.  offsets: ntiles(src) + 1 int32 of
+// scratch, the last of which receives the number of live rows, as does *total.
+hipError_t launch_page_compact(const void* src, const int32_t* src_keys, int64_t src_rows, void* dst, int32_t* dst_keys, int64_t dst_rows,
+                               int D, int32_t* offsets, int64_t* new_rows, int32_t* total, hipStream_t s);
+hipError_t launch_page_count(const int32_t* g_keys, int64_t rows, int32_t* offsets, int32_t* total, hipStream_t s);     // the first half of it
+hipError_t launch_page_kill(int32_t* g_keys, int64_t lo, int64_t hi, hipStream_t s);
+// The first n rows behind a tile's start, in plain order (dense [n, D] fp16).
+hipError_t launch_page_rows(const void* tile_start, void* out, int64_t n, int D, hipStream_t s);
+
 // Sets the dynamic-LDS attributes and resolves the static scratch's address on the CURRENT device;
 // call once per device (repeat calls are cheap).
 hipError_t kernels_init();

@@ -1,0 +1,237 @@
+// HIP kernels that move, free and squeeze the rows of a gallery (gfx950).
+//
+// A gallery keeps its rows in tiles of 256 (its pages), inside a tile chunk by chunk of 64 components:
+//   component c of row r  ->  half index ((r / 256 * (D/64) + c / 64) * 256 + r % 256) * 64 + c % 64
+// so a run of rows is, per chunk, one contiguous run of 128-byte pieces.  All of these kernels are copies: what bounds them
+// is HBM (every moved byte is read once and written once), and each lane moves 16 bytes at a time, eight lanes a row's piece.
+#include <hip/hip_runtime.h>
+#include "frhot_kernels.h"
+
+namespace frhot {
+
+typedef unsigned uint4v __attribute__((ext_vector_type(4)));
+#define FR_DEV __device__ __forceinline__
+
+namespace {
+
+constexpr int32_t kDead = -1;
+
+// byte offset of chunk j of row r
+FR_DEV size_t tiled_at(int64_t r, int j, int nk) {
+    return ((((size_t)(r >> 8) * (size_t)nk + (size_t)j) << 8) + (size_t)(r & 255)) * 128;
+}
+template <bool DENSE>
+FR_DEV size_t piece_at(int64_t r, int j, int nk) {
+    if constexpr (DENSE) return ((size_t)r * nk + j) * 128;
+    return tiled_at(r, j, nk);
+}
+
+FR_DEV int ceil_log2(int n) { return n <= 1 ? 0 : 32 - __builtin_clz((unsigned)(n - 1)); }
+
+// One item (a run of up to 64 rows) and `per` chunks of it per block; the pieces are taken chunk by chunk, rows fastest, a
+// power of two of row slots per chunk so that no index needs a division.
+template <bool SD, bool DD>
+__global__ __launch_bounds__(256) void page_move_kernel(PageSide src, PageSide dst, const PageItem* __restrict__ items, int nk, int per) {
+    const PageItem it = items[blockIdx.x];
+    const int j0 = blockIdx.y * per, j1 = min(nk, j0 + per);
+    const int lg = ceil_log2(it.n), mask = (1 << lg) - 1;
+    const int total = (j1 - j0) << (lg + 3);
+    const int part = (threadIdx.x & 7) * 16;
+    constexpr int U = 4;
+    for (int base = threadIdx.x; base < total; base += 256 * U) {
+        uint4v v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int idx = base + 256 * u;
+            const int i = (idx >> 3) & mask, j = j0 + (idx >> (lg + 3));
+            if (idx < total && i < it.n) v[u] = *(const uint4v*)((const char*)src.rows + piece_at<SD>(it.src + i, j, nk) + part);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int idx = base + 256 * u;
+            const int i = (idx >> 3) & mask, j = j0 + (idx >> (lg + 3));
+            if (idx < total && i < it.n) *(uint4v*)((char*)dst.rows + piece_at<DD>(it.dst + i, j, nk) + part) = v[u];
+        }
+    }
+    if (blockIdx.y == 0 && dst.keys && (int)threadIdx.x < it.n)
+        dst.keys[it.dst + threadIdx.x] = it.key == kKeepKey ? src.keys[it.src + threadIdx.x] : it.key;
+}
+
+__global__ __launch_bounds__(256) void page_free_kernel(int32_t* __restrict__ gk, const int32_t* __restrict__ tiles,
+                                                        const int32_t* __restrict__ keys, int nkeys, int32_t* __restrict__ counts) {
+    __shared__ int red[4];
+    const int64_t r = (int64_t)(tiles ? tiles[blockIdx.x] : (int)blockIdx.x) * 256 + threadIdx.x;
+    const int32_t k = gk[r];
+    int lo = 0, hi = nkeys;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (keys[mid] < k) lo = mid + 1; else hi = mid;
+    }
+    const bool hit = lo < nkeys && keys[lo] == k;
+    if (hit) gk[r] = kDead;
+    const int c = __popcll(__ballot(hit));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = c;
+    __syncthreads();
+    if (threadIdx.x == 0) counts[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+
+// live rows of every tile; a wave takes one tile
+__global__ __launch_bounds__(256) void page_count_kernel(const int32_t* __restrict__ gk, int64_t rows, int ntiles, int32_t* __restrict__ counts) {
+    const int t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (t >= ntiles) return;
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t r = (int64_t)t * 256 + i * 64 + lane;
+        c += __popcll(__ballot(r < rows && gk[r < rows ? r : 0] >= 0));
+    }
+    if (lane == 0) counts[t] = c;
+}
+
+// counts -> exclusive sums in place, the whole in offsets[n] and *total; one block
+__global__ __launch_bounds__(1024) void page_scan_kernel(int32_t* __restrict__ offsets, int n, int32_t* __restrict__ total) {
+    __shared__ int wsum[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int carry = 0;
+    for (int base = 0; base < n; base += 1024) {
+        const int i = base + tid;
+        const int c = i < n ? offsets[i] : 0;
+        int v = c;
+#pragma unroll
+        for (int s = 1; s < 64; s <<= 1) {
+            const int u = __shfl_up(v, s);
+            if (lane >= s) v += u;
+        }
+        if (lane == 63) wsum[wave] = v;
+        __syncthreads();
+        int before = 0, all = 0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            before += w < wave ? wsum[w] : 0;
+            all += wsum[w];
+        }
+        if (i < n) offsets[i] = carry + before + v - c;
+        carry += all;
+        __syncthreads();
+    }
+    if (tid == 0) { offsets[n] = carry; *total = carry; }
+}
+
+// One tile of the source and `per` chunks of it per block: its live rows, in order, go to dst rows offsets[tile] and up.
+__global__ __launch_bounds__(256) void page_compact_kernel(const char* __restrict__ src, const int32_t* __restrict__ sk, int64_t src_rows, int ntiles,
+                                                           char* __restrict__ dst, int32_t* __restrict__ dk, int64_t dst_rows, int nk,
+                                                           int per, const int32_t* __restrict__ offsets, int64_t* __restrict__ new_rows) {
+    __shared__ unsigned char list[256];
+    __shared__ int wcnt[4];
+    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t r = (int64_t)t * 256 + tid;
+    const int live_all = offsets[ntiles];
+    if (blockIdx.y == 0 && r >= live_all && r < dst_rows) dk[r] = kDead;        // what the squeezed rows left behind
+    if (t >= ntiles) return;
+    const int32_t key = r < src_rows ? sk[r] : kDead;
+    const unsigned long long b = __ballot(key >= 0);
+    if (lane == 0) wcnt[wave] = __popcll(b);
+    __syncthreads();
+    int rank = __popcll(b & ((1ull << lane) - 1)), live = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        rank += w < wave ? wcnt[w] : 0;
+        live += wcnt[w];
+    }
+    const int64_t first = offsets[t];
+    if (key >= 0) list[rank] = (unsigned char)tid;
+    if (blockIdx.y == 0) {
+        if (key >= 0) dk[first + rank] = key;
+        if (new_rows && r < src_rows) new_rows[r] = key >= 0 ? first + rank : -1;
+    }
+    __syncthreads();
+    if (live == 0) return;
+    const int j0 = blockIdx.y * per, j1 = min(nk, j0 + per);
+    const int lg = ceil_log2(live), mask = (1 << lg) - 1;
+    const int total = (j1 - j0) << (lg + 3);
+    const int part = (tid & 7) * 16;
+    constexpr int U = 4;
+    for (int base = tid; base < total; base += 256 * U) {
+        uint4v v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int idx = base + 256 * u;
+            const int i = (idx >> 3) & mask, j = j0 + (idx >> (lg + 3));
+            if (idx < total && i < live) v[u] = *(const uint4v*)(src + tiled_at((int64_t)t * 256 + list[i], j, nk) + part);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int idx = base + 256 * u;
+            const int i = (idx >> 3) & mask, j = j0 + (idx >> (lg + 3));
+            if (idx < total && i < live) *(uint4v*)(dst + tiled_at(first + i, j, nk) + part) = v[u];
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void page_rows_kernel(const char* __restrict__ src, char* __restrict__ out, size_t pieces, int nk) {
+    const size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;       // 16 bytes: piece t >> 3 of the output = chunk j of row r
+    if (t >= pieces * 8) return;
+    const int64_t r = (int64_t)((t >> 3) / (unsigned)nk);
+    const int j = (int)((t >> 3) % (unsigned)nk);
+    *(uint4v*)(out + t * 16) = *(const uint4v*)(src + tiled_at(r, j, nk) + (t & 7) * 16);
+}
+
+__global__ __launch_bounds__(256) void page_kill_kernel(int32_t* __restrict__ gk, int64_t lo, int64_t hi) {
+    const int64_t r = lo + (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (r < hi) gk[r] = kDead;
+}
+
+}  // namespace
+
+hipError_t launch_page_move(const PageSide& src, const PageSide& dst, const PageItem* items, int n, int D, hipStream_t s) {
+    if (!src.rows || !dst.rows || !items || n <= 0 || D <= 0 || D % 64 || (src.dense && dst.dense)) return hipErrorInvalidValue;
+    const int nk = D / 64, per = 8;
+    const dim3 grid((unsigned)n, (unsigned)((nk + per - 1) / per));
+    if (src.dense) hipLaunchKernelGGL((page_move_kernel<true, false>), grid, dim3(256), 0, s, src, dst, items, nk, per);
+    else if (dst.dense) hipLaunchKernelGGL((page_move_kernel<false, true>), grid, dim3(256), 0, s, src, dst, items, nk, per);
+    else hipLaunchKernelGGL((page_move_kernel<false, false>), grid, dim3(256), 0, s, src, dst, items, nk, per);
+    return hipGetLastError();
+}
+
+hipError_t launch_page_free(int32_t* gk, const int32_t* tiles, int ntiles, const int32_t* keys, int nkeys, int32_t* counts, hipStream_t s) {
+    if (!gk || !keys || !counts || ntiles <= 0 || nkeys <= 0) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(page_free_kernel, dim3((unsigned)ntiles), dim3(256), 0, s, gk, tiles, keys, nkeys, counts);
+    return hipGetLastError();
+}
+
+hipError_t launch_page_count(const int32_t* gk, int64_t rows, int32_t* offsets, int32_t* total, hipStream_t s) {
+    if (!gk || !offsets || !total || rows <= 0) return hipErrorInvalidValue;
+    const int ntiles = (int)((rows + 255) / 256);
+    hipLaunchKernelGGL(page_count_kernel, dim3((unsigned)((ntiles + 3) / 4)), dim3(256), 0, s, gk, rows, ntiles, offsets);
+    hipLaunchKernelGGL(page_scan_kernel, dim3(1), dim3(1024), 0, s, offsets, ntiles, total);
+    return hipGetLastError();
+}
+
+hipError_t launch_page_compact(const void* src, const int32_t* sk, int64_t src_rows, void* dst, int32_t* dk, int64_t dst_rows, int D,
+                               int32_t* offsets, int64_t* new_rows, int32_t* total, hipStream_t s) {
+    if (!src || !sk || !dst || !dk || !offsets || !total || src_rows <= 0 || D <= 0 || D % 64) return hipErrorInvalidValue;
+    const int ntiles = (int)((src_rows + 255) / 256), dtiles = (int)((dst_rows + 255) / 256), nk = D / 64, per = 2;
+    const hipError_t e = launch_page_count(sk, src_rows, offsets, total, s);
+    if (e != hipSuccess) return e;
+    const dim3 grid((unsigned)(ntiles > dtiles ? ntiles : dtiles), (unsigned)((nk + per - 1) / per));
+    hipLaunchKernelGGL(page_compact_kernel, grid, dim3(256), 0, s, (const char*)src, sk, src_rows, ntiles, (char*)dst, dk, dst_rows, nk, per,
+                       (const int32_t*)offsets, new_rows);
+    return hipGetLastError();
+}
+
+hipError_t launch_page_rows(const void* tile_start, void* out, int64_t n, int D, hipStream_t s) {
+    if (!tile_start || !out || n <= 0 || D <= 0 || D % 64) return hipErrorInvalidValue;
+    const size_t pieces = (size_t)n * (D / 64);
+    hipLaunchKernelGGL(page_rows_kernel, dim3((unsigned)((pieces * 8 + 255) / 256)), dim3(256), 0, s, (const char*)tile_start, (char*)out,
+                       pieces, D / 64);
+    return hipGetLastError();
+}
+
+hipError_t launch_page_kill(int32_t* gk, int64_t lo, int64_t hi, hipStream_t s) {
+    if (!gk || lo < 0) return hipErrorInvalidValue;
+    if (hi <= lo) return hipSuccess;
+    hipLaunchKernelGGL(page_kill_kernel, dim3((unsigned)((hi - lo + 255) / 256)), dim3(256), 0, s, gk, lo, hi);
+    return hipGetLastError();
+}
+
+}  // namespace frhot

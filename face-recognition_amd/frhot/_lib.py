@@ -16,6 +16,8 @@ OK, EINVAL, EHIP, ESTATE, ECAPACITY = 0, -1, -2, -3, -4
 EMBED_DIM = 4096
 FLAG_GAMMA, FLAG_NOFLIP = 1, 2
 KEY_ANY, KEY_DEAD = -2, -1
+DTYPES = {"f16": 0, "f32": 1, "bf16": 2}
+ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
 _p = C.c_void_p
 _i32p = C.POINTER(C.c_int32)
@@ -63,6 +65,20 @@ SIGNATURES = {
     "frhot_crop_sharpness_dev": (C.c_int, [_p, _p, _i64p, _i32p, _i32p, C.c_int, _p]),
     "frhot_recognise_gated": (C.c_int, [_p, _p, _u8pp, _i32p, _i32p, _i32p, C.c_int, C.c_uint, C.c_int,
                                         _f32p, _f32p, _i64p, _i64p]),
+    "frhot_linear_create": (C.c_int, [_p, _p, _p, C.c_int, C.c_int, C.c_int, C.POINTER(_p)]),
+    "frhot_linear_destroy": (C.c_int, [_p]),
+    "frhot_linear_dev": (C.c_int, [_p, _p, C.c_int64, C.c_int64, C.c_int, _p, C.c_int64, C.c_int, _p, C.c_int64, C.c_int]),
+    "frhot_unit_rows_dev": (C.c_int, [_p, _p, C.c_int, C.c_int64, C.c_int64, C.c_int, _p, C.c_int64]),
+    "frhot_head_create": (C.c_int, [_p, C.POINTER(_p), _i32p, _i32p, C.c_int, C.POINTER(_p)]),
+    "frhot_head_destroy": (C.c_int, [_p]),
+    "frhot_head_dev": (C.c_int, [_p, _p, C.c_int64, C.c_int64, _p, C.c_int64]),
+    "frhot_ctx_head": (C.c_int, [_p, _p]),
+    "frhot_gallery_copy": (C.c_int, [_p, _p, _p, _p, _p, _p, C.c_int]),
+    "frhot_gallery_read_dev": (C.c_int, [_p, _p, _p, C.c_int, _p, _p]),
+    "frhot_gallery_write_dev": (C.c_int, [_p, _p, _p, _p, _p, C.c_int]),
+    "frhot_gallery_free_keys": (C.c_int, [_p, _p, C.c_int, _i64p]),
+    "frhot_gallery_compact": (C.c_int, [_p, _p, _p, _i64p]),
+    "frhot_gallery_reproject": (C.c_int, [_p, _p, _p]),
     "frhot_ctx_timing": (C.c_int, [_p, C.c_int]),
     "frhot_ctx_stage_ms": (C.c_int, [_p, _f32p]),
 }

@@ -1,4 +1,4 @@
-"""Python handles over the C ABI: Context (model + embed pipeline) and Gallery.
+"""Python handles over the C ABI: Context (model + embed pipeline), Linear / Head (descriptor heads) and Gallery.
 
 Thin by design: argument marshalling and error translation only.  All
 arithmetic happens in libfrhot.so on the GPU.
@@ -10,7 +10,7 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from ._lib import EMBED_DIM, FLAG_GAMMA, FLAG_NOFLIP, KEY_ANY, check
+from ._lib import ACTS, DTYPES, EMBED_DIM, FLAG_GAMMA, FLAG_NOFLIP, KEY_ANY, check
 
 
 def _ptr(a: np.ndarray, ctype):
@@ -61,6 +61,7 @@ class Context:
         self.device = device
         self.max_batch = max_batch
         self._blob = None
+        self._head = None
 
     def close(self):
         if getattr(self, "_h", None) and self._h.value:
@@ -231,6 +232,146 @@ class Context:
         return laplacian_variance(self.crop_sharpness_sums(images), hw)
 
 
+    def unit_rows_dev(self, x_dev: int, m: int, n: int, out_f16_dev: int, dtype: str = "f32", ldx: int | None = None,
+                      ldo: int | None = None):
+        """Rows [m, n] of `dtype` (device) -> unit fp16 rows: what a gallery stores and a search takes.  Enqueues only."""
+        check(self._lib.frhot_unit_rows_dev(self._h, x_dev, _code(DTYPES, dtype, "type"), n if ldx is None else ldx, m, n, out_f16_dev,
+                                            n if ldo is None else ldo))
+
+    def set_head(self, head: "Head | None"):
+        """Queries of head.dout components (embed_dev's dq, recognise on a gallery of that dimension) come from
+        `head` instead of the descriptor's leading components; None: as before."""
+        check(self._lib.frhot_ctx_head(self._h, head.handle if head is not None else None))
+        self._head = head
+
+
+def _code(table, name, what):
+    try:
+        return table[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"{what} {name!r} is not one of {sorted(table)}") from None
+
+
+def bf16_bits(a: np.ndarray) -> np.ndarray:
+    """float array -> uint16 bfloat16 bit patterns, rounded to nearest even (NaN stays a quiet NaN)."""
+    u = np.ascontiguousarray(a, dtype=np.float32).view(np.uint32)
+    r = ((u + 0x7FFF + ((u >> 16) & 1)) >> 16).astype(np.uint16)
+    return np.where((u & 0x7FFFFFFF) > 0x7F800000, ((u >> 16) | 0x40).astype(np.uint16), r)
+
+
+class Linear:
+    """One layer of a descriptor head (frhot_linear): weights [N, K] on the device in the kernels' own order."""
+
+    def __init__(self, ctx: Context, weight: np.ndarray, bias: np.ndarray | None = None, dtype: str = "f16"):
+        """weight: [N, K] floats, rounded to `dtype` ("f16" or "bf16"); uint16 arrays are taken as the bit
+        patterns themselves.  bias: [N] float32 or None."""
+        self._lib = ctx._lib
+        self.ctx = ctx
+        self._h = C.c_void_p()
+        w = np.asarray(weight)
+        if w.ndim != 2:
+            raise ValueError("weight must be [N, K]")
+        if w.dtype != np.uint16:
+            if dtype == "f16":
+                with np.errstate(over="ignore"):
+                    w = w.astype(np.float16)
+            else:
+                w = bf16_bits(w)
+        w = np.ascontiguousarray(w)
+        self.n, self.k = w.shape
+        b = None if bias is None else np.ascontiguousarray(bias, dtype=np.float32)
+        if b is not None and b.shape != (self.n,):
+            raise ValueError(f"bias of shape {b.shape} for {self.n} outputs")
+        check(self._lib.frhot_linear_create(ctx.handle, w.ctypes.data, b.ctypes.data if b is not None else None, self.n, self.k,
+                                            _code(DTYPES, dtype, "type"), C.byref(self._h)))
+        self.dtype = dtype
+
+    def close(self):
+        if getattr(self, "_h", None) and self._h.value and self.ctx.handle.value:
+            check(self._lib.frhot_linear_destroy(self._h))
+        self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    @property
+    def handle(self):
+        return self._h
+
+    def run_dev(self, x_dev: int, m: int, out_dev: int, act: str = "none", residual_dev: int | None = None, ldx: int | None = None,
+                ldr: int | None = None, ldo: int | None = None, out_dtype: str = "f16", residual_dtype: str = "f16"):
+        """out [m, N] = act(x [m, K] W^T + bias) + residual, all device memory; enqueues only."""
+        n = self.n
+        rc = self._lib.frhot_linear_dev(self._h, x_dev, self.k if ldx is None else ldx, m, _code(ACTS, act, "activation"), residual_dev,
+                                        n if ldr is None else ldr, _code(DTYPES, residual_dtype, "type"), out_dev,
+                                        n if ldo is None else ldo, _code(DTYPES, out_dtype, "type"))
+        if rc:
+            check(rc)
+
+
+class Head:
+    """Layers between the descriptor and the gallery (frhot_head): [(Linear, activation, add its input?), ...];
+    the last layer's rows come out with unit length."""
+
+    def __init__(self, ctx: Context, layers):
+        self._lib = ctx._lib
+        self.ctx = ctx
+        self._h = C.c_void_p()
+        self.layers = [(lin, act, bool(res)) for lin, act, res in layers]       # (keeps the layers alive)
+        n = len(self.layers)
+        handles = (C.c_void_p * max(n, 1))(*[lin.handle.value for lin, _, _ in self.layers])
+        acts = np.array([_code(ACTS, a, "activation") for _, a, _ in self.layers], dtype=np.int32)
+        res = np.array([r for _, _, r in self.layers], dtype=np.int32)
+        check(self._lib.frhot_head_create(ctx.handle, handles, _ptr(acts, C.c_int32), _ptr(res, C.c_int32), n, C.byref(self._h)))
+        self.din, self.dout = self.layers[0][0].k, self.layers[-1][0].n
+
+    def close(self):
+        if getattr(self, "_h", None) and self._h.value and self.ctx.handle.value:
+            check(self._lib.frhot_head_destroy(self._h))
+        self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    @property
+    def handle(self):
+        return self._h
+
+    def run_dev(self, x_f16_dev: int, m: int, out_f16_dev: int, ldx: int | None = None, ldo: int | None = None):
+        """fp16 rows [m, din] -> unit fp16 rows [m, dout] (device); enqueues only."""
+        check(self._lib.frhot_head_dev(self._h, x_f16_dev, self.din if ldx is None else ldx, m, out_f16_dev,
+                                       self.dout if ldo is None else ldo))
+
+
+def _runs(rows, counts, keys=None):
+    """Run lists as the ABI takes them; keys: one for all, one per run, or None."""
+    rows = np.ascontiguousarray(rows, dtype=np.int64).reshape(-1)
+    if counts is not None:
+        counts = np.ascontiguousarray(counts, dtype=np.int32).reshape(-1)
+        if counts.size != rows.size:
+            raise ValueError(f"{counts.size} run lengths for {rows.size} runs")
+    if keys is not None:
+        keys = np.ascontiguousarray(np.broadcast_to(np.asarray(keys, dtype=np.int32), rows.shape))
+    return rows, counts, keys
+
+
+def _at(a):
+    return None if a is None else a.ctypes.data
+
+
+def runs_of(rows):
+    """Row numbers in the order given -> (first rows, run lengths) of their ascending consecutive runs."""
+    rows = np.ascontiguousarray(rows, dtype=np.int64).reshape(-1)
+    edge = np.flatnonzero(np.concatenate([[True], np.diff(rows) != 1])) if rows.size else np.empty(0, np.int64)
+    return rows[edge], np.diff(np.concatenate([edge, [rows.size]])).astype(np.int32)
+
+
 class Gallery:
     """Device-resident [capacity, D] fp16 unit rows + int32 keys (frhot_gallery)."""
 
@@ -343,5 +484,44 @@ class Gallery:
                                                  C.c_void_p(qkeys_local_dev or 0), b, k, C.c_void_p(scores_dev),
                                                  C.c_void_p(rows_dev), row_base))
 
+    # Pages: runs of rows moved on the device (see frhot_gallery_copy).  counts None: every entry is one row.
+    def copy(self, src_rows, dst_rows, counts=None, keys=None, source: "Gallery | None" = None):
+        """Rows of `source` (this gallery by default) to rows of this one, under `keys` (one, or one per run)
+        or with their own.  Enqueues only."""
+        src_rows, counts, _ = _runs(src_rows, counts)
+        dst_rows, _, keys = _runs(dst_rows, None, keys)
+        if dst_rows.size != src_rows.size:
+            raise ValueError(f"{src_rows.size} source runs, {dst_rows.size} destinations")
+        src = self if source is None else source
+        check(self._lib.frhot_gallery_copy(src._h, src_rows.ctypes.data, self._h, dst_rows.ctypes.data, _at(counts), _at(keys), src_rows.size))
 
-__all__ = ["Context", "Gallery", "EMBED_DIM", "KEY_ANY"]
+    def read_dev(self, rows, counts, out_f16_dev: int, out_keys_dev: int | None = None):
+        """The runs back to back as dense fp16 rows [n, D] and int32 keys, in device memory.  Enqueues only."""
+        rows, counts, _ = _runs(rows, counts)
+        check(self._lib.frhot_gallery_read_dev(self._h, rows.ctypes.data, _at(counts), rows.size, out_f16_dev, out_keys_dev))
+
+    def write_dev(self, rows_f16_dev: int, rows, counts, keys):
+        """Dense unit fp16 rows (device) to the runs, one key per run.  Enqueues only."""
+        rows, counts, keys = _runs(rows, counts, keys)
+        check(self._lib.frhot_gallery_write_dev(self._h, rows_f16_dev, rows.ctypes.data, _at(counts), keys.ctypes.data, rows.size))
+
+    def free_keys(self, keys) -> int:
+        """Every row under one of the keys dies; returns how many did."""
+        keys = np.ascontiguousarray(keys, dtype=np.int32).reshape(-1)
+        freed = C.c_int64()
+        check(self._lib.frhot_gallery_free_keys(self._h, keys.ctypes.data, keys.size, C.byref(freed)))
+        return freed.value
+
+    def compact(self, into: "Gallery | None" = None, new_rows_dev: int | None = None) -> int:
+        """Live rows, in order, to the front of `into` (default: of this gallery); returns their number.
+        new_rows_dev: int64 [rows], every row's new place or -1."""
+        live = C.c_int64()
+        check(self._lib.frhot_gallery_compact(self._h, into._h if into is not None else None, new_rows_dev, C.byref(live)))
+        return live.value
+
+    def reproject(self, head: Head, into: "Gallery"):
+        """Row r of `into` becomes the head's output for row r of this gallery, key included.  Enqueues only."""
+        check(self._lib.frhot_gallery_reproject(self._h, head.handle, into._h))
+
+
+__all__ = ["Context", "Gallery", "Head", "Linear", "EMBED_DIM", "KEY_ANY"]

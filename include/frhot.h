@@ -45,8 +45,22 @@ extern "C" {
 #define FRHOT_KEY_ANY       (-2)  /* query matches every live row */
 #define FRHOT_KEY_DEAD      (-1)  /* row key of a tombstoned row; as a query key it matches nothing */
 
+/* element types of device buffers */
+#define FRHOT_F16           0
+#define FRHOT_F32           1
+#define FRHOT_BF16          2
+
+/* activations of a layer */
+#define FRHOT_ACT_NONE      0
+#define FRHOT_ACT_RELU      1     /* max(v, 0); NaN stays NaN */
+#define FRHOT_ACT_SILU      2     /* v / (1 + exp(-v)) */
+#define FRHOT_ACT_GELU      3     /* v erfc(-v / sqrt 2) / 2 */
+#define FRHOT_ACT_GELU_TANH 4     /* v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2 */
+
 typedef struct frhot_ctx frhot_ctx;
 typedef struct frhot_gallery frhot_gallery;
+typedef struct frhot_linear frhot_linear;
+typedef struct frhot_head frhot_head;
 
 /* Message of the last failing call on this thread ("" if none). */
 const char* frhot_last_error(void);
@@ -372,6 +386,85 @@ int frhot_recognise_gated(frhot_ctx* ctx, frhot_gallery* g, const uint8_t* const
  */
 int frhot_ctx_timing(frhot_ctx* ctx, int enable);
 int frhot_ctx_stage_ms(frhot_ctx* ctx, float* ms5);
+
+/*
+ * Descriptor heads: learned projections between the descriptor and the gallery.  No counterpart in
+ * the reference, which compares whole 4096-component descriptors (qdrant_database_FE/app.py:116);
+ * without a head a gallery of fewer components takes the descriptor's leading ones.
+ *
+ * frhot_linear_create: one layer, w [N,K] row-major fp16 or bf16 (`dtype`) and bias [N] float32 or NULL,
+ *   host memory; the weights are laid out for the matrix instructions once, here.  N, K in 1..65536.
+ *   The first layer of a context also allocates the context's 98 MiB of scratch for these calls.
+ *   Destroying a layer that a head still holds is refused (FRHOT_ESTATE).
+ * frhot_linear_dev: out[m][n] = round(act(sum_k x[m][k] w[n][k] + bias[n]) + residual[m][n]), products
+ *   summed in fp32, rounded once.  x [M,K] of the layer's type, residual [M,N] (or NULL) and out [M,N]
+ *   of the given types; ldx / ldr / ldo elements from row to row, any alignment that their elements
+ *   have (rows that 16-byte loads cannot take, i.e. K or ldx not a multiple of 8 or x not 16-byte
+ *   aligned, cost an extra pass).  Nothing beyond out's N columns and M rows is written, nothing
+ *   beyond K columns read.  out may be the residual itself (same address, row distance and element
+ *   size) and may not overlap x or the residual otherwise.  M = 0 does nothing.
+ * frhot_unit_rows_dev: out[m] = fp16(x[m] / |x[m]|), x [M,N] of any type: norm and rounding as
+ *   frhot_gallery_upsert applies them (64-bit sum of squares, float32 norm; rows shorter than 1e-30
+ *   are divided by one).  out may not overlap x.
+ * frhot_head_create: n layers (1..16, fp16, each taking what the one before gives) with their
+ *   activations and, where residuals[i] != 0, the layer's own input added to its output (residuals
+ *   may be NULL); the last layer's rows are brought to unit length.  First input and last output are
+ *   multiples of 64.  Inner layers round to fp16, the last one's output stays fp32 up to the norm.
+ *   The layers stay the caller's and must outlive the head.
+ * frhot_head_dev: fp16 rows x [M,din] -> unit fp16 rows out [M,dout].
+ * frhot_ctx_head: attach (or, NULL, detach) a head of 4096 inputs: frhot_embed_dev with Dq equal to
+ *   its outputs and frhot_recognise* on a gallery of that dimension then use the head's rows as
+ *   queries, where they take the descriptor's leading components otherwise.  Destroying an attached
+ *   head detaches it.
+ * All *_dev calls enqueue on the context's stream and return.  They share the context's scratch:
+ * graphs captured from one context's calls must not be replayed at the same time.
+ */
+int frhot_linear_create(frhot_ctx* ctx, const void* w, const float* bias, int N, int K, int dtype, frhot_linear** out);
+int frhot_linear_destroy(frhot_linear* layer);
+int frhot_linear_dev(frhot_linear* layer, const void* x_dev, int64_t ldx, int64_t M, int act, const void* residual_dev, int64_t ldr,
+                     int residual_dtype, void* out_dev, int64_t ldo, int out_dtype);
+int frhot_unit_rows_dev(frhot_ctx* ctx, const void* x_dev, int dtype, int64_t ldx, int64_t M, int N, void* out_f16_dev, int64_t ldo);
+int frhot_head_create(frhot_ctx* ctx, frhot_linear* const* layers, const int32_t* acts, const int32_t* residuals, int n,
+                      frhot_head** out);
+int frhot_head_destroy(frhot_head* head);
+int frhot_head_dev(frhot_head* head, const void* x_f16_dev, int64_t ldx, int64_t M, void* out_f16_dev, int64_t ldo);
+int frhot_ctx_head(frhot_ctx* ctx, frhot_head* head);
+
+/*
+ * Pages of a gallery: copying, forking, squeezing and freeing rows without a trip through host
+ * memory.  Rows are given as runs: run i is rows first[i] .. first[i] + counts[i] - 1 (counts NULL:
+ * one row each).  Row lists are host memory and checked before anything is enqueued: a run outside
+ * the capacity is FRHOT_ECAPACITY; an empty run, a destination row named twice, or a row that one
+ * frhot_gallery_copy call both reads and writes is FRHOT_EINVAL; on a stream under graph capture they
+ * are FRHOT_ESTATE.  Searches enqueued afterwards see the change.
+ *
+ * frhot_gallery_copy: rows of src to rows of dst (the same gallery or another one of the same
+ *   dimension and context) under keys[i] per run (>= 0), or with the rows' own keys (keys NULL; dead rows
+ *   stay dead).  With new keys this forks a collection.  Replaces: what a create_snapshot +
+ *   recover_snapshot pair does through files (qdrant_database_FE/app.py:131-196).  Enqueues only.
+ * frhot_gallery_read_dev / _write_dev: the runs back to back as dense fp16 [n,D] device rows (16-byte
+ *   aligned) and their keys (device, or NULL), and the way back with one key per run (FRHOT_KEY_DEAD
+ *   allowed): frhot_gallery_read / _write_f16 without the host.  Enqueue only.
+ * frhot_gallery_free_keys: every row whose key is among keys[0..nkeys) dies; *freed (may be NULL) =
+ *   how many did.  Replaces: dropping a collection (test/delete_collection.py).  Waits.
+ * frhot_gallery_compact (what Qdrant's own optimiser does to deleted points): the live rows, in their order, become rows 0, 1, 2 ... of dst, whose
+ *   previous content is gone, or of the gallery itself (dst NULL or src: needs room for a second copy
+ *   while it runs); new_rows_dev, if not NULL, receives every old row's new place (int64 [rows of src],
+ *   device; -1 for dead ones) and *live (may be NULL) their number.  Scores of a search stay what they were,
+ *   and so does the order of equal scores.  Waits.
+ * frhot_gallery_reproject: row r of dst becomes the head's output for row r of src, with its key
+ *   (dead rows stay dead; dst's previous content is gone).  How an enrolled gallery moves to a head:
+ *   src holds descriptors (or another head's rows), dst has the head's output dimension.  Enqueues only.
+ */
+int frhot_gallery_copy(frhot_gallery* src, const int64_t* src_rows, frhot_gallery* dst, const int64_t* dst_rows,
+                       const int32_t* counts, const int32_t* keys, int nruns);
+int frhot_gallery_read_dev(frhot_gallery* g, const int64_t* rows, const int32_t* counts, int nruns, void* out_f16_dev,
+                           int32_t* out_keys_dev);
+int frhot_gallery_write_dev(frhot_gallery* g, const void* rows_f16_dev, const int64_t* rows, const int32_t* counts,
+                            const int32_t* keys, int nruns);
+int frhot_gallery_free_keys(frhot_gallery* g, const int32_t* keys, int nkeys, int64_t* freed);
+int frhot_gallery_compact(frhot_gallery* src, frhot_gallery* dst, int64_t* new_rows_dev, int64_t* live);
+int frhot_gallery_reproject(frhot_gallery* src, frhot_head* head, frhot_gallery* dst);
 
 #ifdef __cplusplus
 }
