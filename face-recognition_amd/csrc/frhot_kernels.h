@@ -166,7 +166,7 @@ struct LinearOut {
 struct LinearIn {
     const void* x; int64_t ldx; size_t xtile; int tiled, xstep;
     const void* wt; const float* bias; const void* zeros; float* slab;
-    int M, K, npad, panels, ksteps, ksteps_per_split, mtiles, ntiles, m_fast;
+    int M, K, npad, panels, ksteps, ksteps_per_split, splits, mtiles, ntiles, m_fast;
 };
 struct LinearCall {
     const void* x; int64_t ldx;     // [M, K] fp16 or bf16 rows ldx elements apart; tiled: rows 0.. of a gallery of dimension K (x = a tile's start)

@@ -6,7 +6,8 @@
 //
 // Weights are laid out once, when a layer is created, in the order the matrix instruction takes them:
 //   fragment (p, s) = 1 KiB holding, for lane l and e = 0..7, w[chan(p, l & 15)][32 s + 8 (l >> 4) + e],
-//   fragments of one panel p of 16 channels back to back over s, zeros beyond N and K.
+//   the two fragments of a 64-deep step back to back, then the next panel of 16 channels, then the next step: what a tile
+//   reads for one step is one contiguous piece, and the tiles of a launch spread over all memory channels.  Zeros beyond N and K.
 // A pair of panels 2u, 2u+1 covers 32 channels, interleaved so that the accumulators of the pair give every
 // lane 8 CONSECUTIVE channels (16-byte fp16 stores):  chan(2u + c, 4 g + j) = 32 u + 8 g + 4 c + j.
 #include <hip/hip_runtime.h>
@@ -58,67 +59,88 @@ FR_DEV void store1(void* p, size_t i, int type, float v) {
 
 // The activation in fp32.  Written so that each keeps its relative accuracy far out (gelu through erfc, the tanh form
 // through its logistic equivalent) and NaN stays NaN (a maximum with zero would turn it into zero).
-FR_DEV float activate(float v, int act) {
-    switch (act) {
-        case kActRelu: return v < 0.f ? 0.f : v;
-        case kActSilu: return v / (1.f + expf(-v));
-        case kActGelu: return 0.5f * v * erfcf(v * -0.70710678118654752f);
-        case kActGeluTanh: return v / (1.f + expf(-1.5957691216057308f * (v + 0.044715f * v * v * v)));
-        default: return v;
+template <int W>
+FR_DEV void activate(float (&v)[W], int act) {
+    if (act == kActRelu) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];
+    } else if (act == kActSilu) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[j] = v[j] / (1.f + expf(-v[j]));
+    } else if (act == kActGelu) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[j] = 0.5f * v[j] * erfcf(v[j] * -0.70710678118654752f);
+    } else if (act == kActGeluTanh) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[j] = v[j] / (1.f + expf(-1.5957691216057308f * (v[j] + 0.044715f * v[j] * v[j] * v[j])));
     }
 }
 
-// Eight consecutive channels n .. n+7 of row m: bias, activation, residual, ONE rounding, store.  Columns from N on are not
-// written.
-FR_DEV void finish8(const LinearOut& o, const float* __restrict__ bias, size_t m, int n, float (&v)[8]) {
-    if (n >= o.N) return;
-    const float4v b0 = *(const float4v*)(bias + n), b1 = *(const float4v*)(bias + n + 4);     // (padded with zeros)
+template <typename T, int W> struct vect { typedef T type __attribute__((ext_vector_type(W))); };
+
+// W (4 or 8) consecutive channels n .. n+W-1 of row m: bias, activation, residual.
+template <int W>
+FR_DEV void load_bias(const float* __restrict__ bias, int n, float (&b)[W]) {      // (padded with zeros to whole panels)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) { v[j] += b0[j]; v[4 + j] += b1[j]; }
+    for (int j = 0; j < W; j += 4) {
+        const float4v t = *(const float4v*)(bias + n + j);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = activate(v[j], o.act);
-    const bool whole = n + 8 <= o.N;
+        for (int i = 0; i < 4; ++i) b[j + i] = t[i];
+    }
+}
+template <int W>
+FR_DEV void epilogue(const LinearOut& o, const float (&b)[W], size_t m, int n, float (&v)[W]) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) v[j] += b[j];
+    activate<W>(v, o.act);
     if (o.res) {
         const size_t at = m * (size_t)o.ldr + n;
-        if (whole && o.vec_res) {
+        if (n + W <= o.N && o.vec_res) {
             if (o.rtype == kF32) {
-                const float4v r0 = *(const float4v*)((const float*)o.res + at), r1 = *(const float4v*)((const float*)o.res + at + 4);
+                const auto r = *(const typename vect<float, W>::type*)((const float*)o.res + at);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) { v[j] += r0[j]; v[4 + j] += r1[j]; }
+                for (int j = 0; j < W; ++j) v[j] += r[j];
             } else if (o.rtype == kBF16) {
-                const bf8 r = *(const bf8*)((const __bf16*)o.res + at);
+                const auto r = *(const typename vect<__bf16, W>::type*)((const __bf16*)o.res + at);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] += (float)r[j];
+                for (int j = 0; j < W; ++j) v[j] += (float)r[j];
             } else {
-                const half8 r = *(const half8*)((const half_t*)o.res + at);
+                const auto r = *(const typename vect<half_t, W>::type*)((const half_t*)o.res + at);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] += (float)r[j];
+                for (int j = 0; j < W; ++j) v[j] += (float)r[j];
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < W; ++j)
                 if (n + j < o.N) v[j] += load1(o.res, at + j, o.rtype);
         }
     }
+}
+
+// The same, then ONE rounding and the store.  Columns from N on are not written.
+template <int W>
+FR_DEV void finish(const LinearOut& o, const float (&b)[W], size_t m, int n, float (&v)[W]) {
+    if (n >= o.N) return;
+    epilogue<W>(o, b, m, n, v);
     const size_t at = m * (size_t)o.ldo + n;
-    if (whole && o.vec_out) {
+    if (n + W <= o.N && o.vec_out) {
         if (o.otype == kF32) {
-            *(float4v*)((float*)o.out + at) = float4v{v[0], v[1], v[2], v[3]};
-            *(float4v*)((float*)o.out + at + 4) = float4v{v[4], v[5], v[6], v[7]};
+#pragma unroll
+            for (int j = 0; j < W; j += 4) *(float4v*)((float*)o.out + at + j) = float4v{v[j], v[j + 1], v[j + 2], v[j + 3]};
         } else if (o.otype == kBF16) {
-            bf8 t;
+            typename vect<__bf16, W>::type t;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) t[j] = (__bf16)v[j];
-            *(bf8*)((__bf16*)o.out + at) = t;
+            for (int j = 0; j < W; ++j) t[j] = (__bf16)v[j];
+            *(typename vect<__bf16, W>::type*)((__bf16*)o.out + at) = t;
         } else {
-            half8 t;
+            typename vect<half_t, W>::type t;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) t[j] = (half_t)v[j];
-            *(half8*)((half_t*)o.out + at) = t;
+            for (int j = 0; j < W; ++j) t[j] = (half_t)v[j];
+            *(typename vect<half_t, W>::type*)((half_t*)o.out + at) = t;
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < W; ++j)
             if (n + j < o.N) store1(o.out, at + j, o.otype, v[j]);
     }
 }
@@ -129,7 +151,7 @@ __global__ __launch_bounds__(256) void linear_layout_kernel(const uint16_t* __re
     const size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
     if (t >= (size_t)panels * ksteps * 64) return;
     const int lane = (int)(t & 63);
-    const int s = (int)((t >> 6) % ksteps), p = (int)((t >> 6) / ksteps);
+    const int kk = (int)(t >> 6) & 1, p = (int)((t >> 7) % panels), s = (int)((t >> 7) / panels) * 2 + kk;
     const int r = lane & 15;
     const int ch = (p >> 1) * 32 + (r >> 2) * 8 + (p & 1) * 4 + (r & 3);
     const int k0 = s * 32 + (lane >> 4) * 8;
@@ -160,102 +182,377 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const uint16_t* __rest
     *(uint4v*)(out + t * 8) = o;
 }
 
-// One TM x TN tile of y (or of a K slice's partial sums) per block, 64 K-elements per step through two LDS stages filled by
-// 16-byte LDS-DMA.  X rows are 128 bytes in LDS, 16-byte chunk c of row r at position c ^ (r & 7) (applied to the
-// source address, undone at the read); weight fragments lie as in memory and are read linearly: neither read has a bank
-// conflict.  Waves WX x WY, each (TM/WX) x (TN/WY).
-template <bool BF, int TM, int TN, int WX, int WY>
+// The tile kernel: TM x TN of y (or of a K slice's partial sums) at a time, 64 K-elements per step.  X and W stages arrive by
+// 16-byte LDS-DMA in rings of XS and WS stages, loads running XS-1 and WS-1 steps ahead, waited for with counted vmcnt so that
+// the newest stages stay in flight across the step's one barrier.  X rows are 128 bytes in LDS, 16-byte chunk c of row
+// r at position c ^ (r & 7) (applied to the source address, undone at the read); weight fragments lie as in memory and are
+// read linearly: neither read has a bank conflict.  Waves WX x WY, each (TM/WX) x (TN/WY).  A step's MFMAs go in four units
+// (32-deep half kk, half of the rows xh); a unit's fragments are read while the one before it computes, and the last unit of
+// a step computes behind the barrier, under the next step's first reads.
+// Behind the last step the stages are free: every wave brings its accumulators through a part of them that is its own, half of
+// its rows at a time, and finishes them row by row, eight consecutive channels a lane (whole cache lines per store, and one
+// copy of the epilogue's code instead of one per accumulator).
+template <bool BF, int TM, int TN, int WX, int WY, int XS, int WS>
+struct TileCore {
+    static constexpr int NW = WX * WY, TX = TM / WX, TY = TN / WY, NX = TX / 16, NY = TY / 16, NXH = NX / 2;
+    static constexpr int XB = TM * 128, WB = TN * 128, LDS = XS * XB + WS * WB;
+    static constexpr int NPX = TM / 8 / NW, NPW = TN / 8 / NW;
+    static constexpr int DX = XS - 1, DW = WS - 1;
+    // loads that may still be in flight when the next step's stages must have landed (issue order: W, then X)
+    static constexpr int KEEP = DX == DW ? (DX - 1) * (NPX + NPW) : NPX;
+    static_assert(TM % (8 * NW) == 0 && TN % (8 * NW) == 0 && TX % 32 == 0 && TY % 32 == 0, "tile shape");
+    static_assert((DX == DW || (DX == 2 && DW == 1)) && KEEP <= 63 && LDS <= 163840, "ring shape");
+    // the wave's part of LDS at the end: HR rows of TY fp32 values, 16 bytes of padding a row (no bank conflict)
+    static constexpr int HR = TX / 2 > 64 ? 64 : TX / 2, ER = TY + 4;
+    static_assert(NW * HR * ER * 4 <= LDS && HR % 16 == 0, "room for the epilogue");
+
+    float4v acc[NY][NX];
+    uint4v fw[2][NY], fx[2][NXH];
+
+    FR_DEV void zero() {
+#pragma unroll
+        for (int y = 0; y < NY; ++y)
+#pragma unroll
+            for (int x = 0; x < NX; ++x) acc[y][x] = float4v{0.f, 0.f, 0.f, 0.f};
+    }
+    template <int U>
+    FR_DEV void read(const char* xb, const char* wb, int lane, int wx, int wy) {
+        constexpr int kk = U >> 1, xh = U & 1;
+        const int coff = ((kk * 4 + (lane >> 4)) ^ (lane & 7)) << 4;
+        if (xh == 0) {
+#pragma unroll
+            for (int y = 0; y < NY; ++y) fw[kk][y] = *(const uint4v*)(wb + ((wy * NY + y) * 2 + kk) * 1024 + lane * 16);
+        }
+#pragma unroll
+        for (int x = 0; x < NXH; ++x) fx[xh][x] = *(const uint4v*)(xb + (wx * TX + (xh * NXH + x) * 16 + (lane & 15)) * 128 + coff);
+    }
+    template <int U>
+    FR_DEV void mma() {
+        constexpr int kk = U >> 1, xh = U & 1;
+#pragma unroll
+        for (int y = 0; y < NY; ++y)
+#pragma unroll
+            for (int x = 0; x < NXH; ++x) acc[y][xh * NXH + x] = mfma<BF>(fw[kk][y], fx[xh][x], acc[y][xh * NXH + x]);
+    }
+    FR_DEV static void wait_keep() {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(KEEP) : "memory");
+    }
+    FR_DEV static void wait_all() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+};
+
+template <bool BF, int TM, int TN, int WX, int WY, int XS, int WS>
 __global__ __launch_bounds__(64 * WX * WY) void linear_tile_kernel(LinearIn a, LinearOut o) {
-    constexpr int NW = WX * WY, TX = TM / WX, TY = TN / WY, NX = TX / 16, NY = TY / 16;
-    constexpr int XB = TM * 128, WB = TN * 128, SB = XB + WB;
-    constexpr int NPX = TM / 8 / NW, NPW = TN / 8 / NW;
-    static_assert(TM % (8 * NW) == 0 && TN % (8 * NW) == 0 && TX % 16 == 0 && TY % 32 == 0, "tile shape");
+    using Core = TileCore<BF, TM, TN, WX, WY, XS, WS>;
+    constexpr int NW = Core::NW, NPX = Core::NPX, NPW = Core::NPW, NY = Core::NY;
     extern __shared__ __attribute__((aligned(16))) char smem[];
+    char* const xs = smem;
+    char* const ws = smem + XS * Core::XB;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wx = wave / WY, wy = wave % WY;
-    const int l15 = lane & 15, g0 = lane >> 4, l7 = lane & 7;
+    const int l15 = lane & 15, g0 = lane >> 4;
 
     const int tiles = a.mtiles * a.ntiles;
     const int id = xcd_remap(blockIdx.x, gridDim.x);
     const int z = id / tiles, t = id % tiles;
-    const int mt = a.m_fast ? t % a.mtiles : t / a.ntiles, nt = a.m_fast ? t / a.mtiles : t % a.ntiles;
-    const int m0 = mt * TM, n0 = nt * TN;
-    const int k_lo = z * a.ksteps_per_split, k_hi = min(a.ksteps, k_lo + a.ksteps_per_split);
+    const int m0 = (a.m_fast ? t % a.mtiles : t / a.ntiles) * TM, n0 = (a.m_fast ? t / a.mtiles : t % a.ntiles) * TN;
+    const int k_lo = z * a.ksteps_per_split, S = min(a.ksteps, k_lo + a.ksteps_per_split) - k_lo;
 
-    const int c = l7 ^ (lane >> 3);                 // the 16-byte chunk this lane fetches of its row
+    const int c = (lane & 7) ^ (lane >> 3);             // the 16-byte chunk this lane fetches of its row
     const char* xp[NPX];
 #pragma unroll
     for (int i = 0; i < NPX; ++i) {
         int m = m0 + 8 * (wave + NW * i) + (lane >> 3);
         m = m < a.M ? m : a.M - 1;
-        xp[i] = (const char*)a.x + (a.tiled ? (size_t)(m >> 8) * a.xtile + (size_t)(m & 255) * 128 : (size_t)m * a.ldx * 2) + c * 16;
+        xp[i] = (const char*)a.x + (a.tiled ? (size_t)(m >> 8) * a.xtile + (size_t)(m & 255) * 128 : (size_t)m * a.ldx * 2) + c * 16 +
+                (size_t)k_lo * a.xstep;
     }
-    const char* wp[NPW];
+    const int wpanel = n0 >> 4;
+    int xk = k_lo, wk = k_lo;                           // what the next issue brings
+    auto next_x = [&](int slot) {
+        char* const st = xs + slot * Core::XB;
+        if (xk * 64 + 64 <= a.K) {
 #pragma unroll
-    for (int i = 0; i < NPW; ++i) {
-        const int piece = wave + NW * i;
-        int p = (n0 >> 4) + (piece >> 1);
-        p = p < a.panels ? p : a.panels - 1;        // (columns beyond N: computed from the last panel and dropped)
-        wp[i] = (const char*)a.wt + ((size_t)p * (2 * a.ksteps) + (piece & 1)) * 1024 + lane * 16;
-    }
-    auto issue = [&](int ks, char* st) {
-        const bool tail = ks * 64 + c * 8 >= a.K;   // chunks behind the K-th element: zeros (K is a multiple of 8 here)
+            for (int i = 0; i < NPX; ++i) {
+                glds16(xp[i], st + (wave + NW * i) * 1024);
+                xp[i] += a.xstep;
+            }
+        } else {                                        // chunks behind the K-th element: zeros (K is a multiple of 8 here)
+            const bool tail = xk * 64 + c * 8 >= a.K;
 #pragma unroll
-        for (int i = 0; i < NPX; ++i) {
-            const char* src = xp[i] + (size_t)ks * a.xstep;
-            glds16(tail ? (const char*)a.zeros + c * 16 : src, st + (wave + NW * i) * 1024);
+            for (int i = 0; i < NPX; ++i) glds16(tail ? (const char*)a.zeros + c * 16 : xp[i], st + (wave + NW * i) * 1024);
         }
+        ++xk;
+    };
+    auto next_w = [&](int slot) {
+        char* const st = ws + slot * Core::WB;
 #pragma unroll
-        for (int i = 0; i < NPW; ++i) glds16(wp[i] + (size_t)ks * 2048, st + XB + (wave + NW * i) * 1024);
+        for (int i = 0; i < NPW; ++i) {
+            const int piece = wave + NW * i;
+            const int p = min(wpanel + (piece >> 1), a.panels - 1);     // (columns beyond N: computed from the last panel and dropped)
+            const char* src = (const char*)a.wt + ((size_t)wk * a.panels + p) * 2048 + (piece & 1) * 1024;
+            glds16(src + lane * 16, st + piece * 1024);
+        }
+        ++wk;
     };
 
-    float4v acc[NY][NX];
-#pragma unroll
-    for (int y = 0; y < NY; ++y)
-#pragma unroll
-        for (int x = 0; x < NX; ++x) acc[y][x] = float4v{0.f, 0.f, 0.f, 0.f};
+    Core core;
+    core.zero();
+    // prologue: stages 0 .. D-1
+    if constexpr (Core::DX == Core::DW) {
+        for (int d = 0; d < Core::DX; ++d)
+            if (d < S) { next_w(d); next_x(d); }
+        if (S >= Core::DX) Core::wait_keep(); else Core::wait_all();
+    } else {
+        next_w(0);
+        next_x(0);
+        if (S > 1) { next_x(1); Core::wait_keep(); } else { Core::wait_all(); }
+    }
+    __builtin_amdgcn_s_barrier();
 
-    issue(k_lo, smem);
-    __syncthreads();
-    for (int ks = k_lo; ks < k_hi; ++ks) {
-        char* const st = smem + ((ks - k_lo) & 1) * SB;
-        if (ks + 1 < k_hi) issue(ks + 1, smem + (((ks - k_lo) & 1) ^ 1) * SB);
+    int xslot = 0, wslot = 0;
+    auto fence = [&]() __attribute__((always_inline)) { __builtin_amdgcn_sched_barrier(0); };
+    auto reads_done = [&]() __attribute__((always_inline)) {
+        fence(); __builtin_amdgcn_s_waitcnt(0xC07F); fence();       // lgkmcnt(0)
+    };
+    for (int s = 0; s < S; ++s) {
+        const char* const xb = xs + xslot * Core::XB;
+        const char* const wb = ws + wslot * Core::WB;
+        core.template read<0>(xb, wb, lane, wx, wy);
+        fence();
+        if (s > 0) {
+            core.template mma<3>();
+            fence();
+        }
+        // the stages that the barrier behind the previous step has freed
+        if (s + Core::DW < S) next_w(wslot == 0 ? WS - 1 : wslot - 1);
+        if (s + Core::DX < S) next_x(xslot == 0 ? XS - 1 : xslot - 1);
+        reads_done();
+        core.template read<1>(xb, wb, lane, wx, wy);
+        fence();
+        core.template mma<0>();
+        reads_done();
+        core.template read<2>(xb, wb, lane, wx, wy);
+        fence();
+        core.template mma<1>();
+        reads_done();
+        core.template read<3>(xb, wb, lane, wx, wy);
+        fence();
+        core.template mma<2>();
+        reads_done();       // every read of this step's stages has returned: they may be refilled behind the barrier
+        if (s + Core::DX < S) Core::wait_keep(); else Core::wait_all();
+        __builtin_amdgcn_s_barrier();
+        fence();
+        xslot = xslot == XS - 1 ? 0 : xslot + 1;
+        wslot = wslot == WS - 1 ? 0 : wslot + 1;
+    }
+    core.template mma<3>();
+
+    // (all stages have been read by all waves: the barrier above)
+    constexpr int HR = Core::HR, ER = Core::ER, LR = Core::TY / 8, RI = 64 / LR;    // LR lanes a row, RI rows an iteration
+    float* const eb = (float*)smem + wave * HR * ER;
+    const int n = n0 + wy * Core::TY + (lane % LR) * 8;
+    float bv[8];
+    load_bias<8>(a.bias, n < a.npad ? n : 0, bv);
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            const int coff = ((kk * 4 + g0) ^ l7) << 4;
-            uint4v fx[NX], fw[NY];
+    for (int h = 0; h < Core::TX / HR; ++h) {
 #pragma unroll
-            for (int x = 0; x < NX; ++x) fx[x] = *(const uint4v*)(st + (wx * TX + x * 16 + l15) * 128 + coff);
-#pragma unroll
-            for (int y = 0; y < NY; ++y) fw[y] = *(const uint4v*)(st + XB + ((wy * NY + y) * 2 + kk) * 1024 + lane * 16);
+        for (int x = 0; x < HR / 16; ++x)
 #pragma unroll
             for (int y = 0; y < NY; ++y)
-#pragma unroll
-                for (int x = 0; x < NX; ++x) acc[y][x] = mfma<BF>(fw[y], fx[x], acc[y][x]);
+                *(float4v*)(eb + (x * 16 + l15) * ER + (y >> 1) * 32 + g0 * 8 + (y & 1) * 4) = core.acc[y][h * (HR / 16) + x];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int r = lane / LR; r < HR; r += RI) {
+            const int m = m0 + wx * Core::TX + h * HR + r;
+            const float4v v0 = *(const float4v*)(eb + r * ER + (lane % LR) * 8), v1 = *(const float4v*)(eb + r * ER + (lane % LR) * 8 + 4);
+            if (m >= a.M || n >= a.npad) continue;
+            if (a.slab) {
+                float* d = a.slab + ((size_t)z * a.M + m) * a.npad + n;
+                *(float4v*)d = v0;
+                *(float4v*)(d + 4) = v1;
+            } else {
+                float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+                finish<8>(o, bv, m, n, v);
+            }
         }
-        __syncthreads();
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// The wave kernel, for calls of few tiles: a block is one 16 FX x 16 FW tile, and its NW waves share out K, 64 elements at a
+// time in turn.  Each wave multiplies its own slices of both operands for the whole tile, with a pipeline of its own: every
+// byte enters the CU once, as it would with a shared stage, but no wave ever waits for another until the sums are joined, in
+// wave order, through LDS.  Weight fragments (1 KiB of consecutive bytes) are loaded straight into registers; X goes through
+// LDS by LDS-DMA, eight rows of 128 bytes an instruction: in fragment order consecutive lanes read different rows, which the
+// load path serves 16 bytes a clock (38 GB/s per CU measured, against 110-145 for whole lines).
+// GATHER: rows that 16-byte loads cannot take, element by element into registers.
+template <int FX, int FW, int NW, int ST>
+struct WaveShape {
+    static constexpr int TM = 16 * FX, TN = 16 * FW, ER = TN + 4;
+    static constexpr int XB = TM * 128, STAGES = NW * ST * XB, PART = NW * TM * ER * 4;
+    static constexpr int LDS = STAGES > PART ? STAGES : PART;
+    static_assert(LDS <= 163840 && (ST - 1) * 2 * (FX + FW) <= 63, "stages");
+};
+template <bool BF, int FX, int FW, int NW, int ST, bool GATHER>
+__global__ __launch_bounds__(64 * NW) void linear_wave_kernel(LinearIn a, LinearOut o) {
+    using Shape = WaveShape<FX, FW, NW, ST>;
+    constexpr int TM = Shape::TM, TN = Shape::TN, ER = Shape::ER;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l15 = lane & 15, g0 = lane >> 4;
+    const int tiles = a.mtiles * a.ntiles;
+    const int id = xcd_remap(blockIdx.x, gridDim.x);
+    const int z = id / tiles, t = id % tiles;
+    const int m0 = (a.m_fast ? t % a.mtiles : t / a.ntiles) * TM, n0 = (a.m_fast ? t / a.mtiles : t % a.ntiles) * TN;
+    const int k_lo = z * a.ksteps_per_split, k_hi = min(a.ksteps, k_lo + a.ksteps_per_split);
+    const int n = (k_hi - k_lo - wave + NW - 1) / NW;       // slices of this wave: k_lo + wave, + NW, ...
+
+    const char* wp[FW];
+#pragma unroll
+    for (int y = 0; y < FW; ++y) wp[y] = (const char*)a.wt + (size_t)min((n0 >> 4) + y, a.panels - 1) * 2048 + lane * 16;
+    const size_t wstep = (size_t)a.panels * 2048;
+    auto row_at = [&](int r) __attribute__((always_inline)) {
+        int m = m0 + r;
+        m = m < a.M ? m : a.M - 1;
+        return (const char*)a.x + (a.tiled ? (size_t)(m >> 8) * a.xtile + (size_t)(m & 255) * 128 : (size_t)m * a.ldx * 2);
+    };
+    float4v acc[FW][FX];
+#pragma unroll
+    for (int y = 0; y < FW; ++y)
+#pragma unroll
+        for (int x = 0; x < FX; ++x) acc[y][x] = float4v{0.f, 0.f, 0.f, 0.f};
+
+    if constexpr (GATHER) {
+        const char* xp[FX];
+#pragma unroll
+        for (int x = 0; x < FX; ++x) xp[x] = row_at(x * 16 + l15);
+        for (int i = 0; i < n; ++i) {
+            const int ks = k_lo + wave + NW * i;
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                uint4v vw[FW], vx[FX];
+#pragma unroll
+                for (int y = 0; y < FW; ++y) vw[y] = *(const uint4v*)(wp[y] + (size_t)ks * wstep + kk * 1024);
+                const int k0 = ks * 64 + kk * 32 + g0 * 8;
+#pragma unroll
+                for (int x = 0; x < FX; ++x) {
+                    const uint16_t* e = (const uint16_t*)xp[x] + k0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const unsigned lo = k0 + 2 * j < a.K ? e[2 * j] : 0u, hi = k0 + 2 * j + 1 < a.K ? e[2 * j + 1] : 0u;
+                        vx[x][j] = lo | (hi << 16);
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < FX; ++x)
+#pragma unroll
+                    for (int y = 0; y < FW; ++y) acc[y][x] = mfma<BF>(vw[y], vx[x], acc[y][x]);
+            }
+        }
+    } else {
+        char* const st0 = smem + wave * (ST * Shape::XB);
+        const int c = (lane & 7) ^ (lane >> 3);             // the 16-byte chunk this lane fetches of its row
+        const char* xp[2 * FX];
+#pragma unroll
+        for (int i = 0; i < 2 * FX; ++i) xp[i] = row_at(8 * i + (lane >> 3)) + c * 16;
+        const char* const zeros = (const char*)a.zeros + c * 16;
+        uint4v bw[ST][2][FW];
+        // slice i -> X stage and weight registers p
+        auto issue = [&](int i, int p, uint4v (&vw)[2][FW]) __attribute__((always_inline)) {
+            const int ks = k_lo + wave + NW * i;
+            char* const st = st0 + p * Shape::XB;
+            if (ks * 64 + 64 <= a.K) {
+#pragma unroll
+                for (int x = 0; x < 2 * FX; ++x) glds16(xp[x] + (size_t)ks * a.xstep, st + x * 1024);
+            } else {                                        // chunks behind the K-th element: zeros (K is a multiple of 8 here)
+                const bool tail = ks * 64 + c * 8 >= a.K;
+#pragma unroll
+                for (int x = 0; x < 2 * FX; ++x) glds16(tail ? zeros : xp[x] + (size_t)ks * a.xstep, st + x * 1024);
+            }
+#pragma unroll
+            for (int y = 0; y < FW; ++y)
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk) vw[kk][y] = *(const uint4v*)(wp[y] + (size_t)ks * wstep + kk * 1024);
+        };
+        auto mma = [&](int p, const uint4v (&vw)[2][FW]) __attribute__((always_inline)) {
+            const char* const st = st0 + p * Shape::XB;
+            uint4v vx[2][FX];
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                for (int x = 0; x < FX; ++x)
+                    vx[kk][x] = *(const uint4v*)(st + (x * 16 + l15) * 128 + (((kk * 4 + g0) ^ (lane & 7)) << 4));
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(0xC07F);             // lgkmcnt(0): the stage has been read and may be refilled
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                for (int x = 0; x < FX; ++x)
+#pragma unroll
+                    for (int y = 0; y < FW; ++y) acc[y][x] = mfma<BF>(vw[kk][y], vx[kk][x], acc[y][x]);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+#pragma unroll
+        for (int p = 0; p < ST - 1; ++p)
+            if (p < n) issue(p, p, bw[p]);
+        int i = 0;
+        for (; i + 2 * ST - 1 <= n; i += ST) {              // nothing in here branches: the compiler can count what is in flight
+#pragma unroll
+            for (int p = 0; p < ST; ++p) {
+                issue(i + p + ST - 1, (p + ST - 1) % ST, bw[(p + ST - 1) % ST]);
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 1) * 2 * (FX + FW)) : "memory");
+                mma(p, bw[p]);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 2 * ST - 2; ++q) {
+            if (i + q < n) {
+                if (i + q + ST - 1 < n) {
+                    issue(i + q + ST - 1, (q + ST - 1) % ST, bw[(q + ST - 1) % ST]);
+                    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 1) * 2 * (FX + FW)) : "memory");
+                } else {
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                }
+                mma(q % ST, bw[q % ST]);
+            }
+        }
+        __syncthreads();                                    // the sums take the stages' place
     }
 
+    // consecutive channels a lane finishes: eight; four where the tile is half a pair of panels
+    constexpr int CH = FW == 1 ? 4 : 8;
+    float* const part = (float*)smem;
+    float* const mine = part + wave * TM * ER;
 #pragma unroll
-    for (int x = 0; x < NX; ++x) {
-        const int m = m0 + wx * TX + x * 16 + l15;
-        if (m >= a.M) continue;
+    for (int x = 0; x < FX; ++x)
 #pragma unroll
-        for (int u = 0; u < NY / 2; ++u) {
-            const int n = n0 + wy * TY + u * 32 + g0 * 8;
-            float v[8];
+        for (int y = 0; y < FW; ++y) *(float4v*)(mine + (x * 16 + l15) * ER + (y >> 1) * 32 + g0 * CH + (y & 1) * 4) = acc[y][x];
+    __syncthreads();
+    for (int i = tid; i < TM * (TN / CH); i += 64 * NW) {
+        const int r = i / (TN / CH), m = m0 + r, cn = (i % (TN / CH)) * CH;
+        const int ch = FW == 1 ? (n0 >> 5) * 32 + cn * 2 + ((n0 >> 4) & 1) * 4 : n0 + cn;
+        if (m >= a.M || ch >= a.npad) continue;
+        float bv[CH], v[CH] = {};
+        load_bias<CH>(a.bias, ch, bv);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { v[j] = acc[2 * u][x][j]; v[4 + j] = acc[2 * u + 1][x][j]; }
-            if (a.slab) {
-                if (n < a.npad) {
-                    float* d = a.slab + ((size_t)z * a.M + m) * a.npad + n;
-                    *(float4v*)d = float4v{v[0], v[1], v[2], v[3]};
-                    *(float4v*)(d + 4) = float4v{v[4], v[5], v[6], v[7]};
-                }
-            } else {
-                finish8(o, a.bias, m, n, v);
+        for (int w = 0; w < NW; ++w) {
+            const float* p = part + w * TM * ER + r * ER + cn;
+#pragma unroll
+            for (int q = 0; q < CH; q += 4) {
+                const float4v t = *(const float4v*)(p + q);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[q + j] += t[j];
             }
+        }
+        if (a.slab) {
+            float* d = a.slab + ((size_t)z * a.M + m) * a.npad + ch;
+#pragma unroll
+            for (int q = 0; q < CH; q += 4) *(float4v*)(d + q) = float4v{v[q], v[q + 1], v[q + 2], v[q + 3]};
+        } else {
+            finish<CH>(o, bv, m, ch, v);
         }
     }
 }
@@ -267,55 +564,218 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearIn a, LinearOut 
     if (t >= (size_t)a.M * per_row) return;
     const int m = (int)(t / per_row), n = (int)(t % per_row) * 8;
     float v[8] = {};
-    for (int z = 0; z < splits; ++z) {
-        const float* p = a.slab + ((size_t)z * a.M + m) * a.npad + n;
-        const float4v p0 = *(const float4v*)p, p1 = *(const float4v*)(p + 4);
+    const float* p = a.slab + (size_t)m * a.npad + n;
+    const size_t step = (size_t)a.M * a.npad;
+    for (int z = 0; z < splits; z += 4) {           // four slices in flight, added in slice order
+        float4v q[4][2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { v[j] += p0[j]; v[4 + j] += p1[j]; }
+        for (int i = 0; i < 4; ++i)
+            if (z + i < splits) { q[i][0] = *(const float4v*)(p + (z + i) * step); q[i][1] = *(const float4v*)(p + (z + i) * step + 4); }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (z + i < splits) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { v[j] += q[i][0][j]; v[4 + j] += q[i][1][j]; }
+            }
     }
-    finish8(o, a.bias, m, n, v);
+    float bv[8];
+    load_bias<8>(a.bias, n, bv);
+    finish<8>(o, bv, m, n, v);
 }
 
 // ------------------------------------------------------------- unit rows ---
-// One wave per row.  The norm comes from a 64-bit sum of squares rounded to fp32, then one IEEE division per
-// element: the stored row is the same whatever the summation order, and the same as the library's own upload makes of
-// it (gallery_upsert_kernel).  A row shorter than 1e-30 is divided by one.
-__global__ __launch_bounds__(256) void unit_rows_kernel(const void* __restrict__ x, int type, int64_t ldx, int M, int N,
-                                                        UnitOut o) {
-    const int m = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (m >= M) return;
-    const size_t at = (size_t)m * ldx;
-    double ss = 0.0;
-    for (int c = lane; c < N; c += 64) {
-        const double v = load1(x, at + c, type);
-        ss += v * v;
-    }
+// The norm comes from a 64-bit sum of squares rounded to fp32, then one IEEE division per element: the stored row is the same
+// whatever the summation order, and the same as the library's own upload makes of it (gallery_upsert_kernel).  A row
+// shorter than 1e-30 is divided by one.
+// L lanes a row, each R vectors of V consecutive elements in registers: x is read once.  R = 0: rows too long for that, or
+// that V does not divide or align, are read twice (the second time out of the cache).
+template <typename T, int V>
+FR_DEV void load_vec(const T* p, float (&v)[V]) {
+    if constexpr (V == 1) {
+        v[0] = (float)*p;
+    } else {
+        const auto t = *(const typename vect<T, V>::type*)p;
 #pragma unroll
-    for (int s = 32; s > 0; s >>= 1) ss += __shfl_xor(ss, s);
-    float nrm = (float)sqrt(ss);
-    nrm = nrm < 1e-30f ? 1.0f : nrm;
-    for (int c = lane; c < N; c += 64) {
-        const half_t v = (half_t)__fdiv_rn(load1(x, at + c, type), nrm);
-        if (o.gallery) {
-            const int64_t r = o.row0 + m;       // (the order of a gallery's rows in memory: see gal_index)
-            ((half_t*)o.out)[((((size_t)(r >> 8) * (N >> 6) + (c >> 6)) << 8) + (r & 255)) * 64 + (c & 63)] = v;
-        } else {
-            ((half_t*)o.out)[(size_t)m * o.ldo + c] = v;
+        for (int j = 0; j < V; ++j) v[j] = (float)t[j];
+    }
+}
+template <int V>
+FR_DEV void store_unit(const UnitOut& o, int N, int m, int c, const float (&v)[V], float nrm) {
+    half_t* d;
+    if (o.gallery) {
+        const int64_t r = o.row0 + m;       // (the order of a gallery's rows in memory: see gal_index)
+        d = (half_t*)o.out + ((((size_t)(r >> 8) * (N >> 6) + (c >> 6)) << 8) + (r & 255)) * 64 + (c & 63);
+    } else {
+        d = (half_t*)o.out + (size_t)m * o.ldo + c;
+    }
+    if constexpr (V == 1) {
+        *d = (half_t)__fdiv_rn(v[0], nrm);
+    } else {
+        typename vect<half_t, V>::type t;
+#pragma unroll
+        for (int j = 0; j < V; ++j) t[j] = (half_t)__fdiv_rn(v[j], nrm);
+        *(typename vect<half_t, V>::type*)d = t;
+    }
+}
+template <typename T, int L, int V, int R>
+__global__ __launch_bounds__(256) void unit_rows_kernel(const T* __restrict__ x, int64_t ldx, int M, int N, UnitOut o) {
+    constexpr int RB = 256 / L;             // rows a block
+    const int m = blockIdx.x * RB + threadIdx.x / L, l = threadIdx.x % L;
+    if (m >= M) return;                     // (the lanes of a row leave together)
+    const T* const row = x + (size_t)m * ldx;
+    double ss = 0.0;
+    float v[R ? R : 1][V];
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int c = (i * L + l) * V;
+            if (c < N) load_vec<T, V>(row + c, v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if ((i * L + l) * V < N) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) ss += (double)v[i][j] * (double)v[i][j];
+            }
+    } else {
+        for (int c = l * V; c < N; c += L * V) {
+            load_vec<T, V>(row + c, v[0]);
+#pragma unroll
+            for (int j = 0; j < V; ++j) ss += (double)v[0][j] * (double)v[0][j];
         }
     }
-    if (lane == 0 && o.keys_dst) o.keys_dst[o.row0 + m] = o.keys_src[o.row0 + m];
+#pragma unroll
+    for (int s = L / 2; s > 0; s >>= 1) ss += __shfl_xor(ss, s);
+    float nrm = (float)sqrt(ss);
+    nrm = nrm < 1e-30f ? 1.0f : nrm;
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int c = (i * L + l) * V;
+            if (c < N) store_unit<V>(o, N, m, c, v[i], nrm);
+        }
+    } else {
+        for (int c = l * V; c < N; c += L * V) {
+            load_vec<T, V>(row + c, v[0]);
+            store_unit<V>(o, N, m, c, v[0], nrm);
+        }
+    }
+    if (l == 0 && o.keys_dst) o.keys_dst[o.row0 + m] = o.keys_src[o.row0 + m];
 }
 
-template <bool BF, int TM, int TN, int WX, int WY>
-hipError_t launch_tile(LinearIn a, const LinearOut& o, int splits, hipStream_t s) {
-    constexpr int SB = (TM + TN) * 128;
+template <typename T, int L, int V, int R>
+hipError_t launch_unit(const void* x, int64_t ldx, int64_t M, int N, const UnitOut& o, hipStream_t s) {
+    const int64_t rb = 256 / L;
+    hipLaunchKernelGGL((unit_rows_kernel<T, L, V, R>), dim3((unsigned)((M + rb - 1) / rb)), dim3(256), 0, s, (const T*)x, ldx, (int)M, N, o);
+    return hipGetLastError();
+}
+template <typename T>
+hipError_t unit_by_width(const void* x, int64_t ldx, int64_t M, int N, const UnitOut& o, hipStream_t s) {
+    constexpr int V = 16 / sizeof(T);
+    const bool vec = N % V == 0 && ldx % V == 0 && (size_t)x % 16 == 0 &&
+                     (o.gallery || (o.ldo % V == 0 && (size_t)o.out % (V * 2) == 0));
+    if (!vec) return N <= 256 ? launch_unit<T, 16, 1, 0>(x, ldx, M, N, o, s) : launch_unit<T, 64, 1, 0>(x, ldx, M, N, o, s);
+    if (N <= 16 * V) return launch_unit<T, 4, V, 4>(x, ldx, M, N, o, s);
+    if (N <= 64 * V) return launch_unit<T, 16, V, 4>(x, ldx, M, N, o, s);
+    if (N <= 256 * V) return launch_unit<T, 64, V, 4>(x, ldx, M, N, o, s);
+    if (N <= 1024 * V) return launch_unit<T, 64, V, 16>(x, ldx, M, N, o, s);
+    return launch_unit<T, 64, V, 0>(x, ldx, M, N, o, s);
+}
+
+template <bool BF, int TM, int TN, int WX, int WY, int XS, int WS>
+hipError_t launch_tile(LinearIn a, const LinearOut& o, int splits, hipStream_t s, bool attr) {
+    using Core = TileCore<BF, TM, TN, WX, WY, XS, WS>;
+    const auto kern = linear_tile_kernel<BF, TM, TN, WX, WY, XS, WS>;
+    if (attr) return hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, Core::LDS);
     a.mtiles = (a.M + TM - 1) / TM;
     a.ntiles = (a.npad + TN - 1) / TN;
     a.m_fast = a.mtiles < a.ntiles;
+    a.splits = splits;
     a.ksteps_per_split = (a.ksteps + splits - 1) / splits;
-    hipLaunchKernelGGL((linear_tile_kernel<BF, TM, TN, WX, WY>), dim3((unsigned)(a.mtiles * a.ntiles * splits)), dim3(64 * WX * WY),
-                       2 * SB, s, a, o);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(a.mtiles * a.ntiles * splits)), dim3(64 * WX * WY), Core::LDS, s, a, o);
     return hipGetLastError();
+}
+
+template <bool BF, int FX, int FW, int NW, int ST, bool HAS_GATHER>
+hipError_t launch_wave(LinearIn a, const LinearOut& o, int splits, bool gather, hipStream_t s, bool attr) {
+    using Shape = WaveShape<FX, FW, NW, ST>;
+    if (gather && !HAS_GATHER) return hipErrorInvalidValue;
+    const auto whole = linear_wave_kernel<BF, FX, FW, NW, ST, false>;
+    if (attr) {
+        if constexpr (HAS_GATHER) {
+            const hipError_t e = hipFuncSetAttribute((const void*)linear_wave_kernel<BF, FX, FW, NW, ST, true>,
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, Shape::PART);
+            if (e != hipSuccess) return e;
+        }
+        return hipFuncSetAttribute((const void*)whole, hipFuncAttributeMaxDynamicSharedMemorySize, Shape::LDS);
+    }
+    a.mtiles = (a.M + Shape::TM - 1) / Shape::TM;
+    a.ntiles = (a.npad + Shape::TN - 1) / Shape::TN;
+    a.m_fast = a.mtiles < a.ntiles;
+    a.splits = splits;
+    a.ksteps_per_split = (a.ksteps + splits - 1) / splits;
+    const dim3 grid((unsigned)(a.mtiles * a.ntiles * splits));
+    if constexpr (HAS_GATHER) {
+        if (gather) {
+            hipLaunchKernelGGL((linear_wave_kernel<BF, FX, FW, NW, ST, true>), grid, dim3(64 * NW), Shape::PART, s, a, o);
+            return hipGetLastError();
+        }
+    }
+    hipLaunchKernelGGL(whole, grid, dim3(64 * NW), Shape::LDS, s, a, o);
+    return hipGetLastError();
+}
+
+// The tile shapes: what one 64-deep step of a tile takes while the whole chip runs such tiles (one a CU), measured at
+// K = 4096, in microseconds.  Per value of a tile they get cheaper from the first to the last, whose tile waits longest for its
+// own end; the wave kernel's tiles are small enough that a single round of them covers a batch.
+struct Shape { int tm, tn; float step; };
+constexpr Shape kShapes[] = {
+    {16, 32, 0.066f},   // wave kernel, 16 waves:  256 x 512 x 4096    8.7 us
+    {32, 32, 0.085f},   // wave kernel,  8 waves:  64 x 4096 x 4096    9.8 us
+    {64, 64, 0.20f},    // wave kernel,  8 waves:  256 x 4096 x 4096  17 us
+    {128, 64, 0.375f},  // wave kernel,  4 waves:  2048 x 1024 x 4096 28 us
+    {256, 128, 1.10f},  // tile kernel:            16384 x 512 x 4096 73 us
+    {256, 256, 1.95f},  // tile kernel:            65536 x 512 x 4096 254 us
+};
+constexpr int kNumShapes = sizeof kShapes / sizeof kShapes[0];
+template <bool BF>
+hipError_t launch_shape(int t, const LinearIn& a, const LinearOut& o, int splits, bool gather, hipStream_t s, bool attr) {
+    switch (t) {
+        case 0: return launch_wave<BF, 1, 2, 16, 3, true>(a, o, splits, gather, s, attr);
+        case 1: return launch_wave<BF, 2, 2, 8, 2, false>(a, o, splits, gather, s, attr);
+        case 2: return launch_wave<BF, 4, 4, 8, 2, false>(a, o, splits, gather, s, attr);
+        case 3: return launch_wave<BF, 8, 4, 4, 2, false>(a, o, splits, gather, s, attr);
+        case 4: return launch_tile<BF, 256, 128, 4, 2, 3, 3>(a, o, splits, s, attr);
+        default: return launch_tile<BF, 256, 256, 2, 4, 3, 2>(a, o, splits, s, attr);
+    }
+}
+
+// What a call runs as: the shape, the number of K slices and the way unaligned rows go in, whichever an estimate of the
+// time puts first.  A round of at most 256 tiles takes its K steps; K slices divide the steps and add the join (a launch, and
+// every slice's sums written and read once: 4.5 us + the bytes at 4 TB/s); rows that 16-byte loads cannot take cost a pass
+// that packs them (2.5 us + the bytes at 3 TB/s) or, element by element in the smallest shape, 1.8 us per slice of a wave
+// (77 x 131 x 500: 6.3 us against 8.5 packed).
+struct Plan { int shape, splits; bool gather; };
+Plan plan_linear(int64_t M, int npad, int ksteps, bool whole, size_t slab_bytes) {
+    Plan best{0, 1, false};
+    double best_t = 1e30;
+    const double pack = whole ? 0.0 : 2.5 + (double)M * ksteps * 256e-6 / 3.0;
+    for (int i = 0; i < kNumShapes; ++i) {
+        const Shape& sh = kShapes[i];
+        const int64_t tiles = (M + sh.tm - 1) / sh.tm * ((npad + sh.tn - 1) / sh.tn);
+        for (int splits = 1; splits <= 16 && splits <= ksteps; splits *= 2) {
+            const double join_bytes = (double)splits * M * npad * 8;
+            if (splits > 1 && (tiles * splits > 512 || join_bytes > 2.0 * slab_bytes)) break;
+            const double t = (double)((tiles * splits + 255) / 256) * ((ksteps + splits - 1) / splits) * sh.step + pack +
+                             (splits > 1 ? 4.5 + join_bytes * 1e-6 / 4.0 : 0.0);
+            if (t < best_t) { best_t = t; best = Plan{i, splits, false}; }
+        }
+        if (i == 0 && !whole) {
+            const double t = (double)((tiles + 255) / 256) * ((ksteps + 15) / 16) * 1.8;
+            if (t < best_t) { best_t = t; best = Plan{0, 1, true}; }
+        }
+    }
+    return best;
 }
 
 }  // namespace
@@ -337,8 +797,11 @@ hipError_t launch_linear(const LinearCall& q, const LinearWork& ws, hipStream_t 
     LinearIn a{};
     a.wt = q.wt; a.bias = q.bias; a.zeros = ws.zeros;
     a.K = q.K; a.npad = linear_npad(q.N); a.panels = a.npad / 16; a.ksteps = linear_kpad(q.K) / 64;
-    const bool direct = q.tiled || (q.K % 8 == 0 && q.ldx % 8 == 0 && (size_t)q.x % 16 == 0);
+    // can 16-byte loads take the rows?
+    const bool whole = q.tiled || (q.K % 8 == 0 && q.ldx % 8 == 0 && (size_t)q.x % 16 == 0);
     const size_t row_bytes = (size_t)linear_kpad(q.K) * 2;
+    Plan plan = plan_linear(q.M, a.npad, a.ksteps, whole, ws.slab_bytes);
+    const bool direct = whole || plan.gather;
     // rows that must be packed first go through the workspace in runs of whole tiles
     const int64_t run = direct ? q.M : (int64_t)(ws.pack_bytes / row_bytes) / 256 * 256;
     if (run <= 0) return hipErrorInvalidValue;
@@ -362,16 +825,10 @@ hipError_t launch_linear(const LinearCall& q, const LinearWork& ws, hipStream_t 
         o.N = q.N;
         o.vec_out = (size_t)o.out % 16 == 0 && (size_t)o.ldo * osz % 16 == 0;
         o.vec_res = o.res && (size_t)o.res % 16 == 0 && (size_t)o.ldr * rsz % 16 == 0;
-        // Few tiles leave CUs idle: K is then cut into slices whose partial sums meet in the workspace.
-        const int tiles = ((rows + 127) / 128) * ((a.npad + 127) / 128);
-        int splits = 256 / tiles;
-        if (splits > a.ksteps) splits = a.ksteps;
-        const size_t slab = (size_t)rows * a.npad * 4;
-        if ((size_t)splits * slab > ws.slab_bytes) splits = (int)(ws.slab_bytes / slab);
-        if (splits < 1) splits = 1;
-        splits = (a.ksteps + (a.ksteps + splits - 1) / splits - 1) / ((a.ksteps + splits - 1) / splits);
+        const int per = (a.ksteps + plan.splits - 1) / plan.splits, splits = (a.ksteps + per - 1) / per;    // (no empty slice)
         a.slab = splits > 1 ? ws.slabs : nullptr;
-        hipError_t e = q.bf16 ? launch_tile<true, 128, 128, 2, 2>(a, o, splits, s) : launch_tile<false, 128, 128, 2, 2>(a, o, splits, s);
+        hipError_t e = q.bf16 ? launch_shape<true>(plan.shape, a, o, splits, plan.gather, s, false)
+                              : launch_shape<false>(plan.shape, a, o, splits, plan.gather, s, false);
         if (e != hipSuccess) return e;
         if (splits > 1) {
             const size_t n = (size_t)rows * (a.npad / 8);
@@ -385,15 +842,18 @@ hipError_t launch_linear(const LinearCall& q, const LinearWork& ws, hipStream_t 
 
 hipError_t launch_unit_rows(const void* x, int type, int64_t ldx, int64_t M, int N, const UnitOut& o, hipStream_t s) {
     if (!x || !o.out || M <= 0 || N <= 0 || (o.gallery && N % 64)) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(unit_rows_kernel, dim3((unsigned)((M + 3) / 4)), dim3(256), 0, s, x, type, ldx, (int)M, N, o);
-    return hipGetLastError();
+    if (type == kF32) return unit_by_width<float>(x, ldx, M, N, o, s);
+    if (type == kBF16) return unit_by_width<__bf16>(x, ldx, M, N, o, s);
+    return unit_by_width<half_t>(x, ldx, M, N, o, s);
 }
 
 hipError_t linear_kernels_init() {
-    hipError_t e = hipFuncSetAttribute((const void*)linear_tile_kernel<false, 128, 128, 2, 2>, hipFuncAttributeMaxDynamicSharedMemorySize, 65536);
-    if (e == hipSuccess)
-        e = hipFuncSetAttribute((const void*)linear_tile_kernel<true, 128, 128, 2, 2>, hipFuncAttributeMaxDynamicSharedMemorySize, 65536);
-    return e;
+    for (int t = 0; t < kNumShapes; ++t) {
+        hipError_t e = launch_shape<false>(t, LinearIn{}, LinearOut{}, 1, false, nullptr, true);
+        if (e == hipSuccess) e = launch_shape<true>(t, LinearIn{}, LinearOut{}, 1, false, nullptr, true);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace frhot

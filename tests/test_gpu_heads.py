@@ -99,7 +99,7 @@ def run_and_check(ctx, m, n, k, dtype="f16", act="none", bias=True, residual=Non
     got = o[:m, :n].double()
     y, tol = layer64(x, w, b, act, r)
     tol = tol + rounding(y.abs() + tol, out)
-    bad = (got - y).abs() > tol
+    bad = ~((got - y).abs() <= tol)
     assert not bad.any(), (int(bad.sum()), ((got - y).abs() / tol).max())
     assert (o[m:] == 7).all() and (o[:m, n:] == 7).all() and (ob[:offo] == 7).all(), "wrote outside [M, N]"
     lin.close()
