@@ -5,6 +5,7 @@
 #include <dlfcn.h>
 
 #include <atomic>
+#include <chrono>
 #include <climits>
 #include <cmath>
 #include <cstdarg>
@@ -2598,12 +2599,15 @@ int page_check_disjoint(const int64_t* first, const int32_t* counts, int nruns, 
     return FRHOT_OK;
 }
 
-// Page-locked memory for a page call of the stream; mark behind the launch that reads it.
-int page_pin_take(frhot_ctx* c, size_t words, IndexPin** out) {
-    // a captured launch would read the list at every replay, long after another call has taken the memory
+int page_refuse_capture(frhot_ctx* c) {
+    // the galleries' host-side tables change with the call, not with a replay
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     HIP_TRY(hipStreamIsCapturing(c->stream, &st));
-    if (st != hipStreamCaptureStatusNone) return fail(FRHOT_ESTATE, "row lists cannot be captured into a graph");
+    if (st != hipStreamCaptureStatusNone) return fail(FRHOT_ESTATE, "page calls cannot be captured into a graph");
+    return FRHOT_OK;
+}
+// Page-locked memory for a page call of the stream; mark behind the launch that reads it.
+int page_pin_take(frhot_ctx* c, size_t words, IndexPin** out) {
     IndexPin& ip = c->page_pin[c->page_next++ & 3];
     const int rc = index_pin_grow(ip, words);
     *out = &ip;
@@ -2614,17 +2618,44 @@ int page_pin_mark(frhot_ctx* c, IndexPin* ip) {
     ip->pending = true;
     return FRHOT_OK;
 }
+// Waits until none of the n words that a kernel of the stream stores one by one is kUntold any more.  Polling spares the
+// event and the wake-up behind it (one store's collection freed: 22 -> 12 us); a kernel that takes long is waited for with the
+// stream, which also reports one that failed.
+constexpr int32_t kUntold = INT32_MIN;
+int page_await(frhot_ctx* c, volatile int32_t* words, size_t n) {
+    const auto t0 = std::chrono::steady_clock::now();
+    bool synced = false;
+    for (size_t i = 0; i < n; ++i)
+        for (int spin = 0; words[i] == kUntold; ++spin) {
+            __builtin_ia32_pause();
+            if (synced) return fail(FRHOT_EHIP, "a page kernel ended without its counts");
+            if ((spin & 255) == 255 && std::chrono::steady_clock::now() - t0 > std::chrono::milliseconds(2)) {
+                HIP_TRY(hipStreamSynchronize(c->stream));
+                synced = true;
+                std::atomic_thread_fence(std::memory_order_acquire);
+                if (words[i] != kUntold) break;
+            }
+        }
+    std::atomic_thread_fence(std::memory_order_acquire);
+    return FRHOT_OK;
+}
 
-// Runs -> items of at most kPageRows rows in page-locked memory, moved by one launch.  A null side's `first` counts from 0 on.
+// Runs -> items of at most kPageRows rows (in page-locked memory, if they are many), moved by one launch.  A null side's `first` counts from 0 on.
 int page_move_enqueue(frhot_ctx* c, const PageSide& src, const int64_t* src_first, const PageSide& dst, const int64_t* dst_first,
                       const int32_t* counts, const int32_t* keys, int nruns, int D) {
     size_t items = 0;
     for (int i = 0; i < nruns; ++i) items += (size_t)((counts ? counts[i] : 1) + kPageRows - 1) / kPageRows;
     if (items > 0x7fffffffu) return fail(FRHOT_ECAPACITY, "%zu row runs in one call", items);
-    IndexPin* ip = nullptr;
-    int rc = page_pin_take(c, items * (sizeof(PageItem) / 4) + 2, &ip);
+    int rc = page_refuse_capture(c);
     if (rc) return rc;
-    PageItem* it = (PageItem*)ip->p;
+    IndexPin* ip = nullptr;
+    PageItem few[kPageInline];
+    PageItem* it = few;
+    if (items > kPageInline) {
+        rc = page_pin_take(c, items * (sizeof(PageItem) / 4) + 2, &ip);
+        if (rc) return rc;
+        it = (PageItem*)ip->p;
+    }
     int64_t dense = 0;
     size_t k = 0;
     for (int i = 0; i < nruns; ++i) {
@@ -2634,8 +2665,8 @@ int page_move_enqueue(frhot_ctx* c, const PageSide& src, const int64_t* src_firs
             it[k++] = PageItem{s0 + at, d0 + at, n - at < kPageRows ? n - at : kPageRows, keys ? keys[i] : kKeepKey};
         dense += n;
     }
-    HIP_TRY(launch_page_move(src, dst, it, (int)items, D, c->stream));
-    return page_pin_mark(c, ip);
+    HIP_TRY(launch_page_move(src, dst, it, (int)items, dense, D, c->stream));
+    return ip ? page_pin_mark(c, ip) : FRHOT_OK;
 }
 
 // What a gallery's host-side tables know after the runs were written: `sorted` ascending destination runs, keys per run (in the
@@ -2651,10 +2682,15 @@ void page_note_writes(frhot_gallery* g, const std::vector<std::pair<int64_t, int
     g->dense = dense;
     g->nrows = end;
     if (!keys) { g->key_tiles_valid = false; return; }
-    for (int i = 0; i < nruns; ++i) {
-        if (keys[i] < 0) continue;
-        const int64_t last = first[i] + (counts ? counts[i] : 1) - 1;
-        for (int64_t r = first[i]; r <= last; r = ((r >> 8) + 1) << 8) key_tiles_add(g, &r, &keys[i], 1);
+    auto add = [&](int64_t lo, int64_t hi, int32_t key) {
+        if (key < 0) return;
+        for (int64_t r = lo; r < hi; r = ((r >> 8) + 1) << 8) key_tiles_add(g, &r, &key, 1);
+    };
+    // one key for all runs (a fork): in ascending order every tile goes to the end of the key's list
+    if (std::all_of(keys, keys + nruns, [&](int32_t k) { return k == keys[0]; })) {
+        for (const auto& r : sorted) add(r.first, r.second, keys[0]);
+    } else {
+        for (int i = 0; i < nruns; ++i) add(first[i], first[i] + (counts ? counts[i] : 1), keys[i]);
     }
 }
 
@@ -2758,6 +2794,10 @@ int frhot_gallery_free_keys(frhot_gallery* g, const int32_t* keys, int nkeys, in
     }
     // only the tiles that may hold one of the keys are looked at (all of them once the lists were given up)
     std::vector<int32_t> tiles;
+    std::vector<TileRun> runs;
+    auto add_run = [&](int32_t first, int32_t n) {
+        for (; n > 0; first += kFreeTiles, n -= kFreeTiles) runs.push_back(TileRun{first, n < kFreeTiles ? n : kFreeTiles});
+    };
     const bool listed = !g->key_tiles_off;
     if (listed) {
         for (int32_t k : want) {
@@ -2769,21 +2809,28 @@ int frhot_gallery_free_keys(frhot_gallery* g, const int32_t* keys, int nkeys, in
             tiles.erase(std::unique(tiles.begin(), tiles.end()), tiles.end());
         }
         if (tiles.empty()) return FRHOT_OK;
+        for (size_t i = 0, j; i < tiles.size(); i = j) {
+            for (j = i + 1; j < tiles.size() && tiles[j] == tiles[j - 1] + 1; ++j) {}
+            add_run(tiles[i], (int32_t)(j - i));
+        }
+    } else {
+        add_run(0, (int32_t)((g->nrows + 255) / 256));
     }
-    const size_t nt = listed ? tiles.size() : (size_t)((g->nrows + 255) / 256);
+    const size_t nr = runs.size();
     IndexPin* ip = nullptr;
-    int rc = page_pin_take(c, nt + want.size() + (listed ? nt : 0), &ip);
+    int rc = page_refuse_capture(c);
+    if (!rc) rc = page_pin_take(c, 3 * nr + want.size(), &ip);
     if (rc) return rc;
-    int32_t *counts = ip->p, *wk = ip->p + nt, *tl = wk + want.size();
+    TileRun* const rl = (TileRun*)ip->p;
+    int32_t *counts = ip->p + 2 * nr, *wk = counts + nr;
+    memcpy(rl, runs.data(), nr * sizeof(TileRun));
+    std::fill(counts, counts + nr, kUntold);
     memcpy(wk, want.data(), want.size() * 4);
-    if (listed) memcpy(tl, tiles.data(), nt * 4);
-    HIP_TRY(launch_page_free(g->keys, listed ? tl : nullptr, (int)nt, wk, (int)want.size(), counts, c->stream));
-    rc = page_pin_mark(c, ip);
+    HIP_TRY(launch_page_free(g->keys, rl, (int)nr, wk, (int)want.size(), counts, c->stream));
+    rc = page_await(c, counts, nr);         // (a run's count comes after its block has read the lists)
     if (rc) return rc;
-    HIP_TRY(hipEventSynchronize(ip->copied));
-    ip->pending = false;
     int64_t n = 0;
-    for (size_t i = 0; i < nt; ++i) n += counts[i];
+    for (size_t i = 0; i < nr; ++i) n += counts[i];
     if (n) g->dense = false;
     if (listed)
         for (int32_t k : want) {
@@ -2822,17 +2869,19 @@ int frhot_gallery_compact(frhot_gallery* src, frhot_gallery* dst, int64_t* new_r
             c->page_off_cap = cap;
         }
         IndexPin* ip = nullptr;
-        int rc = page_pin_take(c, 16, &ip);
+        int rc = page_refuse_capture(c);
+        if (!rc) rc = page_pin_take(c, 16, &ip);
         if (rc) return rc;
+        ip->p[0] = kUntold;
         if (dst && dst->capacity < src->nrows) {
             // the rows must fit, and only the device knows how many there are: count first
             HIP_TRY(launch_page_count(src->keys, src->nrows, c->page_off, ip->p, s));
-            rc = page_pin_mark(c, ip);
+            rc = page_await(c, ip->p, 1);
             if (rc) return rc;
-            HIP_TRY(hipEventSynchronize(ip->copied));
-            ip->pending = false;
             if (ip->p[0] > dst->capacity)
                 return fail(FRHOT_ECAPACITY, "%d live rows, capacity %lld", ip->p[0], (long long)dst->capacity);
+            HIP_TRY(hipStreamSynchronize(s));       // (nothing stores into the word any more)
+            ip->p[0] = kUntold;
         }
         void* rows = g->rows;
         int32_t* keys = g->keys;
@@ -2852,11 +2901,17 @@ int frhot_gallery_compact(frhot_gallery* src, frhot_gallery* dst, int64_t* new_r
             }
         }
         hipError_t e = launch_page_compact(src->rows, src->keys, src->nrows, rows, keys, old_rows, src->D, c->page_off, new_rows_dev, ip->p, s);
-        if (e == hipSuccess) e = hipEventRecord(ip->copied, s);
-        if (e == hipSuccess) e = hipEventSynchronize(ip->copied);
+        // into another gallery only the count is waited for (the first thing the kernels know); in place, the old rows are
+        // given back, so everything is
+        if (e == hipSuccess && !dst) e = hipStreamSynchronize(s);
         if (e != hipSuccess) {
-            if (!dst) { (void)hipFree(rows); (void)hipFree(keys); }
+            if (!dst) { (void)hipStreamSynchronize(s); (void)hipFree(rows); (void)hipFree(keys); }
             return fail(FRHOT_EHIP, "compacting failed: %s", hipGetErrorString(e));
+        }
+        rc = page_await(c, ip->p, 1);
+        if (rc) {
+            if (!dst) { (void)hipFree(rows); (void)hipFree(keys); }
+            return rc;
         }
         live = ip->p[0];
         if (!dst) {

@@ -193,12 +193,16 @@ constexpr int32_t kKeepKey = INT32_MIN;
 struct PageItem { int64_t src, dst; int32_t n, key; };     // n <= kPageRows rows src.. -> dst..; key: the new key or kKeepKey
 constexpr int kPageRows = 64;
 struct PageSide { void* rows; int32_t* keys; int dense; };  // a gallery's rows and keys, or a dense [n, D] buffer and its keys (or null)
-// `items` may lie in page-locked host memory (each is read once)
-hipError_t launch_page_move(const PageSide& src, const PageSide& dst, const PageItem* items, int n, int D, hipStream_t s);
-// Rows of the listed tiles (null: tiles 0 .. ntiles-1) whose key is one of keys[0..nkeys) (ascending) die; counts[i] = how many in tile i.
-hipError_t launch_page_free(int32_t* g_keys, const int32_t* tiles, int ntiles, const int32_t* keys, int nkeys, int32_t* counts, hipStream_t s);
+// Up to kPageInline items are read here and now; a longer list is read by the kernel (page-locked host memory will do).
+constexpr int kPageInline = 64;
+hipError_t launch_page_move(const PageSide& src, const PageSide& dst, const PageItem* items, int n, int64_t rows, int D, hipStream_t s);   // rows: of all items
+// Rows whose key is one of keys[0..nkeys) (ascending) die, in runs of at most kFreeTiles tiles; counts[i] = how many in run i, stored
+// for the host to poll (page-locked).  The lists are host memory, page-locked where they are longer than kFreeInline runs or one key.
+struct TileRun { int32_t first, n; };
+constexpr int kFreeTiles = 16, kFreeInline = 256;
+hipError_t launch_page_free(int32_t* g_keys, const TileRun* runs, int nruns, const int32_t* keys, int nkeys, int32_t* counts, hipStream_t s);
 // Live rows of src to the front of dst in order; dst's rows behind them (up to dst_rows) die.  offsets: ntiles(src) + 1 int32 of
-// scratch, the last of which receives the number of live rows, as does *total.
+// scratch, the last of which receives the number of live rows, as does *total (page-locked, stored for the host to poll).
 hipError_t launch_page_compact(const void* src, const int32_t* src_keys, int64_t src_rows, void* dst, int32_t* dst_keys, int64_t dst_rows,
                                int D, int32_t* offsets, int64_t* new_rows, int32_t* total, hipStream_t s);
 hipError_t launch_page_count(const int32_t* g_keys, int64_t rows, int32_t* offsets, int32_t* total, hipStream_t s);     // the first half of it

@@ -28,11 +28,24 @@ FR_DEV size_t piece_at(int64_t r, int j, int nk) {
 
 FR_DEV int ceil_log2(int n) { return n <= 1 ? 0 : 32 - __builtin_clz((unsigned)(n - 1)); }
 
+// NT: past the caches.  Moves of more than kStreamBytes gain 3 % by it (1 M rows of 512: 405 -> 393 us); smaller ones lose what the next
+// call would have found in the 256 MiB Infinity Cache (20,011 rows of 4096 squeezed, then read: 99 -> 105 us).
+constexpr size_t kStreamBytes = (size_t)512 << 20;
+template <bool NT>
+FR_DEV uint4v load16(const void* p) {
+    if constexpr (NT) return __builtin_nontemporal_load((const uint4v*)p);
+    return *(const uint4v*)p;
+}
+template <bool NT>
+FR_DEV void store16(void* p, uint4v v) {
+    if constexpr (NT) __builtin_nontemporal_store(v, (uint4v*)p);
+    else *(uint4v*)p = v;
+}
+
 // One item (a run of up to 64 rows) and `per` chunks of it per block; the pieces are taken chunk by chunk, rows fastest, a
 // power of two of row slots per chunk so that no index needs a division.
-template <bool SD, bool DD>
-__global__ __launch_bounds__(256) void page_move_kernel(PageSide src, PageSide dst, const PageItem* __restrict__ items, int nk, int per) {
-    const PageItem it = items[blockIdx.x];
+template <bool SD, bool DD, bool NT>
+FR_DEV void move_item(const PageSide& src, const PageSide& dst, const PageItem& it, int nk, int per) {
     const int j0 = blockIdx.y * per, j1 = min(nk, j0 + per);
     const int lg = ceil_log2(it.n), mask = (1 << lg) - 1;
     const int total = (j1 - j0) << (lg + 3);
@@ -44,35 +57,63 @@ __global__ __launch_bounds__(256) void page_move_kernel(PageSide src, PageSide d
         for (int u = 0; u < U; ++u) {
             const int idx = base + 256 * u;
             const int i = (idx >> 3) & mask, j = j0 + (idx >> (lg + 3));
-            if (idx < total && i < it.n) v[u] = *(const uint4v*)((const char*)src.rows + piece_at<SD>(it.src + i, j, nk) + part);
+            if (idx < total && i < it.n) v[u] = load16<NT>((const char*)src.rows + piece_at<SD>(it.src + i, j, nk) + part);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int idx = base + 256 * u;
             const int i = (idx >> 3) & mask, j = j0 + (idx >> (lg + 3));
-            if (idx < total && i < it.n) *(uint4v*)((char*)dst.rows + piece_at<DD>(it.dst + i, j, nk) + part) = v[u];
+            if (idx < total && i < it.n) store16<NT>((char*)dst.rows + piece_at<DD>(it.dst + i, j, nk) + part, v[u]);
         }
     }
     if (blockIdx.y == 0 && dst.keys && (int)threadIdx.x < it.n)
         dst.keys[it.dst + threadIdx.x] = it.key == kKeepKey ? src.keys[it.src + threadIdx.x] : it.key;
 }
+template <bool SD, bool DD, bool NT>
+__global__ __launch_bounds__(256) void page_move_kernel(PageSide src, PageSide dst, const PageItem* __restrict__ items, int nk, int per) {
+    const PageItem it = items[blockIdx.x];
+    move_item<SD, DD, NT>(src, dst, it, nk, per);
+}
+// Short lists travel in the kernel's arguments: one in host memory costs every block a trip over PCIe before its first load.
+struct InlineItems { PageItem it[kPageInline]; };
+template <bool SD, bool DD>
+__global__ __launch_bounds__(256) void page_move_inline_kernel(PageSide src, PageSide dst, InlineItems items, int nk, int per) {
+    const PageItem it = items.it[blockIdx.x];
+    move_item<SD, DD, false>(src, dst, it, nk, per);
+}
 
-__global__ __launch_bounds__(256) void page_free_kernel(int32_t* __restrict__ gk, const int32_t* __restrict__ tiles,
-                                                        const int32_t* __restrict__ keys, int nkeys, int32_t* __restrict__ counts) {
+// A value for the host, which polls page-locked memory for it.
+FR_DEV void tell_host(int32_t* p, int32_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM); }
+
+// One run of up to kFreeTiles tiles per block.
+FR_DEV void free_tiles(int32_t* __restrict__ gk, const TileRun& run, const int32_t* __restrict__ keys, int nkeys, int32_t* count) {
     __shared__ int red[4];
-    const int64_t r = (int64_t)(tiles ? tiles[blockIdx.x] : (int)blockIdx.x) * 256 + threadIdx.x;
-    const int32_t k = gk[r];
-    int lo = 0, hi = nkeys;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (keys[mid] < k) lo = mid + 1; else hi = mid;
+    int mine = 0;
+    for (int t = 0; t < run.n; ++t) {
+        const int64_t r = (int64_t)(run.first + t) * 256 + threadIdx.x;
+        const int32_t k = gk[r];
+        int lo = 0, hi = nkeys;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (keys[mid] < k) lo = mid + 1; else hi = mid;
+        }
+        const bool hit = lo < nkeys && keys[lo] == k;
+        if (hit) gk[r] = kDead;
+        mine += __popcll(__ballot(hit));
     }
-    const bool hit = lo < nkeys && keys[lo] == k;
-    if (hit) gk[r] = kDead;
-    const int c = __popcll(__ballot(hit));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = c;
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mine;
     __syncthreads();
-    if (threadIdx.x == 0) counts[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+    if (threadIdx.x == 0) tell_host(count, red[0] + red[1] + red[2] + red[3]);
+}
+__global__ __launch_bounds__(256) void page_free_kernel(int32_t* __restrict__ gk, const TileRun* __restrict__ runs,
+                                                        const int32_t* __restrict__ keys, int nkeys, int32_t* __restrict__ counts) {
+    const TileRun run = runs[blockIdx.x];
+    free_tiles(gk, run, keys, nkeys, counts + blockIdx.x);
+}
+struct InlineRuns { TileRun run[kFreeInline]; };
+__global__ __launch_bounds__(256) void page_free_inline_kernel(int32_t* __restrict__ gk, InlineRuns runs, int32_t key, int32_t* __restrict__ counts) {
+    const TileRun run = runs.run[blockIdx.x];
+    free_tiles(gk, run, &key, 1, counts + blockIdx.x);
 }
 
 // live rows of every tile; a wave takes one tile
@@ -114,10 +155,47 @@ __global__ __launch_bounds__(1024) void page_scan_kernel(int32_t* __restrict__ o
         carry += all;
         __syncthreads();
     }
-    if (tid == 0) { offsets[n] = carry; *total = carry; }
+    if (tid == 0) { offsets[n] = carry; tell_host(total, carry); }
+}
+
+// Both at once for up to kSmallTiles tiles (65,536 rows): a launch less.
+constexpr int kSmallTiles = 256;
+__global__ __launch_bounds__(1024) void page_count_scan_kernel(const int32_t* __restrict__ gk, int64_t rows, int ntiles, int32_t* __restrict__ offsets,
+                                                               int32_t* __restrict__ total) {
+    __shared__ int cnt[kSmallTiles];
+    __shared__ int wsum[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    for (int t = wave; t < ntiles; t += 16) {
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t r = (int64_t)t * 256 + i * 64 + lane;
+            c += __popcll(__ballot(r < rows && gk[r < rows ? r : 0] >= 0));
+        }
+        if (lane == 0) cnt[t] = c;
+    }
+    __syncthreads();
+    const int c = tid < ntiles ? cnt[tid] : 0;          // (ntiles <= 256: the first four waves)
+    int v = c;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+        const int u = __shfl_up(v, s);
+        if (lane >= s) v += u;
+    }
+    if (wave < 4 && lane == 63) wsum[wave] = v;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        before += w < wave ? wsum[w] : 0;
+        all += wsum[w];
+    }
+    if (tid < ntiles) offsets[tid] = before + v - c;
+    if (tid == 0) { offsets[ntiles] = all; tell_host(total, all); }
 }
 
 // One tile of the source and `per` chunks of it per block: its live rows, in order, go to dst rows offsets[tile] and up.
+template <bool NT>
 __global__ __launch_bounds__(256) void page_compact_kernel(const char* __restrict__ src, const int32_t* __restrict__ sk, int64_t src_rows, int ntiles,
                                                            char* __restrict__ dst, int32_t* __restrict__ dk, int64_t dst_rows, int nk,
                                                            int per, const int32_t* __restrict__ offsets, int64_t* __restrict__ new_rows) {
@@ -157,13 +235,13 @@ __global__ __launch_bounds__(256) void page_compact_kernel(const char* __restric
         for (int u = 0; u < U; ++u) {
             const int idx = base + 256 * u;
             const int i = (idx >> 3) & mask, j = j0 + (idx >> (lg + 3));
-            if (idx < total && i < live) v[u] = *(const uint4v*)(src + tiled_at((int64_t)t * 256 + list[i], j, nk) + part);
+            if (idx < total && i < live) v[u] = load16<NT>(src + tiled_at((int64_t)t * 256 + list[i], j, nk) + part);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int idx = base + 256 * u;
             const int i = (idx >> 3) & mask, j = j0 + (idx >> (lg + 3));
-            if (idx < total && i < live) *(uint4v*)(dst + tiled_at(first + i, j, nk) + part) = v[u];
+            if (idx < total && i < live) store16<NT>(dst + tiled_at(first + i, j, nk) + part, v[u]);
         }
     }
 }
@@ -183,25 +261,49 @@ __global__ __launch_bounds__(256) void page_kill_kernel(int32_t* __restrict__ gk
 
 }  // namespace
 
-hipError_t launch_page_move(const PageSide& src, const PageSide& dst, const PageItem* items, int n, int D, hipStream_t s) {
-    if (!src.rows || !dst.rows || !items || n <= 0 || D <= 0 || D % 64 || (src.dense && dst.dense)) return hipErrorInvalidValue;
-    const int nk = D / 64, per = 8;
+hipError_t launch_page_move(const PageSide& src, const PageSide& dst, const PageItem* items, int n, int64_t rows, int D, hipStream_t s) {
+    if (!src.rows || !dst.rows || !items || n <= 0 || rows <= 0 || D <= 0 || D % 64 || (src.dense && dst.dense)) return hipErrorInvalidValue;
+    // one chunk a block while that makes no more than four blocks per CU, up to about 64 KiB a block beyond (256-row items of two
+    // chunks a block: 411 us for 1 M rows of 512 against 404)
+    const int nk = D / 64;
+    int per = 1;
+    while (per < nk && rows / n * per < 400 && (int64_t)n * ((nk + per - 1) / per) > 1024) per *= 2;
     const dim3 grid((unsigned)n, (unsigned)((nk + per - 1) / per));
-    if (src.dense) hipLaunchKernelGGL((page_move_kernel<true, false>), grid, dim3(256), 0, s, src, dst, items, nk, per);
-    else if (dst.dense) hipLaunchKernelGGL((page_move_kernel<false, true>), grid, dim3(256), 0, s, src, dst, items, nk, per);
-    else hipLaunchKernelGGL((page_move_kernel<false, false>), grid, dim3(256), 0, s, src, dst, items, nk, per);
+    if (n <= kPageInline) {
+        InlineItems list;
+        for (int i = 0; i < kPageInline; ++i) list.it[i] = items[i < n ? i : 0];
+        if (src.dense) hipLaunchKernelGGL((page_move_inline_kernel<true, false>), grid, dim3(256), 0, s, src, dst, list, nk, per);
+        else if (dst.dense) hipLaunchKernelGGL((page_move_inline_kernel<false, true>), grid, dim3(256), 0, s, src, dst, list, nk, per);
+        else hipLaunchKernelGGL((page_move_inline_kernel<false, false>), grid, dim3(256), 0, s, src, dst, list, nk, per);
+        return hipGetLastError();
+    }
+    const bool nt = (size_t)rows * D * 2 >= kStreamBytes;
+    const auto kern = src.dense   ? (nt ? page_move_kernel<true, false, true> : page_move_kernel<true, false, false>)
+                      : dst.dense ? (nt ? page_move_kernel<false, true, true> : page_move_kernel<false, true, false>)
+                                  : (nt ? page_move_kernel<false, false, true> : page_move_kernel<false, false, false>);
+    hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, src, dst, items, nk, per);
     return hipGetLastError();
 }
 
-hipError_t launch_page_free(int32_t* gk, const int32_t* tiles, int ntiles, const int32_t* keys, int nkeys, int32_t* counts, hipStream_t s) {
-    if (!gk || !keys || !counts || ntiles <= 0 || nkeys <= 0) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(page_free_kernel, dim3((unsigned)ntiles), dim3(256), 0, s, gk, tiles, keys, nkeys, counts);
+hipError_t launch_page_free(int32_t* gk, const TileRun* runs, int nruns, const int32_t* keys, int nkeys, int32_t* counts, hipStream_t s) {
+    if (!gk || !runs || !keys || !counts || nruns <= 0 || nkeys <= 0) return hipErrorInvalidValue;
+    if (nruns <= kFreeInline && nkeys == 1) {
+        InlineRuns list;
+        for (int i = 0; i < kFreeInline; ++i) list.run[i] = runs[i < nruns ? i : 0];
+        hipLaunchKernelGGL(page_free_inline_kernel, dim3((unsigned)nruns), dim3(256), 0, s, gk, list, keys[0], counts);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL(page_free_kernel, dim3((unsigned)nruns), dim3(256), 0, s, gk, runs, keys, nkeys, counts);
     return hipGetLastError();
 }
 
 hipError_t launch_page_count(const int32_t* gk, int64_t rows, int32_t* offsets, int32_t* total, hipStream_t s) {
     if (!gk || !offsets || !total || rows <= 0) return hipErrorInvalidValue;
     const int ntiles = (int)((rows + 255) / 256);
+    if (ntiles <= kSmallTiles) {
+        hipLaunchKernelGGL(page_count_scan_kernel, dim3(1), dim3(1024), 0, s, gk, rows, ntiles, offsets, total);
+        return hipGetLastError();
+    }
     hipLaunchKernelGGL(page_count_kernel, dim3((unsigned)((ntiles + 3) / 4)), dim3(256), 0, s, gk, rows, ntiles, offsets);
     hipLaunchKernelGGL(page_scan_kernel, dim3(1), dim3(1024), 0, s, offsets, ntiles, total);
     return hipGetLastError();
@@ -214,7 +316,8 @@ hipError_t launch_page_compact(const void* src, const int32_t* sk, int64_t src_r
     const hipError_t e = launch_page_count(sk, src_rows, offsets, total, s);
     if (e != hipSuccess) return e;
     const dim3 grid((unsigned)(ntiles > dtiles ? ntiles : dtiles), (unsigned)((nk + per - 1) / per));
-    hipLaunchKernelGGL(page_compact_kernel, grid, dim3(256), 0, s, (const char*)src, sk, src_rows, ntiles, (char*)dst, dk, dst_rows, nk, per,
+    const auto kern = (size_t)src_rows * D * 2 >= kStreamBytes ? page_compact_kernel<true> : page_compact_kernel<false>;
+    hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, (const char*)src, sk, src_rows, ntiles, (char*)dst, dk, dst_rows, nk, per,
                        (const int32_t*)offsets, new_rows);
     return hipGetLastError();
 }

@@ -349,15 +349,23 @@ class Head:
                                        self.dout if ldo is None else ldo))
 
 
+def _list(a, dtype):
+    if type(a) is np.ndarray and a.dtype == dtype and a.ndim == 1 and a.flags.c_contiguous:
+        return a
+    return np.ascontiguousarray(a, dtype=dtype).reshape(-1)
+
+
 def _runs(rows, counts, keys=None):
     """Run lists as the ABI takes them; keys: one for all, one per run, or None."""
-    rows = np.ascontiguousarray(rows, dtype=np.int64).reshape(-1)
+    rows = _list(rows, np.int64)
     if counts is not None:
-        counts = np.ascontiguousarray(counts, dtype=np.int32).reshape(-1)
+        counts = _list(counts, np.int32)
         if counts.size != rows.size:
             raise ValueError(f"{counts.size} run lengths for {rows.size} runs")
     if keys is not None:
-        keys = np.ascontiguousarray(np.broadcast_to(np.asarray(keys, dtype=np.int32), rows.shape))
+        keys = _list(keys, np.int32)
+        if keys.size != rows.size:
+            keys = np.ascontiguousarray(np.broadcast_to(keys, rows.shape))
     return rows, counts, keys
 
 

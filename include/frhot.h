@@ -451,7 +451,7 @@ int frhot_ctx_head(frhot_ctx* ctx, frhot_head* head);
  *   previous content is gone, or of the gallery itself (dst NULL or src: needs room for a second copy
  *   while it runs); new_rows_dev, if not NULL, receives every old row's new place (int64 [rows of src],
  *   device; -1 for dead ones) and *live (may be NULL) their number.  Scores of a search stay what they were,
- *   and so does the order of equal scores.  Waits.
+ *   and so does the order of equal scores.  Waits for the count (in place: for the whole).
  * frhot_gallery_reproject: row r of dst becomes the head's output for row r of src, with its key
  *   (dead rows stay dead; dst's previous content is gone).  How an enrolled gallery moves to a head:
  *   src holds descriptors (or another head's rows), dst has the head's output dimension.  Enqueues only.
