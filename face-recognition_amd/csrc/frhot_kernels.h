@@ -161,7 +161,7 @@ inline int linear_kpad(int K) { return (K + 63) / 64 * 64; }
 struct LinearOut {
     void* out; int64_t ldo; int otype;
     const void* res; int64_t ldr; int rtype;        // residual added after the activation, or null
-    int act, N, vec_out, vec_res;                   // (N and vec_*: filled in by launch_linear)
+    int act, N;                                     // (N: filled in by launch_linear)
 };
 struct LinearIn {
     const void* x; int64_t ldx; size_t xtile; int tiled, xstep;

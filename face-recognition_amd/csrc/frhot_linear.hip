@@ -57,8 +57,39 @@ FR_DEV void store1(void* p, size_t i, int type, float v) {
     else ((half_t*)p)[i] = (half_t)v;
 }
 
-// The activation in fp32.  Written so that each keeps its relative accuracy far out (gelu through erfc, the tanh form
-// through its logistic equivalent) and NaN stays NaN (a maximum with zero would turn it into zero).
+// exp(x + lo) for x <= 0 as exp2 of the rounded product, the product's rounding put back to first order: within 3 units of
+// 2^-24 of its value down to fp32's normal range (x > -87), below that zero.
+FR_DEV float exp_neg(float x, float lo) {
+    const float t = x * 1.44269504f;
+    float r = __builtin_fmaf(x, 1.44269504f, -t);
+    r = __builtin_fmaf(x, 1.92596299e-8f, r);
+    r = __builtin_fmaf(lo, 1.44269504f, r);
+    const float p = __builtin_amdgcn_exp2f(t);
+    return __builtin_fmaf(p, r * 0.693147181f, p);
+}
+// 1 / (1 + exp(-x)), from exp(-|x|) so that nothing overflows; the hardware's reciprocal is off by at most one unit.
+FR_DEV float logistic(float x) {
+    const float e = exp_neg(fmaxf(-fabsf(x), -200.f), 0.f);
+    const float q = __builtin_amdgcn_rcpf(1.f + e);
+    return x < 0.f ? e * q : q;
+}
+// The normal distribution's function: erfc(z) = exp(-z^2) erfcx(z) with erfcx(z) = t P(t), t = 1 / (1 + z / 2), z = |v| / sqrt 2; P of
+// degree 9 is a least-squares fit to scipy's erfcx over z = 0..10, reweighted towards an even relative error (2e-8; 2.9e-7 as
+// evaluated in fp32).  v^2 is carried with its rounding.
+FR_DEV float normal_cdf(float v) {
+    constexpr float C[10] = {0.282064497f, 0.282857031f, 0.238644838f, 0.22554186f, -0.0983176306f, 0.421274275f, -0.670022488f, 0.428928405f, -0.123254694f, 0.0122838775f};
+    const float a = fminf(fabsf(v), 100.f);
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(a, 0.353553391f, 1.f));
+    float p = C[9];
+#pragma unroll
+    for (int i = 8; i >= 0; --i) p = __builtin_fmaf(p, t, C[i]);
+    const float s = a * a, lo = __builtin_fmaf(a, a, -s);
+    const float h = 0.5f * p * t * exp_neg(-0.5f * s, -0.5f * lo);      // erfc(z) / 2
+    return v < 0.f ? h : 1.f - h;
+}
+// The activations in fp32.  Each keeps its relative accuracy far out, and NaN stays NaN (a maximum with zero would turn it into
+// zero).  With the library's expf and erfcf and an IEEE division, silu / gelu / tanh gelu of 21,888 x 1568 values cost 22 / 38 / 25 us
+// on top of the 36 us of the product without one; these forms 7 / 26 / 10 us.
 template <int W>
 FR_DEV void activate(float (&v)[W], int act) {
     if (act == kActRelu) {
@@ -66,19 +97,21 @@ FR_DEV void activate(float (&v)[W], int act) {
         for (int j = 0; j < W; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];
     } else if (act == kActSilu) {
 #pragma unroll
-        for (int j = 0; j < W; ++j) v[j] = v[j] / (1.f + expf(-v[j]));
+        for (int j = 0; j < W; ++j) v[j] = v[j] * logistic(v[j]);
     } else if (act == kActGelu) {
 #pragma unroll
-        for (int j = 0; j < W; ++j) v[j] = 0.5f * v[j] * erfcf(v[j] * -0.70710678118654752f);
-    } else if (act == kActGeluTanh) {
+        for (int j = 0; j < W; ++j) v[j] = v[j] * normal_cdf(v[j]);
+    } else if (act == kActGeluTanh) {       // (1 + tanh u) / 2 = logistic(2 u)
 #pragma unroll
-        for (int j = 0; j < W; ++j) v[j] = v[j] / (1.f + expf(-1.5957691216057308f * (v[j] + 0.044715f * v[j] * v[j] * v[j])));
+        for (int j = 0; j < W; ++j) v[j] = v[j] * logistic(1.59576912f * __builtin_fmaf(0.044715f * v[j] * v[j], v[j], v[j]));
     }
 }
 
-template <typename T, int W> struct vect { typedef T type __attribute__((ext_vector_type(W))); };
+// W elements at any address their type may have: this memory takes 16-byte accesses at such addresses, so odd widths and row
+// distances need no code of their own (21,897 x 24 x 1561 to fp32: 109 us with a store per element).
+template <typename T, int W> struct vect { typedef T type __attribute__((ext_vector_type(W), aligned(sizeof(T)))); };
 
-// W (4 or 8) consecutive channels n .. n+W-1 of row m: bias, activation, residual.
+// W consecutive channels n .. n+W-1 of row m: bias, activation, residual.
 template <int W>
 FR_DEV void load_bias(const float* __restrict__ bias, int n, float (&b)[W]) {      // (padded with zeros to whole panels)
 #pragma unroll
@@ -95,7 +128,7 @@ FR_DEV void epilogue(const LinearOut& o, const float (&b)[W], size_t m, int n, f
     activate<W>(v, o.act);
     if (o.res) {
         const size_t at = m * (size_t)o.ldr + n;
-        if (n + W <= o.N && o.vec_res) {
+        if (n + W <= o.N) {
             if (o.rtype == kF32) {
                 const auto r = *(const typename vect<float, W>::type*)((const float*)o.res + at);
 #pragma unroll
@@ -123,10 +156,10 @@ FR_DEV void finish(const LinearOut& o, const float (&b)[W], size_t m, int n, flo
     if (n >= o.N) return;
     epilogue<W>(o, b, m, n, v);
     const size_t at = m * (size_t)o.ldo + n;
-    if (n + W <= o.N && o.vec_out) {
+    if (n + W <= o.N) {
         if (o.otype == kF32) {
 #pragma unroll
-            for (int j = 0; j < W; j += 4) *(float4v*)((float*)o.out + at + j) = float4v{v[j], v[j + 1], v[j + 2], v[j + 3]};
+            for (int j = 0; j < W; j += 4) *(typename vect<float, 4>::type*)((float*)o.out + at + j) = typename vect<float, 4>::type{v[j], v[j + 1], v[j + 2], v[j + 3]};
         } else if (o.otype == kBF16) {
             typename vect<__bf16, W>::type t;
 #pragma unroll
@@ -143,6 +176,18 @@ FR_DEV void finish(const LinearOut& o, const float (&b)[W], size_t m, int n, flo
         for (int j = 0; j < W; ++j)
             if (n + j < o.N) store1(o.out, at + j, o.otype, v[j]);
     }
+}
+
+// Eight 16-bit elements at any address, zeros from the n-th on (nothing behind them is read).
+FR_DEV uint4v load_tail(const uint16_t* p, int n) {
+    if (n >= 8) return __builtin_bit_cast(uint4v, *(const vect<uint16_t, 8>::type*)p);
+    uint4v o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const unsigned lo = 2 * e < n ? p[2 * e] : 0u, hi = 2 * e + 1 < n ? p[2 * e + 1] : 0u;
+        o[e] = lo | (hi << 16);
+    }
+    return o;
 }
 
 // w [N][K] -> fragments (see the head of the file); thread = one lane's 16 bytes of one fragment
@@ -164,22 +209,15 @@ __global__ __launch_bounds__(256) void linear_layout_kernel(const uint16_t* __re
     *(uint4v*)(wt + t * 8) = o;
 }
 
-// Rows whose addresses the 16-byte loads cannot take (odd strides, K not a multiple of 8) are first brought into rows of
-// `kpad` elements with zeros behind the K-th.
+// Rows whose addresses LDS-DMA cannot take (odd strides, K not a multiple of 8) are first brought into rows of `kpad` elements
+// with zeros behind the K-th.
 __global__ __launch_bounds__(256) void linear_pack_kernel(const uint16_t* __restrict__ x, int64_t ldx, int K, int kpad,
                                                           uint16_t* __restrict__ out, int rows) {
     const int per_row = kpad >> 3;
     const size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
     if (t >= (size_t)rows * per_row) return;
     const int r = (int)(t / per_row), k0 = (int)(t % per_row) * 8;
-    const uint16_t* src = x + (size_t)r * ldx + k0;
-    uint4v o;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const unsigned lo = k0 + 2 * e < K ? src[2 * e] : 0u, hi = k0 + 2 * e + 1 < K ? src[2 * e + 1] : 0u;
-        o[e] = lo | (hi << 16);
-    }
-    *(uint4v*)(out + t * 8) = o;
+    *(uint4v*)(out + t * 8) = load_tail(x + (size_t)r * ldx + k0, K - k0);
 }
 
 // The tile kernel: TM x TN of y (or of a K slice's partial sums) at a time, 64 K-elements per step.  X and W stages arrive by
@@ -386,7 +424,7 @@ __global__ __launch_bounds__(64 * WX * WY) void linear_tile_kernel(LinearIn a, L
 // wave order, through LDS.  Weight fragments (1 KiB of consecutive bytes) are loaded straight into registers; X goes through
 // LDS by LDS-DMA, eight rows of 128 bytes an instruction: in fragment order consecutive lanes read different rows, which the
 // load path serves 16 bytes a clock (38 GB/s per CU measured, against 110-145 for whole lines).
-// GATHER: rows that 16-byte loads cannot take, element by element into registers.
+// GATHER: rows that LDS-DMA cannot take (not 16-byte aligned, K not a multiple of 8), by unaligned loads into registers.
 template <int FX, int FW, int NW, int ST>
 struct WaveShape {
     static constexpr int TM = 16 * FX, TN = 16 * FW, ER = TN + 4;
@@ -437,14 +475,7 @@ __global__ __launch_bounds__(64 * NW) void linear_wave_kernel(LinearIn a, Linear
                 for (int y = 0; y < FW; ++y) vw[y] = *(const uint4v*)(wp[y] + (size_t)ks * wstep + kk * 1024);
                 const int k0 = ks * 64 + kk * 32 + g0 * 8;
 #pragma unroll
-                for (int x = 0; x < FX; ++x) {
-                    const uint16_t* e = (const uint16_t*)xp[x] + k0;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const unsigned lo = k0 + 2 * j < a.K ? e[2 * j] : 0u, hi = k0 + 2 * j + 1 < a.K ? e[2 * j + 1] : 0u;
-                        vx[x][j] = lo | (hi << 16);
-                    }
-                }
+                for (int x = 0; x < FX; ++x) vx[x] = load_tail((const uint16_t*)xp[x] + k0, a.K - k0);
 #pragma unroll
                 for (int x = 0; x < FX; ++x)
 #pragma unroll
@@ -522,37 +553,31 @@ __global__ __launch_bounds__(64 * NW) void linear_wave_kernel(LinearIn a, Linear
         __syncthreads();                                    // the sums take the stages' place
     }
 
-    // consecutive channels a lane finishes: eight; four where the tile is half a pair of panels
-    constexpr int CH = FW == 1 ? 4 : 8;
     float* const part = (float*)smem;
     float* const mine = part + wave * TM * ER;
 #pragma unroll
     for (int x = 0; x < FX; ++x)
 #pragma unroll
-        for (int y = 0; y < FW; ++y) *(float4v*)(mine + (x * 16 + l15) * ER + (y >> 1) * 32 + g0 * CH + (y & 1) * 4) = acc[y][x];
+        for (int y = 0; y < FW; ++y) *(float4v*)(mine + (x * 16 + l15) * ER + (y >> 1) * 32 + g0 * 8 + (y & 1) * 4) = acc[y][x];
     __syncthreads();
-    for (int i = tid; i < TM * (TN / CH); i += 64 * NW) {
-        const int r = i / (TN / CH), m = m0 + r, cn = (i % (TN / CH)) * CH;
-        const int ch = FW == 1 ? (n0 >> 5) * 32 + cn * 2 + ((n0 >> 4) & 1) * 4 : n0 + cn;
+    for (int i = tid; i < TM * (TN / 8); i += 64 * NW) {
+        const int r = i / (TN / 8), m = m0 + r, cn = (i % (TN / 8)) * 8, ch = n0 + cn;
         if (m >= a.M || ch >= a.npad) continue;
-        float bv[CH], v[CH] = {};
-        load_bias<CH>(a.bias, ch, bv);
+        float bv[8], v[8] = {};
+        load_bias<8>(a.bias, ch, bv);
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
             const float* p = part + w * TM * ER + r * ER + cn;
+            const float4v p0 = *(const float4v*)p, p1 = *(const float4v*)(p + 4);
 #pragma unroll
-            for (int q = 0; q < CH; q += 4) {
-                const float4v t = *(const float4v*)(p + q);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[q + j] += t[j];
-            }
+            for (int j = 0; j < 4; ++j) { v[j] += p0[j]; v[4 + j] += p1[j]; }
         }
         if (a.slab) {
             float* d = a.slab + ((size_t)z * a.M + m) * a.npad + ch;
-#pragma unroll
-            for (int q = 0; q < CH; q += 4) *(float4v*)(d + q) = float4v{v[q], v[q + 1], v[q + 2], v[q + 3]};
+            *(float4v*)d = float4v{v[0], v[1], v[2], v[3]};
+            *(float4v*)(d + 4) = float4v{v[4], v[5], v[6], v[7]};
         } else {
-            finish<CH>(o, bv, m, ch, v);
+            finish<8>(o, bv, m, ch, v);
         }
     }
 }
@@ -563,7 +588,8 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearIn a, LinearOut 
     const size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
     if (t >= (size_t)a.M * per_row) return;
     const int m = (int)(t / per_row), n = (int)(t % per_row) * 8;
-    float v[8] = {};
+    float bv[8], v[8] = {};
+    load_bias<8>(a.bias, n, bv);
     const float* p = a.slab + (size_t)m * a.npad + n;
     const size_t step = (size_t)a.M * a.npad;
     for (int z = 0; z < splits; z += 4) {           // four slices in flight, added in slice order
@@ -578,8 +604,6 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearIn a, LinearOut 
                 for (int j = 0; j < 4; ++j) { v[j] += q[i][0][j]; v[4 + j] += q[i][1][j]; }
             }
     }
-    float bv[8];
-    load_bias<8>(a.bias, n, bv);
     finish<8>(o, bv, m, n, v);
 }
 
@@ -587,16 +611,17 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearIn a, LinearOut 
 // The norm comes from a 64-bit sum of squares rounded to fp32, then one IEEE division per element: the stored row is the same
 // whatever the summation order, and the same as the library's own upload makes of it (gallery_upsert_kernel).  A row
 // shorter than 1e-30 is divided by one.
-// L lanes a row, each R vectors of V consecutive elements in registers: x is read once.  R = 0: rows too long for that, or
-// that V does not divide or align, are read twice (the second time out of the cache).
+// L lanes a row, each R vectors of V consecutive elements (16 bytes, at any address) in registers: x is read once.  R = 0: rows too
+// long for that are read twice, the second time out of the cache.
 template <typename T, int V>
-FR_DEV void load_vec(const T* p, float (&v)[V]) {
-    if constexpr (V == 1) {
-        v[0] = (float)*p;
-    } else {
+FR_DEV void load_row(const T* p, int n, float (&v)[V]) {
+    if (n >= V) {
         const auto t = *(const typename vect<T, V>::type*)p;
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] = (float)t[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = j < n ? (float)p[j] : 0.f;
     }
 }
 template <int V>
@@ -608,18 +633,23 @@ FR_DEV void store_unit(const UnitOut& o, int N, int m, int c, const float (&v)[V
     } else {
         d = (half_t*)o.out + (size_t)m * o.ldo + c;
     }
-    if constexpr (V == 1) {
-        *d = (half_t)__fdiv_rn(v[0], nrm);
-    } else {
-        typename vect<half_t, V>::type t;
+    half_t t[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) t[j] = (half_t)__fdiv_rn(v[j], nrm);
-        *(typename vect<half_t, V>::type*)d = t;
+    for (int j = 0; j < V; ++j) t[j] = (half_t)__fdiv_rn(v[j], nrm);
+    if (c + V <= N) {
+        typename vect<half_t, V>::type u;
+#pragma unroll
+        for (int j = 0; j < V; ++j) u[j] = t[j];
+        *(typename vect<half_t, V>::type*)d = u;
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (c + j < N) d[j] = t[j];
     }
 }
-template <typename T, int L, int V, int R>
+template <typename T, int L, int R>
 __global__ __launch_bounds__(256) void unit_rows_kernel(const T* __restrict__ x, int64_t ldx, int M, int N, UnitOut o) {
-    constexpr int RB = 256 / L;             // rows a block
+    constexpr int V = 16 / sizeof(T), RB = 256 / L;             // RB rows a block
     const int m = blockIdx.x * RB + threadIdx.x / L, l = threadIdx.x % L;
     if (m >= M) return;                     // (the lanes of a row leave together)
     const T* const row = x + (size_t)m * ldx;
@@ -629,7 +659,7 @@ __global__ __launch_bounds__(256) void unit_rows_kernel(const T* __restrict__ x,
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const int c = (i * L + l) * V;
-            if (c < N) load_vec<T, V>(row + c, v[i]);
+            if (c < N) load_row<T, V>(row + c, N - c, v[i]);
         }
 #pragma unroll
         for (int i = 0; i < R; ++i)
@@ -639,7 +669,7 @@ __global__ __launch_bounds__(256) void unit_rows_kernel(const T* __restrict__ x,
             }
     } else {
         for (int c = l * V; c < N; c += L * V) {
-            load_vec<T, V>(row + c, v[0]);
+            load_row<T, V>(row + c, N - c, v[0]);
 #pragma unroll
             for (int j = 0; j < V; ++j) ss += (double)v[0][j] * (double)v[0][j];
         }
@@ -656,30 +686,27 @@ __global__ __launch_bounds__(256) void unit_rows_kernel(const T* __restrict__ x,
         }
     } else {
         for (int c = l * V; c < N; c += L * V) {
-            load_vec<T, V>(row + c, v[0]);
+            load_row<T, V>(row + c, N - c, v[0]);
             store_unit<V>(o, N, m, c, v[0], nrm);
         }
     }
     if (l == 0 && o.keys_dst) o.keys_dst[o.row0 + m] = o.keys_src[o.row0 + m];
 }
 
-template <typename T, int L, int V, int R>
+template <typename T, int L, int R>
 hipError_t launch_unit(const void* x, int64_t ldx, int64_t M, int N, const UnitOut& o, hipStream_t s) {
     const int64_t rb = 256 / L;
-    hipLaunchKernelGGL((unit_rows_kernel<T, L, V, R>), dim3((unsigned)((M + rb - 1) / rb)), dim3(256), 0, s, (const T*)x, ldx, (int)M, N, o);
+    hipLaunchKernelGGL((unit_rows_kernel<T, L, R>), dim3((unsigned)((M + rb - 1) / rb)), dim3(256), 0, s, (const T*)x, ldx, (int)M, N, o);
     return hipGetLastError();
 }
 template <typename T>
 hipError_t unit_by_width(const void* x, int64_t ldx, int64_t M, int N, const UnitOut& o, hipStream_t s) {
     constexpr int V = 16 / sizeof(T);
-    const bool vec = N % V == 0 && ldx % V == 0 && (size_t)x % 16 == 0 &&
-                     (o.gallery || (o.ldo % V == 0 && (size_t)o.out % (V * 2) == 0));
-    if (!vec) return N <= 256 ? launch_unit<T, 16, 1, 0>(x, ldx, M, N, o, s) : launch_unit<T, 64, 1, 0>(x, ldx, M, N, o, s);
-    if (N <= 16 * V) return launch_unit<T, 4, V, 4>(x, ldx, M, N, o, s);
-    if (N <= 64 * V) return launch_unit<T, 16, V, 4>(x, ldx, M, N, o, s);
-    if (N <= 256 * V) return launch_unit<T, 64, V, 4>(x, ldx, M, N, o, s);
-    if (N <= 1024 * V) return launch_unit<T, 64, V, 16>(x, ldx, M, N, o, s);
-    return launch_unit<T, 64, V, 0>(x, ldx, M, N, o, s);
+    if (N <= 16 * V) return launch_unit<T, 4, 4>(x, ldx, M, N, o, s);
+    if (N <= 64 * V) return launch_unit<T, 16, 4>(x, ldx, M, N, o, s);
+    if (N <= 256 * V) return launch_unit<T, 64, 4>(x, ldx, M, N, o, s);
+    if (N <= 1024 * V) return launch_unit<T, 64, 16>(x, ldx, M, N, o, s);
+    return launch_unit<T, 64, 0>(x, ldx, M, N, o, s);
 }
 
 template <bool BF, int TM, int TN, int WX, int WY, int XS, int WS>
@@ -752,9 +779,9 @@ hipError_t launch_shape(int t, const LinearIn& a, const LinearOut& o, int splits
 
 // What a call runs as: the shape, the number of K slices and the way unaligned rows go in, whichever an estimate of the
 // time puts first.  A round of at most 256 tiles takes its K steps; K slices divide the steps and add the join (a launch, and
-// every slice's sums written and read once: 4.5 us + the bytes at 4 TB/s); rows that 16-byte loads cannot take cost a pass
-// that packs them (2.5 us + the bytes at 3 TB/s) or, element by element in the smallest shape, 1.8 us per slice of a wave
-// (77 x 131 x 500: 6.3 us against 8.5 packed).
+// every slice's sums written and read once: 4.5 us + the bytes at 4 TB/s); rows that LDS-DMA cannot take cost a pass
+// that packs them (2.5 us + the bytes at 3 TB/s) or go straight into registers in the smallest shape, 1.8 us per slice of a wave
+// (77 x 131 x 500: 4.5 us against 8.1 packed; 3000 x 500 x 1001: 36 us against 19).
 struct Plan { int shape, splits; bool gather; };
 Plan plan_linear(int64_t M, int npad, int ksteps, bool whole, size_t slab_bytes) {
     Plan best{0, 1, false};
@@ -797,10 +824,10 @@ hipError_t launch_linear(const LinearCall& q, const LinearWork& ws, hipStream_t 
     LinearIn a{};
     a.wt = q.wt; a.bias = q.bias; a.zeros = ws.zeros;
     a.K = q.K; a.npad = linear_npad(q.N); a.panels = a.npad / 16; a.ksteps = linear_kpad(q.K) / 64;
-    // can 16-byte loads take the rows?
+    // can LDS-DMA take the rows?
     const bool whole = q.tiled || (q.K % 8 == 0 && q.ldx % 8 == 0 && (size_t)q.x % 16 == 0);
     const size_t row_bytes = (size_t)linear_kpad(q.K) * 2;
-    Plan plan = plan_linear(q.M, a.npad, a.ksteps, whole, ws.slab_bytes);
+    const Plan plan = plan_linear(q.M, a.npad, a.ksteps, whole, ws.slab_bytes);
     const bool direct = whole || plan.gather;
     // rows that must be packed first go through the workspace in runs of whole tiles
     const int64_t run = direct ? q.M : (int64_t)(ws.pack_bytes / row_bytes) / 256 * 256;
@@ -823,8 +850,6 @@ hipError_t launch_linear(const LinearCall& q, const LinearWork& ws, hipStream_t 
         o.out = (char*)o.out + (size_t)m0 * o.ldo * osz;
         if (o.res) o.res = (const char*)o.res + (size_t)m0 * o.ldr * rsz;
         o.N = q.N;
-        o.vec_out = (size_t)o.out % 16 == 0 && (size_t)o.ldo * osz % 16 == 0;
-        o.vec_res = o.res && (size_t)o.res % 16 == 0 && (size_t)o.ldr * rsz % 16 == 0;
         const int per = (a.ksteps + plan.splits - 1) / plan.splits, splits = (a.ksteps + per - 1) / per;    // (no empty slice)
         a.slab = splits > 1 ? ws.slabs : nullptr;
         hipError_t e = q.bf16 ? launch_shape<true>(plan.shape, a, o, splits, plan.gather, s, false)

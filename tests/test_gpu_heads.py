@@ -171,6 +171,32 @@ def test_nonfinite_values_stay_in_their_rows(ctx):
         assert (err[ok] <= (tol + rounding(y.abs() + tol, "f16"))[ok]).all()
 
 
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu", "gelu_tanh"])
+def test_activations_over_their_range(ctx, act):
+    """act(x) itself (a layer that passes its input on), from the far negative tail to large values, to fp32: relative accuracy
+    down to where the value leaves fp32's normal range, and zero or the smallest numbers beyond."""
+    v = torch.cat([torch.linspace(-16, 16, 8193), torch.tensor([0.0, -0.0, 6e-8, -6e-8, 1e-3, -1e-3, 50, -50, 80, -80, 200, -200, 60000, -60000])]).half()
+    x = torch.zeros(v.numel(), 8, dtype=torch.float16)
+    x[:, 0] = v
+    w = torch.zeros(32, 8, dtype=torch.float16)
+    w[:, 0] = 1
+    lin = linear_of(ctx, w, None, "f16")
+    xd, o = x.cuda(), torch.empty(v.numel(), 32, dtype=torch.float32, device="cuda")
+    torch.cuda.synchronize()
+    lin.run_dev(xd.data_ptr(), v.numel(), o.data_ptr(), act=act, out_dtype="f32")
+    ctx.sync()
+    o = o.cpu().double()
+    assert (o == o[:, :1]).all()
+    y, d = act64(v.double(), act), v.double()
+    y = torch.where(torch.isnan(y), torch.zeros_like(y), y)         # 0 * inf of the 64-bit formula's own overflow (tanh form, far left)
+    # the fit and its evaluation: 5 units of 2^-24, exp 3, the reciprocals 2, products and the final rounding 4; the exponents' own
+    # rounding: gelu carries v^2 exactly, the tanh form's argument has three roundings of |2 u|
+    u2 = 1.6 * (d.abs() + 0.044715 * d.abs() ** 3)
+    tol = (16 + (3 * u2 if act == "gelu_tanh" else 0)) * 2.0 ** -24 * y.abs() + d.abs() * 2.0 ** -125
+    bad = ~((o[:, 0] - y).abs() <= tol)
+    assert not bad.any(), (v[bad][:8], o[bad, 0][:8], y[bad][:8])
+
+
 def test_overflow_rounds_to_infinity(ctx):
     x = torch.full((2, 64), 100.0, dtype=torch.float16)
     w = torch.full((32, 64), 100.0, dtype=torch.float16)
