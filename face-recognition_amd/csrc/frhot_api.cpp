@@ -2549,6 +2549,32 @@ int frhot_head_dev(frhot_head* h, const void* x_f16_dev, int64_t ldx, int64_t M,
     });
 }
 
+int frhot_head_apply(frhot_head* h, const float* x, int M, float* out) {
+    return guarded([&]() -> int {
+    if (!h || !x || !out) return fail(FRHOT_EINVAL, "null argument");
+    if (M <= 0 || M > h->rows) return fail(FRHOT_EINVAL, "%d rows outside 1..%lld", M, (long long)h->rows);
+    frhot_ctx* c = h->ctx;
+    std::lock_guard<std::mutex> lk(c->mu);
+    DeviceGuard dg(c->device);
+    const size_t nx = (size_t)M * h->din, no = (size_t)M * h->dout;
+    std::vector<_Float16> x16(nx), o16(no);
+    for (size_t i = 0; i < nx; ++i) x16[i] = (_Float16)x[i];
+    void* dev = nullptr;
+    HIP_TRY(hipMalloc(&dev, (nx + no) * 2));
+    hipError_t e = hipMemcpyAsync(dev, x16.data(), nx * 2, hipMemcpyHostToDevice, c->stream);
+    int rc = FRHOT_OK;
+    if (e == hipSuccess) rc = head_enqueue(h, dev, h->din, false, M, UnitOut{(char*)dev + nx * 2, h->dout, 0, 0, nullptr, nullptr});
+    if (e == hipSuccess && rc == FRHOT_OK) e = hipMemcpyAsync(o16.data(), (char*)dev + nx * 2, no * 2, hipMemcpyDeviceToHost, c->stream);
+    const hipError_t es = hipStreamSynchronize(c->stream);
+    if (e == hipSuccess) e = es;
+    (void)hipFree(dev);
+    if (rc) return rc;
+    if (e != hipSuccess) return fail(FRHOT_EHIP, "head pass failed: %s", hipGetErrorString(e));
+    for (size_t i = 0; i < no; ++i) out[i] = (float)o16[i];
+    return FRHOT_OK;
+    });
+}
+
 int frhot_ctx_head(frhot_ctx* c, frhot_head* h) {
     return guarded([&]() -> int {
     if (!c) return fail(FRHOT_EINVAL, "ctx is null");

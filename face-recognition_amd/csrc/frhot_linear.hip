@@ -613,9 +613,10 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearIn a, LinearOut 
 // shorter than 1e-30 is divided by one.
 // L lanes a row, each R vectors of V consecutive elements (16 bytes, at any address) in registers: x is read once.  R = 0: rows too
 // long for that are read twice, the second time out of the cache.
-template <typename T, int V>
+// TAIL: V does not divide the row, its last vector is taken element by element.
+template <typename T, int V, bool TAIL>
 FR_DEV void load_row(const T* p, int n, float (&v)[V]) {
-    if (n >= V) {
+    if (!TAIL || n >= V) {
         const auto t = *(const typename vect<T, V>::type*)p;
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] = (float)t[j];
@@ -624,7 +625,7 @@ FR_DEV void load_row(const T* p, int n, float (&v)[V]) {
         for (int j = 0; j < V; ++j) v[j] = j < n ? (float)p[j] : 0.f;
     }
 }
-template <int V>
+template <int V, bool TAIL>
 FR_DEV void store_unit(const UnitOut& o, int N, int m, int c, const float (&v)[V], float nrm) {
     half_t* d;
     if (o.gallery) {
@@ -636,7 +637,7 @@ FR_DEV void store_unit(const UnitOut& o, int N, int m, int c, const float (&v)[V
     half_t t[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) t[j] = (half_t)__fdiv_rn(v[j], nrm);
-    if (c + V <= N) {
+    if (!TAIL || c + V <= N) {
         typename vect<half_t, V>::type u;
 #pragma unroll
         for (int j = 0; j < V; ++j) u[j] = t[j];
@@ -647,7 +648,7 @@ FR_DEV void store_unit(const UnitOut& o, int N, int m, int c, const float (&v)[V
             if (c + j < N) d[j] = t[j];
     }
 }
-template <typename T, int L, int R>
+template <typename T, int L, int R, bool TAIL>
 __global__ __launch_bounds__(256) void unit_rows_kernel(const T* __restrict__ x, int64_t ldx, int M, int N, UnitOut o) {
     constexpr int V = 16 / sizeof(T), RB = 256 / L;             // RB rows a block
     const int m = blockIdx.x * RB + threadIdx.x / L, l = threadIdx.x % L;
@@ -659,7 +660,7 @@ __global__ __launch_bounds__(256) void unit_rows_kernel(const T* __restrict__ x,
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const int c = (i * L + l) * V;
-            if (c < N) load_row<T, V>(row + c, N - c, v[i]);
+            if (c < N) load_row<T, V, TAIL>(row + c, N - c, v[i]);
         }
 #pragma unroll
         for (int i = 0; i < R; ++i)
@@ -669,7 +670,7 @@ __global__ __launch_bounds__(256) void unit_rows_kernel(const T* __restrict__ x,
             }
     } else {
         for (int c = l * V; c < N; c += L * V) {
-            load_row<T, V>(row + c, N - c, v[0]);
+            load_row<T, V, TAIL>(row + c, N - c, v[0]);
 #pragma unroll
             for (int j = 0; j < V; ++j) ss += (double)v[0][j] * (double)v[0][j];
         }
@@ -682,12 +683,12 @@ __global__ __launch_bounds__(256) void unit_rows_kernel(const T* __restrict__ x,
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const int c = (i * L + l) * V;
-            if (c < N) store_unit<V>(o, N, m, c, v[i], nrm);
+            if (c < N) store_unit<V, TAIL>(o, N, m, c, v[i], nrm);
         }
     } else {
         for (int c = l * V; c < N; c += L * V) {
-            load_row<T, V>(row + c, N - c, v[0]);
-            store_unit<V>(o, N, m, c, v[0], nrm);
+            load_row<T, V, TAIL>(row + c, N - c, v[0]);
+            store_unit<V, TAIL>(o, N, m, c, v[0], nrm);
         }
     }
     if (l == 0 && o.keys_dst) o.keys_dst[o.row0 + m] = o.keys_src[o.row0 + m];
@@ -696,7 +697,8 @@ __global__ __launch_bounds__(256) void unit_rows_kernel(const T* __restrict__ x,
 template <typename T, int L, int R>
 hipError_t launch_unit(const void* x, int64_t ldx, int64_t M, int N, const UnitOut& o, hipStream_t s) {
     const int64_t rb = 256 / L;
-    hipLaunchKernelGGL((unit_rows_kernel<T, L, R>), dim3((unsigned)((M + rb - 1) / rb)), dim3(256), 0, s, (const T*)x, ldx, (int)M, N, o);
+    const auto kern = N % (16 / (int)sizeof(T)) ? unit_rows_kernel<T, L, R, true> : unit_rows_kernel<T, L, R, false>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)((M + rb - 1) / rb)), dim3(256), 0, s, (const T*)x, ldx, (int)M, N, o);
     return hipGetLastError();
 }
 template <typename T>

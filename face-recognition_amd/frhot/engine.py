@@ -348,6 +348,15 @@ class Head:
         check(self._lib.frhot_head_dev(self._h, x_f16_dev, self.din if ldx is None else ldx, m, out_f16_dev,
                                        self.dout if ldo is None else ldo))
 
+    def apply(self, x: np.ndarray) -> np.ndarray:
+        """Descriptors [n, din] (host floats) -> unit rows [n, dout] float32, for a few at a time."""
+        x = np.ascontiguousarray(x, dtype=np.float32).reshape(-1, self.din)
+        out = np.empty((len(x), self.dout), dtype=np.float32)
+        for lo in range(0, len(x), 2048):
+            part, sub = x[lo:lo + 2048], out[lo:lo + 2048]
+            check(self._lib.frhot_head_apply(self._h, _ptr(part, C.c_float), len(part), _ptr(sub, C.c_float)))
+        return out
+
 
 def _list(a, dtype):
     if type(a) is np.ndarray and a.dtype == dtype and a.ndim == 1 and a.flags.c_contiguous:

@@ -10,7 +10,9 @@ device-resident gallery (frhot.engine.Gallery) instead of Qdrant collections:
     (app.py:207-240), delete-by-payload-id (app.py:409-438) and the threshold + vote
     (app.py:340-384) stay on the host;
   * per-collection snapshots (app.py:130-196) are one .npz file each: the stored fp16
-    rows read back from the device plus the point table, restored bit for bit.
+    rows read back from the device plus the point table, restored bit for bit;
+  * a collection is copied, dropped and the gallery squeezed on the device (frhot_gallery_copy /
+    _free_keys / _compact): no row leaves HBM.
 
 Methods return (status_code, content) exactly as the handlers answer.
 """
@@ -70,11 +72,32 @@ class _RowAllocator:
     def release(self, row: int):
         self._free.setdefault(self._owner[row // TILE], []).append(row)
 
+    def reset(self, keys):
+        """Rows 0 .. len(keys)-1 are taken by these keys and nothing else is: the state behind a squeeze.
+        A tile belongs to the key with the most rows in it; the rows behind the last one to the last tile's."""
+        self._owner, self._free = {}, {}
+        self._next_tile = (len(keys) + TILE - 1) // TILE
+        for t in range(self._next_tile):
+            inside = list(keys[t * TILE:(t + 1) * TILE])
+            self._owner[t] = max(dict.fromkeys(inside), key=inside.count)
+        if self._next_tile:
+            t = self._next_tile - 1
+            hi = min((t + 1) * TILE, self.capacity)
+            self._free[self._owner[t]] = list(range(hi - 1, len(keys) - 1, -1))
+
 
 class GalleryService:
-    def __init__(self, ctx, capacity: int = 1 << 16, dim: int = DIM, gallery=None):
+    def __init__(self, ctx, capacity: int = 1 << 16, dim: int = DIM, gallery=None, head=None):
         """`gallery`: an object with the upsert / tombstone / search / close methods of
-        frhot.engine.Gallery to use instead of creating one on `ctx` (tests inject a stand-in)."""
+        frhot.engine.Gallery to use instead of creating one on `ctx` (tests inject a stand-in).
+        `head`: a frhot.engine.Head: the gallery holds its rows (dim = head.dout), vectors of
+        head.din components are taken through it on their way in and on their way to a search, and
+        it is attached to `ctx`, so that recognise_points does the same."""
+        self.head = head
+        if head is not None:
+            dim = head.dout
+            if ctx is not None:
+                ctx.set_head(head)
         self.dim = dim
         self.capacity = capacity
         if gallery is None:
@@ -89,6 +112,7 @@ class GalleryService:
         self._by_id: dict[tuple, list] = {}        # (collection, payload id) -> rows in insertion order
         self._rows = _RowAllocator(capacity)
         self._seq = 0
+        self._moves = 0                            # how often rows changed their numbers (compact)
 
     def close(self):
         self.gallery.close()
@@ -134,7 +158,104 @@ class GalleryService:
         with self._lock:
             return sum(1 for p in self._points.values() if p["collection"] == collection_name)
 
+    def delete_collection(self, collection_name):
+        """test/delete_collection.py: the collection and its points go, in one device call."""
+        if collection_name is None or collection_name == "":
+            return 404, {"message": "Collection name not found or invalid!"}
+        with self._lock:
+            if collection_name not in self._collections:
+                return 404, {"message": "Collection name not found or invalid!"}
+            try:
+                keys = [k for (col, _sid), k in self._keys.items() if col == collection_name]
+                if keys:
+                    self.gallery.free_keys(np.asarray(keys, dtype=np.int32))
+                rows = [r for r, p in self._points.items() if p["collection"] == collection_name]
+                for r in rows:
+                    self._forget(r)
+                del self._collections[collection_name]
+                return 200, {"message": "Collection deleted"}
+            except Exception as e:
+                return 404, {"message": str(e)}
+
+    def copy_collection(self, source_name, collection_name):
+        """The points of one collection under another one's name as well (new point ids, same
+        payloads), copied on the device: what create_snapshot + recover_snapshot (app.py:130-196) do
+        through a file.  The target is created; one that already holds points is refused."""
+        if not source_name or not collection_name:
+            return 404, {"message": "Collection name not found or invalid!"}
+        with self._lock:
+            if source_name not in self._collections or source_name == collection_name:
+                return 404, {"message": "Collection name not found or invalid!"}
+            if any(p["collection"] == collection_name for p in self._points.values()):
+                return 409, {"message": "Collection already holds points"}
+            src = sorted(r for r, p in self._points.items() if p["collection"] == source_name)
+            if len(src) > self._rows.free_count():
+                return 404, {"message": f"collection holds {len(src)} points, the gallery has room for "
+                                        f"{self._rows.free_count()}"}
+            dst, keys = [], []
+            try:
+                for r in src:
+                    keys.append(self._key(collection_name, self._points[r]["payload"].get("store_id")))
+                    dst.append(self._alloc_row(keys[-1]))
+                if src:
+                    s, d, k = (np.asarray(a, dtype=np.int64) for a in (src, dst, keys))
+                    edge = np.flatnonzero(np.concatenate([[True], (np.diff(s) != 1) | (np.diff(d) != 1) | (np.diff(k) != 0)]))
+                    counts = np.diff(np.concatenate([edge, [len(s)]])).astype(np.int32)
+                    self.gallery.copy(s[edge], d[edge], counts, k[edge].astype(np.int32))
+            except Exception as e:
+                for r in dst:
+                    self._rows.release(r)
+                return 404, {"message": str(e)}
+            self._collections.setdefault(collection_name, None)
+            # in the order the points were inserted, so that the eviction of the oldest goes on as in the source
+            for r, new in sorted(zip(src, dst), key=lambda rn: self._points[rn[0]]["seq"]):
+                self._seq += 1
+                p = self._points[r]
+                self._points[new] = {"uid": str(uuid.uuid4()), "payload": dict(p["payload"]), "collection": collection_name,
+                                     "seq": self._seq}
+                self._by_id.setdefault((collection_name, p["payload"]["id"]), []).append(new)
+            return 201, {"message": "Collection copied", "points": len(src)}
+
+    def compact(self):
+        """Squeeze the gallery: live rows, in order, to its front, so that a scan reads no dead ones.
+        Searches that are on the device meanwhile are repeated against the new row numbers."""
+        with self._lock:
+            try:
+                live = sorted(self._points)
+                stray = np.setdiff1d(np.arange(self.gallery.rows), np.asarray(live, dtype=np.int64))
+                if stray.size:          # rows of the table's gaps that a failed write may have left alive
+                    self.gallery.tombstone(stray)
+                n = self.gallery.compact()
+                if n != len(live):
+                    raise RuntimeError(f"{n} live rows on the device, {len(live)} points in the table")
+            except Exception as e:
+                return 404, {"message": str(e)}
+            place = {r: i for i, r in enumerate(live)}
+            self._points = {place[r]: self._points[r] for r in live}
+            self._by_id = {k: [place[r] for r in rows] for k, rows in self._by_id.items()}
+            self._rows.reset([self._keys[(p["collection"], p["payload"].get("store_id"))] for p in self._points.values()])
+            self._moves += 1
+            return 200, {"message": "Gallery compacted", "points": len(live)}
+
     # ----------------------------------------------------------------- points
+    def _forget(self, row):
+        """Drop a row from the tables and hand it back (its device row is dead already)."""
+        p = self._points.pop(row)
+        lst = self._by_id[(p["collection"], p["payload"]["id"])]
+        lst.remove(row)
+        if not lst:
+            del self._by_id[(p["collection"], p["payload"]["id"])]
+        self._rows.release(row)
+
+    def _fits(self, vec):
+        return vec is not None and (len(vec) == self.dim or (self.head is not None and len(vec) == self.head.din))
+
+    def _as_row(self, vec):
+        vec = np.asarray(vec, dtype=np.float32).reshape(-1)
+        if self.head is not None and vec.size == self.head.din:
+            vec = self.head.apply(vec)[0]
+        return vec
+
     def _key(self, collection, store_id) -> int:
         k = (collection, store_id)
         if k not in self._keys:
@@ -149,12 +270,7 @@ class GalleryService:
             return
         self.gallery.tombstone(np.asarray(rows, dtype=np.int64))
         for r in rows:
-            p = self._points.pop(r)
-            lst = self._by_id[(p["collection"], p["payload"]["id"])]
-            lst.remove(r)
-            if not lst:
-                del self._by_id[(p["collection"], p["payload"]["id"])]
-            self._rows.release(r)
+            self._forget(r)
 
     def _enforce_face_limit(self, collection, pid, limit=10):
         """app.py:207-240: among the first limit+5 points of this id, delete the oldest so limit-1 stay."""
@@ -174,7 +290,7 @@ class GalleryService:
         with self._lock:
             if collection_name not in self._collections:
                 return 404, {"message": "Collection name not found or invalid!"}
-            if vector_embedding is None or len(vector_embedding) != self.dim:
+            if not self._fits(vector_embedding):
                 return 404, {"message": "Embedding not found or invalid!"}
             if id is None or id == "":
                 return 404, {"message": "ID not found or invalid!"}
@@ -187,7 +303,7 @@ class GalleryService:
                 print(f"Error checking face limit: {e}")
             payload = {'id': id, 'name': name, 'store_id': store_id, 'time_created': time_created}
             try:
-                vec = np.asarray(vector_embedding, dtype=np.float32).reshape(1, self.dim)
+                vec = self._as_row(vector_embedding).reshape(1, self.dim)
                 if is_update_id:
                     rows = self._by_id.get((collection_name, id))
                     if not rows:
@@ -232,7 +348,7 @@ class GalleryService:
             return 404, {"message": "Collection name not found or invalid!"}
         if collection_name not in self._collections:
             return 404, {"message": "Collection name not found or invalid!"}
-        if vector_embedding is None or len(vector_embedding) != self.dim:
+        if not self._fits(vector_embedding):
             return 404, {"message": "Embedding not found or invalid!"}
         return None
 
@@ -292,12 +408,14 @@ class GalleryService:
                     out[i] = (200, {"message": "Point not found", "data": []})
                     continue
                 idx.append(i)
-                vecs.append(np.asarray(vec, dtype=np.float32))
+                vecs.append(self._as_row(vec))
                 keys.append(k)
             if idx or self._always_search:
                 try:
-                    seq0 = self._seq
+                    seq0, moves = self._seq, self._moves
                     with self._device_call():
+                        scores, rows = self._search_batch(vecs, keys)
+                    if self._moves != moves:        # the rows' numbers changed meanwhile: once more, with the lock held
                         scores, rows = self._search_batch(vecs, keys)
                     for j, i in enumerate(idx):
                         out[i] = (200, vote(self._hits(scores[j], rows[j], seq0)))
@@ -333,11 +451,18 @@ class GalleryService:
                     bad[i] = (404, {"message": "Collection name not found or invalid!"})
                 k = self._keys.get((col, store_id))
                 keys.append(self.NO_KEY if (k is None or i in bad) else k)
-            seq0 = self._seq
-            with self._device_call():
-                scores, rows, emb, *sharp = self.gallery.ctx.recognise(
+            seq0, moves = self._seq, self._moves
+
+            def run():
+                return self.gallery.ctx.recognise(
                     self.gallery, [r[1] for r in requests], np.asarray(keys, np.int32), SEARCH_LIMIT, gamma=gamma,
                     want_embeddings=want_embeddings, want_sharpness=want_sharpness)
+
+            with self._device_call():
+                answer = run()
+            if self._moves != moves:                # the rows' numbers changed meanwhile: once more, with the lock held
+                answer = run()
+            scores, rows, emb, *sharp = answer
             for i in range(len(requests)):
                 e = emb[i].copy() if emb is not None else None
                 if i in bad:

@@ -161,6 +161,9 @@ class _ShardedGallery:
         if mine.any():
             self.b.gallery.tombstone(rows[mine] % self.cap)
 
+    def free_keys(self, keys):
+        return self.b.gallery.free_keys(keys)       # this rank's shard; every rank makes the call
+
     def read(self, rows):
         """COLLECTIVE: the stored fp16 rows and keys of global rows, from whichever shard holds them."""
         rows, mine = self._mine(rows)
@@ -216,7 +219,8 @@ class ShardedGalleryService(GalleryService):
     # ------------------------------------------------------------- mutations
     def mutate(self, ops):
         """COLLECTIVE.  ops: this rank's pending mutations, each ("create_collection", name),
-        ("insert_point", {keyword arguments of insert_point}) or ("delete_point", collection, id).
+        ("insert_point", {keyword arguments of insert_point}), ("delete_point", collection, id) or
+        ("delete_collection", name).
         Every rank applies all ranks' mutations, rank by rank; returns the answers to this rank's."""
         mine = []
         for op in ops:
@@ -241,6 +245,8 @@ class ShardedGalleryService(GalleryService):
                     res = GalleryService.insert_point(self, **op[1])
                 elif op[0] == "delete_point":
                     res = GalleryService.delete_point(self, op[1], op[2])
+                elif op[0] == "delete_collection":
+                    res = GalleryService.delete_collection(self, op[1])
                 else:
                     res = (404, {"message": f"unknown mutation {op[0]!r}"})
                 if r == self.rank:
@@ -253,6 +259,12 @@ class ShardedGalleryService(GalleryService):
         if self.world > 1 and kwargs.get("uid") is None and not kwargs.get("is_update_id"):
             raise RuntimeError("insert_point on a sharded service: use mutate(), which agrees on the point's id")
         return GalleryService.insert_point(self, *args, **kwargs)
+
+    def copy_collection(self, source_name, collection_name):
+        raise NotImplementedError("rows do not move between shards: copy a collection through a snapshot")
+
+    def compact(self):
+        raise NotImplementedError("a sharded gallery is not squeezed")
 
     # ---------------------------------------------------------------- search
     def _search_batch(self, vecs, keys):

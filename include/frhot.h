@@ -412,6 +412,8 @@ int frhot_ctx_stage_ms(frhot_ctx* ctx, float* ms5);
  *   multiples of 64.  Inner layers round to fp16, the last one's output stays fp32 up to the norm.
  *   The layers stay the caller's and must outlive the head.
  * frhot_head_dev: fp16 rows x [M,din] -> unit fp16 rows out [M,dout].
+ * frhot_head_apply: the same for host rows (x [M,din] float32, rounded to fp16; out [M,dout] float32
+ *   holding the fp16 rows), for a few descriptors at a time (M up to 2048 at least); waits.
  * frhot_ctx_head: attach (or, NULL, detach) a head of 4096 inputs: frhot_embed_dev with Dq equal to
  *   its outputs and frhot_recognise* on a gallery of that dimension then use the head's rows as
  *   queries, where they take the descriptor's leading components otherwise.  Destroying an attached
@@ -428,6 +430,7 @@ int frhot_head_create(frhot_ctx* ctx, frhot_linear* const* layers, const int32_t
                       frhot_head** out);
 int frhot_head_destroy(frhot_head* head);
 int frhot_head_dev(frhot_head* head, const void* x_f16_dev, int64_t ldx, int64_t M, void* out_f16_dev, int64_t ldo);
+int frhot_head_apply(frhot_head* head, const float* x, int M, float* out);
 int frhot_ctx_head(frhot_ctx* ctx, frhot_head* head);
 
 /*

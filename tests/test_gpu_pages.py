@@ -481,3 +481,96 @@ def test_reproject_refusals(ctx):
     lin.close()
     for g in (a, b, small, empty):
         g.close()
+
+
+# ------------------------------------------------------------------------- as a service uses them
+def test_service_with_a_head_copies_drops_and_squeezes(gpu_ctx):
+    """Faces enrolled through a head into a 256-wide gallery, recognised from their crops, the collection forked, the
+    original dropped, the gallery squeezed: every step answers for the same people."""
+    from frhot import synth
+    from frhot.engine import Head
+    from frhot.gallery_service import GalleryService
+    from test_gpu_heads import head_layers, linear_of
+    crops = synth.crops(seed=9, n=8, lo=90, hi=180)
+    emb = gpu_ctx.embed(crops, gamma=True)
+    # a layer that spreads the synthetic network's similar faces: random directions around their mean
+    g = torch.Generator().manual_seed(3)
+    w = (torch.randn(256, 4096, generator=g) / 8).half()
+    mean = torch.from_numpy(emb).double().mean(0)
+    lin = linear_of(gpu_ctx, w, (-(w.double() @ mean)).float(), "f16")
+    head = Head(gpu_ctx, [(lin, "none", False)])
+    rows = head.apply(emb)
+    x16 = torch.from_numpy(emb).half()
+    y = x16.double() @ w.double().t() - (w.double() @ mean).float().double()
+    y = y / y.norm(dim=1, keepdim=True)
+    assert (torch.from_numpy(rows).double() - y).abs().max() <= 2e-3
+    svc = GalleryService(gpu_ctx, capacity=2000, head=head)
+    try:
+        assert svc.dim == 256
+        svc.create_collection("7_Employees")
+        rng = np.random.default_rng(1)
+        for i in range(300):                                    # strangers around them, some of whom leave again
+            svc.insert_point("7_Employees", rng.standard_normal(256).astype(np.float32), f"s{i}", "x", 7)
+        for i, e in enumerate(emb):
+            assert svc.insert_point("7_Employees", e, f"p{i}", f"n{i}", 7)[0] == 201
+        for i in range(0, 300, 2):
+            svc.delete_point("7_Employees", f"s{i}")
+
+        def who(col):
+            return [content["data"][0][1]["id"] if content["data"] else None
+                    for _s, content, _e in svc.recognise_points([(col, c, 7) for c in crops])]
+        want = [f"p{i}" for i in range(8)]
+        assert who("7_Employees") == want
+        assert svc.copy_collection("7_Employees", "8_Employees")[1]["points"] == 158
+        assert who("8_Employees") == want
+        assert svc.delete_collection("7_Employees")[0] == 200
+        assert svc.recognise_points([("7_Employees", crops[0], 7)])[0][0] == 404
+        assert who("8_Employees") == want
+        assert svc.compact() == (200, {"message": "Gallery compacted", "points": 158})
+        assert svc.gallery.rows == 158 and who("8_Employees") == want
+        for i in range(8):
+            assert svc.search_point("8_Employees", emb[i], 7)[1]["data"][0][1]["id"] == f"p{i}"
+        assert svc.insert_point("8_Employees", emb[0] * 2, "again", "n", 7)[0] == 201
+        assert svc.gallery.rows == 159
+    finally:
+        gpu_ctx.set_head(None)
+        svc.close()
+        head.close()
+        lin.close()
+
+
+def test_squeezing_while_others_recognise(gpu_ctx):
+    """Threads that search while collections are dropped and the gallery squeezed: every answer names the asked person."""
+    import threading
+    from frhot.gallery_service import GalleryService
+    svc = GalleryService(gpu_ctx, capacity=6000, dim=512)
+    rng = np.random.default_rng(2)
+    vecs = rng.standard_normal((60, 512)).astype(np.float32)
+    svc.create_collection("1_Employees")
+    for k in range(4):
+        svc.create_collection(f"{k + 2}_Customers")
+        for i in range(150):
+            svc.insert_point(f"{k + 2}_Customers", rng.standard_normal(512).astype(np.float32), f"c{i}", "n", 1)
+        for i in range(15 * k, 15 * k + 15):
+            svc.insert_point("1_Employees", vecs[i], f"p{i}", "n", 1)
+    errors, stop = [], threading.Event()
+
+    def ask(j):
+        r = np.random.default_rng(j)
+        try:
+            while not stop.is_set():
+                i = int(r.integers(60))
+                status, content = svc.search_point("1_Employees", vecs[i], 1)
+                assert status == 200 and content["data"][0][1]["id"] == f"p{i}", content
+        except Exception as e:
+            errors.append(e)
+    ts = [threading.Thread(target=ask, args=(j,)) for j in range(3)]
+    [t.start() for t in ts]
+    for k in range(4):
+        assert svc.delete_collection(f"{k + 2}_Customers")[0] == 200
+        assert svc.compact()[0] == 200
+    stop.set()
+    [t.join() for t in ts]
+    assert not errors, errors[0]
+    assert svc.gallery.rows == 60
+    svc.close()
