@@ -807,13 +807,13 @@ int key_tiles_rebuild(frhot_gallery* g) {
     return FRHOT_OK;
 }
 
-int index_pin_grow(IndexPin& ip, size_t n) {
+int index_pin_grow(IndexPin& ip, size_t n, unsigned flags = hipHostMallocDefault) {
     if (!ip.copied) HIP_TRY(hipEventCreateWithFlags(&ip.copied, hipEventDisableTiming));
     if (ip.pending) { ip.pending = false; HIP_TRY(hipEventSynchronize(ip.copied)); }   // an enqueue-only call's upload
     if (n <= ip.cap) return FRHOT_OK;
     if (ip.p) { int32_t* old = ip.p; ip.p = nullptr; ip.cap = 0; HIP_TRY(hipHostFree(old)); }
     const size_t cap = n + n / 2 + 1024;
-    HIP_TRY(hipHostMalloc((void**)&ip.p, cap * 4, hipHostMallocDefault));
+    HIP_TRY(hipHostMalloc((void**)&ip.p, cap * 4, flags));
     ip.cap = cap;
     return FRHOT_OK;
 }
@@ -2635,7 +2635,7 @@ int page_refuse_capture(frhot_ctx* c) {
 // Page-locked memory for a page call of the stream; mark behind the launch that reads it.
 int page_pin_take(frhot_ctx* c, size_t words, IndexPin** out) {
     IndexPin& ip = c->page_pin[c->page_next++ & 3];
-    const int rc = index_pin_grow(ip, words);
+    const int rc = index_pin_grow(ip, words, hipHostMallocCoherent);    // (the host polls what kernels store there)
     *out = &ip;
     return rc;
 }
@@ -2909,43 +2909,44 @@ int frhot_gallery_compact(frhot_gallery* src, frhot_gallery* dst, int64_t* new_r
             HIP_TRY(hipStreamSynchronize(s));       // (nothing stores into the word any more)
             ip->p[0] = kUntold;
         }
+        // In place: by way of a second copy of the rows that is given back at the end.  The gallery's own memory stays where it
+        // is: a captured search replayed later may be out of date, but not astray.
         void* rows = g->rows;
         int32_t* keys = g->keys;
-        int64_t old_rows = g->nrows;
+        const size_t copied_rows = ntiles * 256;
         if (!dst) {
-            // in place: into fresh buffers, which take the old ones' place once everything has landed
-            const size_t padded = ((size_t)src->capacity + 255) & ~(size_t)255;
-            rows = nullptr; keys = nullptr; old_rows = 0;
-            hipError_t e = hipMalloc(&rows, padded * src->D * 2);
-            if (e == hipSuccess) e = hipMalloc((void**)&keys, padded * 4);
-            if (e == hipSuccess) e = hipMemsetAsync(rows, 0, padded * src->D * 2, s);
-            if (e == hipSuccess) e = hipMemsetAsync(keys, 0xFF, padded * 4, s);
+            rows = nullptr; keys = nullptr;
+            hipError_t e = hipMalloc(&rows, copied_rows * src->D * 2);
+            if (e == hipSuccess) e = hipMalloc((void**)&keys, copied_rows * 4);
             if (e != hipSuccess) {
                 if (rows) (void)hipFree(rows);
-                if (keys) (void)hipFree(keys);
                 return fail(FRHOT_ECAPACITY, "no room for a second copy of the gallery: %s", hipGetErrorString(e));
             }
         }
-        hipError_t e = launch_page_compact(src->rows, src->keys, src->nrows, rows, keys, old_rows, src->D, c->page_off, new_rows_dev, ip->p, s);
-        // into another gallery only the count is waited for (the first thing the kernels know); in place, the old rows are
-        // given back, so everything is
-        if (e == hipSuccess && !dst) e = hipStreamSynchronize(s);
-        if (e != hipSuccess) {
-            if (!dst) { (void)hipStreamSynchronize(s); (void)hipFree(rows); (void)hipFree(keys); }
-            return fail(FRHOT_EHIP, "compacting failed: %s", hipGetErrorString(e));
+        hipError_t e = launch_page_compact(src->rows, src->keys, src->nrows, rows, keys, dst ? dst->nrows : 0, src->D, c->page_off, new_rows_dev, ip->p, s);
+        // (the count is the first thing the kernels know; into another gallery nothing else is waited for)
+        if (e == hipSuccess) rc = page_await(c, ip->p, 1);
+        if (e == hipSuccess && !rc) {
+            live = ip->p[0];
+            if (!dst && live > 0) {
+                // whole tiles, then the live rows of the last one (128 bytes a row in each of its chunks of 32 KiB)
+                const size_t whole = (size_t)(live / 256) * 256 * src->D * 2, rest = (size_t)(live % 256) * 128;
+                if (whole) e = hipMemcpyAsync(src->rows, rows, whole, hipMemcpyDeviceToDevice, s);
+                if (e == hipSuccess && rest)
+                    e = hipMemcpy2DAsync((char*)src->rows + whole, 32768, (char*)rows + whole, 32768, rest, (size_t)src->D / 64,
+                                         hipMemcpyDeviceToDevice, s);
+                if (e == hipSuccess) e = hipMemcpyAsync(src->keys, keys, (size_t)live * 4, hipMemcpyDeviceToDevice, s);
+            }
+            if (!dst && e == hipSuccess) e = launch_page_kill(src->keys, live, src->nrows, s);
         }
-        rc = page_await(c, ip->p, 1);
-        if (rc) {
-            if (!dst) { (void)hipFree(rows); (void)hipFree(keys); }
-            return rc;
-        }
-        live = ip->p[0];
         if (!dst) {
-            (void)hipFree(src->rows);
-            (void)hipFree(src->keys);
-            src->rows = rows;
-            src->keys = keys;
+            const hipError_t es = hipStreamSynchronize(s);
+            if (e == hipSuccess) e = es;
+            (void)hipFree(rows);
+            (void)hipFree(keys);
         }
+        if (rc) return rc;
+        if (e != hipSuccess) return fail(FRHOT_EHIP, "compacting failed: %s", hipGetErrorString(e));
     }
     g->nrows = live;
     g->dense = true;

@@ -64,6 +64,7 @@ class Context:
         self._head = None
 
     def close(self):
+        self._head = None                       # (a head that only the context held goes before it)
         if getattr(self, "_h", None) and self._h.value:
             self._lib.frhot_ctx_destroy(self._h)
             self._h = C.c_void_p()
