@@ -694,12 +694,22 @@ __global__ __launch_bounds__(256) void unit_rows_kernel(const T* __restrict__ x,
     if (l == 0 && o.keys_dst) o.keys_dst[o.row0 + m] = o.keys_src[o.row0 + m];
 }
 
+constexpr int64_t kRunRows = 1 << 22;       // rows of one launch
+
 template <typename T, int L, int R>
 hipError_t launch_unit(const void* x, int64_t ldx, int64_t M, int N, const UnitOut& o, hipStream_t s) {
     const int64_t rb = 256 / L;
     const auto kern = N % (16 / (int)sizeof(T)) ? unit_rows_kernel<T, L, R, true> : unit_rows_kernel<T, L, R, false>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)((M + rb - 1) / rb)), dim3(256), 0, s, (const T*)x, ldx, (int)M, N, o);
-    return hipGetLastError();
+    for (int64_t m0 = 0; m0 < M; m0 += kRunRows) {
+        const int64_t n = M - m0 < kRunRows ? M - m0 : kRunRows;
+        UnitOut u = o;
+        if (o.gallery) u.row0 = o.row0 + m0;
+        else u.out = (half_t*)o.out + (size_t)m0 * o.ldo;
+        hipLaunchKernelGGL(kern, dim3((unsigned)((n + rb - 1) / rb)), dim3(256), 0, s, (const T*)x + (size_t)m0 * ldx, ldx, (int)n, N, u);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 template <typename T>
 hipError_t unit_by_width(const void* x, int64_t ldx, int64_t M, int N, const UnitOut& o, hipStream_t s) {
@@ -829,16 +839,18 @@ hipError_t launch_linear(const LinearCall& q, const LinearWork& ws, hipStream_t 
     // can LDS-DMA take the rows?
     const bool whole = q.tiled || (q.K % 8 == 0 && q.ldx % 8 == 0 && (size_t)q.x % 16 == 0);
     const size_t row_bytes = (size_t)linear_kpad(q.K) * 2;
-    const Plan plan = plan_linear(q.M, a.npad, a.ksteps, whole, ws.slab_bytes);
+    const Plan plan = plan_linear(q.M < kRunRows ? q.M : kRunRows, a.npad, a.ksteps, whole, ws.slab_bytes);
     const bool direct = whole || plan.gather;
-    // rows that must be packed first go through the workspace in runs of whole tiles
-    const int64_t run = direct ? q.M : (int64_t)(ws.pack_bytes / row_bytes) / 256 * 256;
+    // rows that must be packed first go through the workspace in runs of whole tiles; others in runs of which no shape makes
+    // 2^32 threads, the most that a launch may have
+    const int64_t run = direct ? kRunRows : (int64_t)(ws.pack_bytes / row_bytes) / 256 * 256;
     if (run <= 0) return hipErrorInvalidValue;
     for (int64_t m0 = 0; m0 < q.M; m0 += run) {
         const int rows = (int)(q.M - m0 < run ? q.M - m0 : run);
         a.M = rows;
         if (direct) {
-            a.x = q.x; a.ldx = q.ldx; a.tiled = q.tiled; a.xtile = (size_t)(q.K / 64) * 32768; a.xstep = q.tiled ? 32768 : 128;
+            a.ldx = q.ldx; a.tiled = q.tiled; a.xtile = (size_t)(q.K / 64) * 32768; a.xstep = q.tiled ? 32768 : 128;
+            a.x = (const char*)q.x + (q.tiled ? (size_t)(m0 / 256) * a.xtile : (size_t)m0 * q.ldx * 2);
         } else {
             const size_t n = (size_t)rows * (row_bytes / 16);
             hipLaunchKernelGGL(linear_pack_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s,

@@ -268,10 +268,11 @@ hipError_t launch_page_move(const PageSide& src, const PageSide& dst, const Page
     const int nk = D / 64;
     int per = 1;
     while (per < nk && rows / n * per < 400 && (int64_t)n * ((nk + per - 1) / per) > 1024) per *= 2;
-    const dim3 grid((unsigned)n, (unsigned)((nk + per - 1) / per));
+    const unsigned parts = (unsigned)((nk + per - 1) / per);
     if (n <= kPageInline) {
         InlineItems list;
         for (int i = 0; i < kPageInline; ++i) list.it[i] = items[i < n ? i : 0];
+        const dim3 grid((unsigned)n, parts);
         if (src.dense) hipLaunchKernelGGL((page_move_inline_kernel<true, false>), grid, dim3(256), 0, s, src, dst, list, nk, per);
         else if (dst.dense) hipLaunchKernelGGL((page_move_inline_kernel<false, true>), grid, dim3(256), 0, s, src, dst, list, nk, per);
         else hipLaunchKernelGGL((page_move_inline_kernel<false, false>), grid, dim3(256), 0, s, src, dst, list, nk, per);
@@ -281,8 +282,14 @@ hipError_t launch_page_move(const PageSide& src, const PageSide& dst, const Page
     const auto kern = src.dense   ? (nt ? page_move_kernel<true, false, true> : page_move_kernel<true, false, false>)
                       : dst.dense ? (nt ? page_move_kernel<false, true, true> : page_move_kernel<false, true, false>)
                                   : (nt ? page_move_kernel<false, false, true> : page_move_kernel<false, false, false>);
-    hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, src, dst, items, nk, per);
-    return hipGetLastError();
+    constexpr int kLaunch = 1 << 22;            // (a launch may have fewer than 2^32 threads)
+    for (int at = 0; at < n; at += kLaunch) {
+        hipLaunchKernelGGL(kern, dim3((unsigned)(n - at < kLaunch ? n - at : kLaunch), parts), dim3(256), 0, s, src, dst, items + at, nk, per);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        if (n - at <= kLaunch) break;
+    }
+    return hipSuccess;
 }
 
 hipError_t launch_page_free(int32_t* gk, const TileRun* runs, int nruns, const int32_t* keys, int nkeys, int32_t* counts, hipStream_t s) {

@@ -539,3 +539,32 @@ def test_recognise_through_a_head(gpu_ctx):
     assert np.array_equal(before[1], again[1])
     gal.close()
     [l.close() for l in lins]
+
+
+def test_more_rows_than_a_launch_has_threads(ctx):
+    """Calls whose rows times lanes pass 2^32 are several launches.  Small whole numbers: the products are exact."""
+    gen = torch.Generator("cuda").manual_seed(8)
+    m = (1 << 26) + 17
+    x = torch.randint(-2, 3, (m, 8), generator=gen, device="cuda", dtype=torch.int8).to(torch.float16)
+    w = torch.randint(-2, 3, (2, 8), generator=gen, device="cuda").float()
+    lin = linear_of(ctx, w.cpu(), torch.tensor([1.0, -3.0]), "f16")
+    o = torch.empty(m, 2, dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    lin.run_dev(x.data_ptr(), m, o.data_ptr())
+    ctx.sync()
+    for lo in range(0, m, 1 << 24):
+        part = x[lo:lo + (1 << 24)].float()
+        want = torch.stack([(part * w[i]).sum(1) for i in range(2)], 1) + torch.tensor([1.0, -3.0], device="cuda")
+        assert torch.equal(o[lo:lo + (1 << 24)].float(), want), lo
+    lin.close()
+    del o, w
+    m = (1 << 30) + 3
+    x = torch.randint(-2, 3, (m,), generator=gen, device="cuda", dtype=torch.int8).to(torch.float16)
+    o = torch.full((m,), 7.0, dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    ctx.unit_rows_dev(x.data_ptr(), m, 1, o.data_ptr(), dtype="f16")
+    ctx.sync()
+    for lo in range(0, m, 1 << 28):
+        assert torch.equal(o[lo:lo + (1 << 28)], torch.sign(x[lo:lo + (1 << 28)])), lo
+    del x, o
+    torch.cuda.empty_cache()

@@ -574,3 +574,25 @@ def test_squeezing_while_others_recognise(gpu_ctx):
     assert not errors, errors[0]
     assert svc.gallery.rows == 60
     svc.close()
+
+
+def test_more_runs_than_a_launch_has_threads():
+    """2^24 + 5 runs of one row: several launches."""
+    from frhot.engine import Context, Gallery
+    ctx = Context(device=0, max_batch=1)                    # (its page-locked run list of 600 MB goes with it)
+    n = (1 << 24) + 5
+    gal = Gallery(ctx, 64, 2 * n)
+    gen = torch.Generator("cuda").manual_seed(3)
+    src = torch.randint(-30000, 30000, (2 * n, 64), generator=gen, device="cuda", dtype=torch.int16)
+    out = torch.empty(n, 64, dtype=torch.int16, device="cuda")
+    keys = torch.empty(n, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    gal.write_dev(src.data_ptr(), [0, n], [n, n], [4, 9])
+    gal.read_dev(2 * np.arange(n, dtype=np.int64), None, out.data_ptr(), keys.data_ptr())
+    ctx.sync()
+    assert torch.equal(out, src[::2])
+    assert torch.equal(keys, torch.where(2 * torch.arange(n, device="cuda") < n, 4, 9).int())
+    gal.close()
+    ctx.close()
+    del src, out, keys
+    torch.cuda.empty_cache()
