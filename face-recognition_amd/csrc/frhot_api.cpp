@@ -2372,6 +2372,14 @@ int check_rows_args(const char* what, const void* p, int64_t ld, int64_t M, int6
     return FRHOT_OK;
 }
 
+// Calls that wait or that change a gallery's host-side tables (they change with the call, not with a replay).
+int refuse_capture(frhot_ctx* c) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    HIP_TRY(hipStreamIsCapturing(c->stream, &st));
+    if (st != hipStreamCaptureStatusNone) return fail(FRHOT_ESTATE, "the call cannot be captured into a graph");
+    return FRHOT_OK;
+}
+
 void head_free(frhot_head* h) {
     void* ptrs[] = {h->in16, h->mid[0], h->mid[1], h->y, h->desc};
     for (void* p : ptrs) if (p) (void)hipFree(p);
@@ -2556,6 +2564,8 @@ int frhot_head_apply(frhot_head* h, const float* x, int M, float* out) {
     frhot_ctx* c = h->ctx;
     std::lock_guard<std::mutex> lk(c->mu);
     DeviceGuard dg(c->device);
+    const int held = refuse_capture(c);
+    if (held) return held;
     const size_t nx = (size_t)M * h->din, no = (size_t)M * h->dout;
     std::vector<_Float16> x16(nx), o16(no);
     for (size_t i = 0; i < nx; ++i) x16[i] = (_Float16)x[i];
@@ -2625,13 +2635,6 @@ int page_check_disjoint(const int64_t* first, const int32_t* counts, int nruns, 
     return FRHOT_OK;
 }
 
-int page_refuse_capture(frhot_ctx* c) {
-    // the galleries' host-side tables change with the call, not with a replay
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    HIP_TRY(hipStreamIsCapturing(c->stream, &st));
-    if (st != hipStreamCaptureStatusNone) return fail(FRHOT_ESTATE, "page calls cannot be captured into a graph");
-    return FRHOT_OK;
-}
 // Page-locked memory for a page call of the stream; mark behind the launch that reads it.
 int page_pin_take(frhot_ctx* c, size_t words, IndexPin** out) {
     IndexPin& ip = c->page_pin[c->page_next++ & 3];
@@ -2672,7 +2675,7 @@ int page_move_enqueue(frhot_ctx* c, const PageSide& src, const int64_t* src_firs
     size_t items = 0;
     for (int i = 0; i < nruns; ++i) items += (size_t)((counts ? counts[i] : 1) + kPageRows - 1) / kPageRows;
     if (items > 0x7fffffffu) return fail(FRHOT_ECAPACITY, "%zu row runs in one call", items);
-    int rc = page_refuse_capture(c);
+    int rc = refuse_capture(c);
     if (rc) return rc;
     IndexPin* ip = nullptr;
     PageItem few[kPageInline];
@@ -2708,6 +2711,10 @@ void page_note_writes(frhot_gallery* g, const std::vector<std::pair<int64_t, int
     g->dense = dense;
     g->nrows = end;
     if (!keys) { g->key_tiles_valid = false; return; }
+    struct Guard {                  // lists that memory ran out for are rebuilt from the device when next needed
+        frhot_gallery* g; bool whole;
+        ~Guard() { if (!whole) g->key_tiles_valid = false; }
+    } guard{g, false};
     auto add = [&](int64_t lo, int64_t hi, int32_t key) {
         if (key < 0) return;
         for (int64_t r = lo; r < hi; r = ((r >> 8) + 1) << 8) key_tiles_add(g, &r, &key, 1);
@@ -2718,6 +2725,7 @@ void page_note_writes(frhot_gallery* g, const std::vector<std::pair<int64_t, int
     } else {
         for (int i = 0; i < nruns; ++i) add(first[i], first[i] + (counts ? counts[i] : 1), keys[i]);
     }
+    guard.whole = true;
 }
 
 }  // namespace
@@ -2766,6 +2774,7 @@ int frhot_gallery_read_dev(frhot_gallery* g, const int64_t* rows, const int32_t*
     if (!g || !rows || !out_f16_dev) return fail(FRHOT_EINVAL, "null argument");
     if (nruns <= 0) return fail(FRHOT_EINVAL, "nruns must be positive");
     if ((uintptr_t)out_f16_dev % 16) return fail(FRHOT_EINVAL, "out is not 16-byte aligned");
+    if ((uintptr_t)out_keys_dev % 4) return fail(FRHOT_EINVAL, "out_keys is not aligned to its elements");
     frhot_ctx* c = g->ctx;
     std::lock_guard<std::mutex> lk(c->mu);
     int64_t total = 0;
@@ -2813,9 +2822,10 @@ int frhot_gallery_free_keys(frhot_gallery* g, const int32_t* keys, int nkeys, in
     frhot_ctx* c = g->ctx;
     std::lock_guard<std::mutex> lk(c->mu);
     DeviceGuard dg(c->device);
-    if (g->nrows == 0) return FRHOT_OK;
+    int rc = refuse_capture(c);
+    if (rc || g->nrows == 0) return rc;
     if (!g->key_tiles_off && !g->key_tiles_valid) {
-        const int rc = key_tiles_rebuild(g);
+        rc = key_tiles_rebuild(g);
         if (rc) return rc;
     }
     // only the tiles that may hold one of the keys are looked at (all of them once the lists were given up)
@@ -2844,8 +2854,7 @@ int frhot_gallery_free_keys(frhot_gallery* g, const int32_t* keys, int nkeys, in
     }
     const size_t nr = runs.size();
     IndexPin* ip = nullptr;
-    int rc = page_refuse_capture(c);
-    if (!rc) rc = page_pin_take(c, 3 * nr + want.size(), &ip);
+    rc = page_pin_take(c, 3 * nr + want.size(), &ip);
     if (rc) return rc;
     TileRun* const rl = (TileRun*)ip->p;
     int32_t *counts = ip->p + 2 * nr, *wk = counts + nr;
@@ -2882,6 +2891,8 @@ int frhot_gallery_compact(frhot_gallery* src, frhot_gallery* dst, int64_t* new_r
     hipStream_t s = c->stream;
     frhot_gallery* g = dst ? dst : src;
     int64_t live = 0;
+    int rc = refuse_capture(c);
+    if (rc) return rc;
     if (src->nrows == 0) {
         HIP_TRY(launch_page_kill(g->keys, 0, g->nrows, s));
     } else {
@@ -2895,8 +2906,7 @@ int frhot_gallery_compact(frhot_gallery* src, frhot_gallery* dst, int64_t* new_r
             c->page_off_cap = cap;
         }
         IndexPin* ip = nullptr;
-        int rc = page_refuse_capture(c);
-        if (!rc) rc = page_pin_take(c, 16, &ip);
+        rc = page_pin_take(c, 16, &ip);
         if (rc) return rc;
         ip->p[0] = kUntold;
         if (dst && dst->capacity < src->nrows) {
@@ -2970,16 +2980,19 @@ int frhot_gallery_reproject(frhot_gallery* src, frhot_head* h, frhot_gallery* ds
     std::lock_guard<std::mutex> lk(c->mu);
     if (dst->capacity < src->nrows) return fail(FRHOT_ECAPACITY, "%lld rows, capacity %lld", (long long)src->nrows, (long long)dst->capacity);
     DeviceGuard dg(c->device);
+    int rc = refuse_capture(c);
+    if (rc) return rc;
     if (src->nrows > 0) {
-        const int rc = head_enqueue(h, src->rows, 0, true, src->nrows, UnitOut{dst->rows, 0, 1, 0, src->keys, dst->keys});
+        rc = head_enqueue(h, src->rows, 0, true, src->nrows, UnitOut{dst->rows, 0, 1, 0, src->keys, dst->keys});
         if (rc) return rc;
     }
     HIP_TRY(launch_page_kill(dst->keys, src->nrows, dst->nrows, c->stream));
     dst->nrows = src->nrows;
     dst->dense = src->dense;
+    dst->key_tiles_off = src->key_tiles_off;
+    dst->key_tiles_valid = false;           // (until the lists are copied: that may run out of memory)
     dst->key_tiles = src->key_tiles;
     dst->key_tiles_entries = src->key_tiles_entries;
-    dst->key_tiles_off = src->key_tiles_off;
     dst->key_tiles_valid = src->key_tiles_valid;
     return FRHOT_OK;
     });

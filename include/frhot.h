@@ -413,7 +413,8 @@ int frhot_ctx_stage_ms(frhot_ctx* ctx, float* ms5);
  *   The layers stay the caller's and must outlive the head.
  * frhot_head_dev: fp16 rows x [M,din] -> unit fp16 rows out [M,dout].
  * frhot_head_apply: the same for host rows (x [M,din] float32, rounded to fp16; out [M,dout] float32
- *   holding the fp16 rows), for a few descriptors at a time (M up to 2048 at least); waits.
+ *   holding the fp16 rows), for a few descriptors at a time (M up to 2048 at least); waits, and is
+ *   FRHOT_ESTATE on a stream under graph capture.
  * frhot_ctx_head: attach (or, NULL, detach) a head of 4096 inputs: frhot_embed_dev with Dq equal to
  *   its outputs and frhot_recognise* on a gallery of that dimension then use the head's rows as
  *   queries, where they take the descriptor's leading components otherwise.  Destroying an attached
@@ -438,8 +439,8 @@ int frhot_ctx_head(frhot_ctx* ctx, frhot_head* head);
  * memory.  Rows are given as runs: run i is rows first[i] .. first[i] + counts[i] - 1 (counts NULL:
  * one row each).  Row lists are host memory and checked before anything is enqueued: a run outside
  * the capacity is FRHOT_ECAPACITY; an empty run, a destination row named twice, or a row that one
- * frhot_gallery_copy call both reads and writes is FRHOT_EINVAL; on a stream under graph capture they
- * are FRHOT_ESTATE.  Searches enqueued afterwards see the change.
+ * frhot_gallery_copy call both reads and writes is FRHOT_EINVAL.  On a stream under graph capture
+ * every one of these calls is FRHOT_ESTATE.  Searches enqueued afterwards see the change.
  *
  * frhot_gallery_copy: rows of src to rows of dst (the same gallery or another one of the same
  *   dimension and context) under keys[i] per run (>= 0), or with the rows' own keys (keys NULL; dead rows

@@ -596,3 +596,49 @@ def test_more_runs_than_a_launch_has_threads():
     ctx.close()
     del src, out, keys
     torch.cuda.empty_cache()
+
+
+def test_refused_under_capture():
+    """Calls that wait or change the host's tables leave a capture as they found it: it goes on and replays."""
+    from frhot.engine import Context, Gallery, Head, Linear
+    from frhot._lib import FrhotError
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        c = Context(device=0, max_batch=1, stream=s.cuda_stream)
+        lin = Linear(c, np.eye(64, dtype=np.float32))
+        head = Head(c, [(lin, "none", False)])
+        g, h = Gallery(c, 64, 600), Gallery(c, 64, 600)
+        buf = torch.randn(600, 64, device="cuda").half()
+        out = torch.zeros(4, 64, dtype=torch.float16, device="cuda")
+        g.write_dev(buf.data_ptr(), [0, 300], [300, 300], [1, 2])
+        h.copy([0], [0], [600], source=g)                   # (own keys: the key lists of h are rebuilt when next needed)
+        s.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        gr.capture_begin()
+        for call in (lambda: g.free_keys([1]), lambda: h.free_keys([1]), lambda: g.compact(), lambda: g.compact(h),
+                     lambda: g.reproject(head, h), lambda: g.copy([0], [300], [4], 1), lambda: g.read_dev([0], [4], out.data_ptr()),
+                     lambda: g.write_dev(buf.data_ptr(), [0], [4], 1), lambda: head.apply(np.ones((1, 64), np.float32))):
+            with pytest.raises(FrhotError) as e:
+                call()
+            assert e.value.code == -3
+        head.run_dev(buf.data_ptr(), 4, out.data_ptr())
+        gr.capture_end()
+        for _ in range(3):
+            out.zero_()
+            gr.replay()
+            s.synchronize()
+            want = buf[:4].double()
+            assert ((out.double() - want / want.norm(dim=1, keepdim=True)).abs() <= 2.0 ** -10).all()
+        assert (g.rows, h.rows) == (600, 600)
+        assert h.free_keys([1]) == 300 and g.free_keys([1, 2]) == 600 and g.compact() == 0
+        g.close(), h.close(), head.close(), lin.close(), c.close()
+
+
+def test_read_refuses_keys_off_their_alignment(ctx):
+    from frhot._lib import FrhotError
+    p = Pair(ctx, 64, 300, 20)
+    buf = torch.empty(16, 64, dtype=torch.float16, device="cuda")
+    k = torch.empty(16, dtype=torch.int32, device="cuda")
+    with pytest.raises(FrhotError):
+        p.gal.read_dev([0], [4], buf.data_ptr(), k.data_ptr() + 2)
+    p.gal.close()
