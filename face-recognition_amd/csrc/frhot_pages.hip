@@ -10,6 +10,7 @@
 namespace frhot {
 
 typedef unsigned uint4v __attribute__((ext_vector_type(4)));
+typedef int int4v __attribute__((ext_vector_type(4)));
 #define FR_DEV __device__ __forceinline__
 
 namespace {
@@ -158,21 +159,29 @@ __global__ __launch_bounds__(1024) void page_scan_kernel(int32_t* __restrict__ o
     if (tid == 0) { offsets[n] = carry; tell_host(total, carry); }
 }
 
-// Both at once for up to kSmallTiles tiles (65,536 rows): a launch less.
+// Both at once for up to kSmallTiles tiles (65,536 rows): a launch less.  (The keys of a gallery fill whole tiles.)
 constexpr int kSmallTiles = 256;
 __global__ __launch_bounds__(1024) void page_count_scan_kernel(const int32_t* __restrict__ gk, int64_t rows, int ntiles, int32_t* __restrict__ offsets,
                                                                int32_t* __restrict__ total) {
     __shared__ int cnt[kSmallTiles];
     __shared__ int wsum[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int t = wave; t < ntiles; t += 16) {
-        int c = 0;
+    for (int t0 = wave; t0 < ntiles; t0 += 64) {        // four tiles' keys in flight a wave, four consecutive ones a lane
+        int4v k[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t r = (int64_t)t * 256 + i * 64 + lane;
-            c += __popcll(__ballot(r < rows && gk[r < rows ? r : 0] >= 0));
+        for (int u = 0; u < 4; ++u) {
+            const int t = t0 + 16 * u;
+            k[u] = *(const int4v*)(gk + (size_t)(t < ntiles ? t : t0) * 256 + lane * 4);
         }
-        if (lane == 0) cnt[t] = c;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int t = t0 + 16 * u;
+            const int64_t r = (int64_t)t * 256 + lane * 4;
+            int c = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) c += __popcll(__ballot(r + j < rows && k[u][j] >= 0));
+            if (lane == 0 && t < ntiles) cnt[t] = c;
+        }
     }
     __syncthreads();
     const int c = tid < ntiles ? cnt[tid] : 0;          // (ntiles <= 256: the first four waves)
