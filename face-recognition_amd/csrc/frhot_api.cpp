@@ -196,6 +196,7 @@ struct frhot_linear {
     int N = 0, K = 0, dtype = 0;
     void* wt = nullptr;
     float* bias = nullptr;
+    LinearPlan plan;
     int heads = 0;              // heads that hold this layer
 };
 
@@ -314,7 +315,7 @@ int head_enqueue(frhot_head* h, const void* x, int64_t ldx, bool tiled, int64_t 
             }
             LinearCall q{};
             q.x = in; q.ldx = ld; q.tiled = t ? 1 : 0; q.bf16 = 0;
-            q.wt = L.lin->wt; q.bias = L.lin->bias; q.M = n; q.N = L.lin->N; q.K = L.lin->K;
+            q.wt = L.lin->wt; q.bias = L.lin->bias; q.M = n; q.N = L.lin->N; q.K = L.lin->K; q.plan = &L.lin->plan;
             const bool last = l == nl - 1;
             q.out.out = last ? (void*)h->y : h->mid[l & 1];
             q.out.ldo = q.N; q.out.otype = last ? kF32 : kF16; q.out.act = L.act;
@@ -2460,7 +2461,7 @@ int frhot_linear_dev(frhot_linear* l, const void* x_dev, int64_t ldx, int64_t M,
     std::lock_guard<std::mutex> lk(c->mu);
     DeviceGuard dg(c->device);
     LinearCall q{};
-    q.x = x_dev; q.ldx = ldx; q.bf16 = l->dtype == kBF16; q.wt = l->wt; q.bias = l->bias; q.M = M; q.N = l->N; q.K = l->K;
+    q.x = x_dev; q.ldx = ldx; q.bf16 = l->dtype == kBF16; q.wt = l->wt; q.bias = l->bias; q.M = M; q.N = l->N; q.K = l->K; q.plan = &l->plan;
     q.out.out = out_dev; q.out.ldo = ldo; q.out.otype = out_dtype; q.out.act = act;
     q.out.res = residual_dev; q.out.ldr = residual_dev ? ldr : 0; q.out.rtype = residual_dev ? residual_dtype : kF16;
     HIP_TRY(launch_linear(q, c->lin, c->stream));

@@ -168,12 +168,14 @@ struct LinearIn {
     const void* wt; const float* bias; const void* zeros; float* slab;
     int M, K, npad, panels, ksteps, ksteps_per_split, splits, mtiles, ntiles, m_fast;
 };
+struct LinearPlan { int64_t M = 0; int whole = 0, shape = 0, splits = 0, gather = 0; };     // what calls of M rows of a layer run as
 struct LinearCall {
     const void* x; int64_t ldx;     // [M, K] fp16 or bf16 rows ldx elements apart; tiled: rows 0.. of a gallery of dimension K (x = a tile's start)
     int tiled, bf16;
     const void* wt; const float* bias;      // launch_linear_layout's result; linear_npad(N) floats
     int64_t M; int N, K;
     LinearOut out;
+    LinearPlan* plan;               // the layer's last one (kept by its sizes: estimating takes 0.5 us of a 4 us call)
 };
 // Device scratch of the linear kernels.  Calls that use one such scratch must be ordered among themselves.
 struct LinearWork { float* slabs; size_t slab_bytes; void* pack; size_t pack_bytes; const void* zeros; };   // zeros: 128 bytes of 0

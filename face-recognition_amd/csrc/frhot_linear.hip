@@ -178,16 +178,25 @@ FR_DEV void finish(const LinearOut& o, const float (&b)[W], size_t m, int n, flo
     }
 }
 
-// Eight 16-bit elements at any address, zeros from the n-th on (nothing behind them is read).
-FR_DEV uint4v load_tail(const uint16_t* p, int n) {
-    if (n >= 8) return __builtin_bit_cast(uint4v, *(const vect<uint16_t, 8>::type*)p);
-    uint4v o;
+// Elements k0 .. k0+7 of a row of K at any address, zeros from the K-th on (nothing outside the row is read): where the row ends
+// inside or in front of them, the row's last eight are loaded and shifted down.
+FR_DEV uint4v load_chunk(const uint16_t* row, int k0, int K) {
+    if (K < 8) {
+        uint4v o;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const unsigned lo = 2 * e < n ? p[2 * e] : 0u, hi = 2 * e + 1 < n ? p[2 * e + 1] : 0u;
-        o[e] = lo | (hi << 16);
+        for (int e = 0; e < 4; ++e) {
+            const unsigned lo = k0 + 2 * e < K ? row[k0 + 2 * e] : 0u, hi = k0 + 2 * e + 1 < K ? row[k0 + 2 * e + 1] : 0u;
+            o[e] = lo | (hi << 16);
+        }
+        return o;
     }
-    return o;
+    typedef unsigned long long ulong2v __attribute__((ext_vector_type(2)));
+    const int at = min(k0, K - 8), b = (k0 - at) * 16;         // (b: 0 .. 16 * (k0 - K + 8))
+    const ulong2v v = __builtin_bit_cast(ulong2v, *(const vect<uint16_t, 8>::type*)(row + at));
+    ulong2v o;
+    o[0] = b == 0 ? v[0] : b < 64 ? (v[0] >> (b & 63)) | (v[1] << (64 - b & 63)) : b < 128 ? v[1] >> (b & 63) : 0ull;
+    o[1] = b < 64 ? v[1] >> (b & 63) : 0ull;
+    return __builtin_bit_cast(uint4v, o);
 }
 
 // w [N][K] -> fragments (see the head of the file); thread = one lane's 16 bytes of one fragment
@@ -217,7 +226,7 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const uint16_t* __rest
     const size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
     if (t >= (size_t)rows * per_row) return;
     const int r = (int)(t / per_row), k0 = (int)(t % per_row) * 8;
-    *(uint4v*)(out + t * 8) = load_tail(x + (size_t)r * ldx + k0, K - k0);
+    *(uint4v*)(out + t * 8) = load_chunk(x + (size_t)r * ldx, k0, K);
 }
 
 // The tile kernel: TM x TN of y (or of a K slice's partial sums) at a time, 64 K-elements per step.  X and W stages arrive by
@@ -278,7 +287,7 @@ struct TileCore {
     FR_DEV static void wait_all() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 };
 
-template <bool BF, int TM, int TN, int WX, int WY, int XS, int WS>
+template <bool BF, int TM, int TN, int WX, int WY, int XS, int WS, bool GATHER>
 __global__ __launch_bounds__(64 * WX * WY) void linear_tile_kernel(LinearIn a, LinearOut o) {
     using Core = TileCore<BF, TM, TN, WX, WY, XS, WS>;
     constexpr int NW = Core::NW, NPX = Core::NPX, NPW = Core::NPW, NY = Core::NY;
@@ -307,20 +316,34 @@ __global__ __launch_bounds__(64 * WX * WY) void linear_tile_kernel(LinearIn a, L
     }
     const int wpanel = n0 >> 4;
     int xk = k_lo, wk = k_lo;                           // what the next issue brings
-    auto next_x = [&](int slot) {
+    uint4v gx[GATHER ? NPX : 1];                        // GATHER: a stage of X on its way through registers
+    auto next_x = [&](int slot) __attribute__((always_inline)) {
         char* const st = xs + slot * Core::XB;
         if (xk * 64 + 64 <= a.K) {
 #pragma unroll
             for (int i = 0; i < NPX; ++i) {
-                glds16(xp[i], st + (wave + NW * i) * 1024);
+                if constexpr (GATHER) gx[i] = __builtin_bit_cast(uint4v, *(const typename vect<uint16_t, 8>::type*)xp[i]);
+                else glds16(xp[i], st + (wave + NW * i) * 1024);
                 xp[i] += a.xstep;
             }
+        } else if constexpr (GATHER) {
+#pragma unroll
+            for (int i = 0; i < NPX; ++i) gx[i] = load_chunk((const uint16_t*)xp[i] - xk * 64 - c * 8, xk * 64 + c * 8, a.K);
         } else {                                        // chunks behind the K-th element: zeros (K is a multiple of 8 here)
             const bool tail = xk * 64 + c * 8 >= a.K;
 #pragma unroll
             for (int i = 0; i < NPX; ++i) glds16(tail ? (const char*)a.zeros + c * 16 : xp[i], st + (wave + NW * i) * 1024);
         }
         ++xk;
+    };
+    // What is counted by vmcnt stays in the order written: loads into registers are not moved across.
+    auto order = [&]() __attribute__((always_inline)) {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto put_x = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NPX; ++i) *(uint4v*)(xs + slot * Core::XB + (wave + NW * i) * 1024 + lane * 16) = gx[i];
     };
     auto next_w = [&](int slot) {
         char* const st = ws + slot * Core::WB;
@@ -337,7 +360,15 @@ __global__ __launch_bounds__(64 * WX * WY) void linear_tile_kernel(LinearIn a, L
     Core core;
     core.zero();
     // prologue: stages 0 .. D-1
-    if constexpr (Core::DX == Core::DW) {
+    if constexpr (GATHER) {
+        next_w(0);
+        if (Core::DW > 1 && S > 1) next_w(1);
+        next_x(0);
+        put_x(0);
+        if (S > 1) next_x(1);                           // (put into its stage by the first step)
+        Core::wait_all();
+        __builtin_amdgcn_s_waitcnt(0xC07F);             // lgkmcnt(0)
+    } else if constexpr (Core::DX == Core::DW) {
         for (int d = 0; d < Core::DX; ++d)
             if (d < S) { next_w(d); next_x(d); }
         if (S >= Core::DX) Core::wait_keep(); else Core::wait_all();
@@ -364,6 +395,10 @@ __global__ __launch_bounds__(64 * WX * WY) void linear_tile_kernel(LinearIn a, L
         }
         // the stages that the barrier behind the previous step has freed
         if (s + Core::DW < S) next_w(wslot == 0 ? WS - 1 : wslot - 1);
+        if constexpr (GATHER) {
+            order();
+            if (s + 1 < S) put_x(xslot == XS - 1 ? 0 : xslot + 1);
+        }
         if (s + Core::DX < S) next_x(xslot == 0 ? XS - 1 : xslot - 1);
         reads_done();
         core.template read<1>(xb, wb, lane, wx, wy);
@@ -475,7 +510,7 @@ __global__ __launch_bounds__(64 * NW) void linear_wave_kernel(LinearIn a, Linear
                 for (int y = 0; y < FW; ++y) vw[y] = *(const uint4v*)(wp[y] + (size_t)ks * wstep + kk * 1024);
                 const int k0 = ks * 64 + kk * 32 + g0 * 8;
 #pragma unroll
-                for (int x = 0; x < FX; ++x) vx[x] = load_tail((const uint16_t*)xp[x] + k0, a.K - k0);
+                for (int x = 0; x < FX; ++x) vx[x] = load_chunk((const uint16_t*)xp[x], k0, a.K);
 #pragma unroll
                 for (int x = 0; x < FX; ++x)
 #pragma unroll
@@ -722,16 +757,20 @@ hipError_t unit_by_width(const void* x, int64_t ldx, int64_t M, int N, const Uni
 }
 
 template <bool BF, int TM, int TN, int WX, int WY, int XS, int WS>
-hipError_t launch_tile(LinearIn a, const LinearOut& o, int splits, hipStream_t s, bool attr) {
+hipError_t launch_tile(LinearIn a, const LinearOut& o, int splits, bool gather, hipStream_t s, bool attr) {
     using Core = TileCore<BF, TM, TN, WX, WY, XS, WS>;
-    const auto kern = linear_tile_kernel<BF, TM, TN, WX, WY, XS, WS>;
-    if (attr) return hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, Core::LDS);
+    const auto whole = linear_tile_kernel<BF, TM, TN, WX, WY, XS, WS, false>;
+    const auto pieces = linear_tile_kernel<BF, TM, TN, WX, WY, XS, WS, true>;
+    if (attr) {
+        const hipError_t e = hipFuncSetAttribute((const void*)whole, hipFuncAttributeMaxDynamicSharedMemorySize, Core::LDS);
+        return e != hipSuccess ? e : hipFuncSetAttribute((const void*)pieces, hipFuncAttributeMaxDynamicSharedMemorySize, Core::LDS);
+    }
     a.mtiles = (a.M + TM - 1) / TM;
     a.ntiles = (a.npad + TN - 1) / TN;
     a.m_fast = a.mtiles < a.ntiles;
     a.splits = splits;
     a.ksteps_per_split = (a.ksteps + splits - 1) / splits;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(a.mtiles * a.ntiles * splits)), dim3(64 * WX * WY), Core::LDS, s, a, o);
+    hipLaunchKernelGGL(gather ? pieces : whole, dim3((unsigned)(a.mtiles * a.ntiles * splits)), dim3(64 * WX * WY), Core::LDS, s, a, o);
     return hipGetLastError();
 }
 
@@ -764,17 +803,21 @@ hipError_t launch_wave(LinearIn a, const LinearOut& o, int splits, bool gather, 
     return hipGetLastError();
 }
 
-// The tile shapes: what one 64-deep step of a tile takes while the whole chip runs such tiles (one a CU), measured at
-// K = 4096, in microseconds.  Per value of a tile they get cheaper from the first to the last, whose tile waits longest for its
-// own end; the wave kernel's tiles are small enough that a single round of them covers a batch.
-struct Shape { int tm, tn; float step; };
+// The tile shapes and what their tiles take, in microseconds: the first round (256 tiles, one a CU, with the launch) first + steps *
+// first_step, each further one more + steps * more_step.  Fitted to 600 calls of 32 to 4096 tiles, K = 64 to 4096, N = 32 to 2048
+// (7 to 15 % rms).  The wave kernel's small tiles have a batch done in one round; the tile kernel's 128-row tiles run two to a CU,
+// which hides their beginnings and ends (short K: 6533 x 1504 x 128 12.9 us, 28 with the wave kernel); per value the 256-row tiles are
+// the cheapest.
+struct Shape { int tm, tn; float first, first_step, more, more_step; bool pieces; };   // pieces: takes rows that LDS-DMA cannot
 constexpr Shape kShapes[] = {
-    {16, 32, 0.066f},   // wave kernel, 16 waves:  256 x 512 x 4096    8.7 us
-    {32, 32, 0.085f},   // wave kernel,  8 waves:  64 x 4096 x 4096    9.8 us
-    {64, 64, 0.20f},    // wave kernel,  8 waves:  256 x 4096 x 4096  17 us
-    {64, 128, 0.36f},   // wave kernel,  4 waves:  2011 x 1024 x 4096 with gelu 25.7 us (a tile of 128 x 64, more of it through LDS: 27)
-    {256, 128, 1.10f},  // tile kernel:            16384 x 512 x 4096 73 us
-    {256, 256, 1.95f},  // tile kernel:            65536 x 512 x 4096 254 us
+    {16, 32, 4.0f, 0.040f, 2.45f, 0.059f, false},       // wave kernel, 16 waves:  256 x 512 x 4096    8.1 us
+    {32, 32, 3.6f, 0.070f, 0.82f, 0.081f, false},       // wave kernel,  8 waves:  64 x 4096 x 4096    9.8 us
+    {64, 64, 4.8f, 0.165f, 3.05f, 0.22f, false},         // wave kernel,  8 waves:  256 x 4096 x 4096  17 us
+    {64, 128, 6.0f, 0.26f, 4.8f, 0.31f, false},         // wave kernel,  4 waves:  2011 x 1024 x 4096 24 us (128 x 64, more through LDS: 27)
+    {128, 32, 3.2f, 0.33f, 0.63f, 0.57f, true},         // tile kernel, two a CU:  115728 x 32 x 2496 106 us (32 x 32 wave tiles: 121)
+    {128, 64, 3.9f, 0.36f, 1.3f, 0.27f, true},          // tile kernel, two a CU:  13373 x 224 x 1024 14 us (256 x 128: 18)
+    {256, 128, 6.7f, 0.76f, 4.9f, 0.97f, true},         // tile kernel:            16384 x 512 x 4096 70 us
+    {256, 256, 10.6f, 1.23f, 8.6f, 1.57f, true},        // tile kernel:            65536 x 512 x 4096 242 us
 };
 constexpr int kNumShapes = sizeof kShapes / sizeof kShapes[0];
 template <bool BF>
@@ -784,36 +827,51 @@ hipError_t launch_shape(int t, const LinearIn& a, const LinearOut& o, int splits
         case 1: return launch_wave<BF, 2, 2, 8, 2, false>(a, o, splits, gather, s, attr);
         case 2: return launch_wave<BF, 4, 4, 8, 2, false>(a, o, splits, gather, s, attr);
         case 3: return launch_wave<BF, 4, 8, 4, 2, false>(a, o, splits, gather, s, attr);
-        case 4: return launch_tile<BF, 256, 128, 4, 2, 3, 3>(a, o, splits, s, attr);
-        default: return launch_tile<BF, 256, 256, 2, 4, 3, 2>(a, o, splits, s, attr);
+        case 4: return launch_tile<BF, 128, 32, 4, 1, 3, 3>(a, o, splits, gather, s, attr);
+        case 5: return launch_tile<BF, 128, 64, 2, 2, 3, 3>(a, o, splits, gather, s, attr);
+        case 6: return launch_tile<BF, 256, 128, 4, 2, 3, 3>(a, o, splits, gather, s, attr);
+        default: return launch_tile<BF, 256, 256, 2, 4, 3, 2>(a, o, splits, gather, s, attr);
     }
 }
 
 // What a call runs as: the shape, the number of K slices and the way unaligned rows go in, whichever an estimate of the
-// time puts first.  A round of at most 256 tiles takes its K steps; K slices divide the steps and add the join (a launch, and
-// every slice's sums written and read once: 4.5 us + the bytes at 4 TB/s); rows that LDS-DMA cannot take cost a pass
-// that packs them (2.5 us + the bytes at 3 TB/s) or go straight into registers in the smallest shape, 1.8 us per slice of a wave
-// (77 x 131 x 500: 4.5 us against 8.1 packed; 3000 x 500 x 1001: 36 us against 19).
-struct Plan { int shape, splits; bool gather; };
-Plan plan_linear(int64_t M, int npad, int ksteps, bool whole, size_t slab_bytes) {
-    Plan best{0, 1, false};
-    double best_t = 1e30;
-    const double pack = whole ? 0.0 : 2.5 + (double)M * ksteps * 256e-6 / 3.0;
-    for (int i = 0; i < kNumShapes; ++i) {
-        const Shape& sh = kShapes[i];
-        const int64_t tiles = (M + sh.tm - 1) / sh.tm * ((npad + sh.tn - 1) / sh.tn);
-        for (int splits = 1; splits <= 16 && splits <= ksteps; splits *= 2) {
-            const double join_bytes = (double)splits * M * npad * 8;
-            if (splits > 1 && (tiles * splits > 512 || join_bytes > 2.0 * slab_bytes)) break;
-            const double t = (double)((tiles * splits + 255) / 256) * ((ksteps + splits - 1) / splits) * sh.step + pack +
-                             (splits > 1 ? 4.5 + join_bytes * 1e-6 / 4.0 : 0.0);
-            if (t < best_t) { best_t = t; best = Plan{i, splits, false}; }
+// time puts first.  K slices divide the steps and add the join (a launch, and every slice's sums written and read once: 3.5 us +
+// the bytes at 4 TB/s).  Rows that LDS-DMA cannot take
+//   go through registers in the tile kernel, whose steps then take about 1.7 times as long (16384 x 512 x 4095: 106 us, 200 packed),
+//   or, for few tiles, in the smallest wave tiles (77 x 131 x 500: 4.8 us, 7.6 packed),
+//   or, if the workspace holds them, are packed by a pass of their own, 2 us + the bytes at 4.5 TB/s (394 x 512 x 4095: 18 us, 31 without).
+LinearPlan plan_linear(int M, int npad, int ksteps, bool whole, int64_t pack_rows, size_t slab_bytes) {
+    LinearPlan best;
+    float best_t = 1e30f;
+    auto consider = [&](float t, int shape, int splits, bool gather) {
+        if (t < best_t) { best_t = t; best.shape = shape; best.splits = splits; best.gather = gather; }
+    };
+    const float sums = (float)M * (float)npad * 4e-6f;          // MB of a slice's sums
+    auto shapes = [&](float extra, float slow, bool gather) {
+        for (int i = 0; i < kNumShapes; ++i) {
+            const Shape& sh = kShapes[i];
+            if (gather && !sh.pieces) continue;
+            const int tiles = (M + sh.tm - 1) / sh.tm * ((npad + sh.tn - 1) / sh.tn);       // (at most 2^18 x 2^11)
+            const float steps = (float)ksteps * slow;
+            consider(extra + sh.first + steps * sh.first_step + (float)((tiles - 1) >> 8) * (sh.more + steps * sh.more_step), i, 1, gather);
+            if (tiles > 256) continue;
+            for (int splits : {2, 3, 4, 6, 8, 12, 16}) {
+                if (splits > ksteps || tiles * splits > 512 || splits * sums * 1e6f > (float)slab_bytes) break;
+                const float part = (float)((ksteps + splits - 1) / splits) * slow;
+                consider(extra + sh.first + part * sh.first_step + (float)((tiles * splits - 1) >> 8) * (sh.more + part * sh.more_step) + 3.5f +
+                             splits * sums * 0.5f, i, splits, gather);
+            }
         }
-        if (i == 0 && !whole) {
-            const double t = (double)((tiles + 255) / 256) * ((ksteps + 15) / 16) * 1.8;
-            if (t < best_t) { best_t = t; best = Plan{0, 1, true}; }
-        }
+    };
+    if (whole) {
+        shapes(0.f, 1.f, false);
+        return best;
     }
+    if (M <= pack_rows) shapes(2.f + (float)M * (float)ksteps * 256e-6f / 4.5f, 1.f, false);
+    shapes(0.f, 1.7f, true);
+    const int tiles = (M + 15) / 16 * ((npad + 31) / 32);
+    const float slices = (float)((ksteps + 15) / 16);           // of a wave
+    consider(2.8f + 1.25f * slices + (float)((tiles - 1) >> 8) * (2.6f + 1.9f * slices), 0, 1, true);
     return best;
 }
 
@@ -831,7 +889,7 @@ hipError_t launch_linear_layout(const void* w, void* wt, int N, int K, hipStream
 }
 
 hipError_t launch_linear(const LinearCall& q, const LinearWork& ws, hipStream_t s) {
-    if (q.M <= 0 || q.N <= 0 || q.K <= 0 || !q.x || !q.wt || !q.bias || !q.out.out || !ws.slabs || !ws.pack || !ws.zeros)
+    if (q.M <= 0 || q.N <= 0 || q.K <= 0 || !q.x || !q.wt || !q.bias || !q.out.out || !ws.slabs || !ws.pack || !ws.zeros || !q.plan)
         return hipErrorInvalidValue;
     LinearIn a{};
     a.wt = q.wt; a.bias = q.bias; a.zeros = ws.zeros;
@@ -839,22 +897,24 @@ hipError_t launch_linear(const LinearCall& q, const LinearWork& ws, hipStream_t 
     // can LDS-DMA take the rows?
     const bool whole = q.tiled || (q.K % 8 == 0 && q.ldx % 8 == 0 && (size_t)q.x % 16 == 0);
     const size_t row_bytes = (size_t)linear_kpad(q.K) * 2;
-    const Plan plan = plan_linear(q.M < kRunRows ? q.M : kRunRows, a.npad, a.ksteps, whole, ws.slab_bytes);
-    const bool direct = whole || plan.gather;
-    // rows that must be packed first go through the workspace in runs of whole tiles; others in runs of which no shape makes
-    // 2^32 threads, the most that a launch may have
-    const int64_t run = direct ? kRunRows : (int64_t)(ws.pack_bytes / row_bytes) / 256 * 256;
-    if (run <= 0) return hipErrorInvalidValue;
-    for (int64_t m0 = 0; m0 < q.M; m0 += run) {
-        const int rows = (int)(q.M - m0 < run ? q.M - m0 : run);
+    const int64_t pack_rows = (int64_t)(ws.pack_bytes / row_bytes);
+    if (q.plan->M != q.M || q.plan->whole != whole) {
+        *q.plan = plan_linear((int)(q.M < kRunRows ? q.M : kRunRows), a.npad, a.ksteps, whole, pack_rows, ws.slab_bytes);
+        q.plan->M = q.M;
+        q.plan->whole = whole;
+    }
+    const LinearPlan& plan = *q.plan;
+    const bool pack = !whole && !plan.gather;
+    for (int64_t m0 = 0; m0 < q.M; m0 += kRunRows) {        // (a launch has fewer than 2^32 threads)
+        const int rows = (int)(q.M - m0 < kRunRows ? q.M - m0 : kRunRows);
         a.M = rows;
-        if (direct) {
+        if (!pack) {
             a.ldx = q.ldx; a.tiled = q.tiled; a.xtile = (size_t)(q.K / 64) * 32768; a.xstep = q.tiled ? 32768 : 128;
             a.x = (const char*)q.x + (q.tiled ? (size_t)(m0 / 256) * a.xtile : (size_t)m0 * q.ldx * 2);
-        } else {
+        } else {                                            // (M <= pack_rows: one run)
             const size_t n = (size_t)rows * (row_bytes / 16);
-            hipLaunchKernelGGL(linear_pack_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s,
-                               (const uint16_t*)q.x + (size_t)m0 * q.ldx, q.ldx, q.K, (int)(row_bytes / 2), (uint16_t*)ws.pack, rows);
+            hipLaunchKernelGGL(linear_pack_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, (const uint16_t*)q.x, q.ldx, q.K,
+                               (int)(row_bytes / 2), (uint16_t*)ws.pack, rows);
             const hipError_t e = hipGetLastError();
             if (e != hipSuccess) return e;
             a.x = ws.pack; a.ldx = (int64_t)(row_bytes / 2); a.tiled = 0; a.xtile = 0; a.xstep = 128;

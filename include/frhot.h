@@ -399,8 +399,8 @@ int frhot_ctx_stage_ms(frhot_ctx* ctx, float* ms5);
  * frhot_linear_dev: out[m][n] = round(act(sum_k x[m][k] w[n][k] + bias[n]) + residual[m][n]), products
  *   summed in fp32, rounded once.  x [M,K] of the layer's type, residual [M,N] (or NULL) and out [M,N]
  *   of the given types; ldx / ldr / ldo elements from row to row, any alignment that their elements
- *   have (rows that LDS-DMA cannot take, i.e. K or ldx not a multiple of 8 or x not 16-byte
- *   aligned, cost large calls an extra pass).  Nothing beyond out's N columns and M rows is written, nothing
+ *   have (rows that 16-byte LDS-DMA cannot take, i.e. K or ldx not a multiple of 8 or x not 16-byte
+ *   aligned, make a large call take up to 1.7 times as long).  Nothing beyond out's N columns and M rows is written, nothing
  *   beyond K columns read.  out may be the residual itself (same address, row distance and element
  *   size) and may not overlap x or the residual otherwise.  M = 0 does nothing.
  * frhot_unit_rows_dev: out[m] = fp16(x[m] / |x[m]|), x [M,N] of any type: norm and rounding as

@@ -144,6 +144,40 @@ def test_packed_rows_in_several_runs(ctx):
     run_and_check(ctx, 9000, 40, 4097, "f16", out="f32", padx=2)
 
 
+@pytest.mark.parametrize("m,n,k,padx,offx", [(9001, 137, 358, 0, 0), (20011, 19, 613, 1, 1), (3001, 700, 7, 0, 0), (2100, 300, 1, 2, 0),
+                                             (4097, 512, 999, 0, 3), (12000, 1100, 65, 0, 1), (5000, 520, 2049, 3, 0), (70000, 33, 127, 0, 0),
+                                             (33000, 600, 130, 6, 5), (394, 512, 4095, 0, 0), (20000, 600, 136, 1, 0), (300, 2100, 4097, 0, 7)])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_many_rows_off_16_bytes(ctx, m, n, k, padx, offx, dtype):
+    """Row addresses, row distances and widths that LDS-DMA cannot take, in every tile that takes them; NaN behind every row."""
+    run_and_check(ctx, m, n, k, dtype, act="relu", out="f32", padx=padx, offx=offx)
+
+
+@pytest.mark.parametrize("m,n,k", [(98304, 160, 384), (6533, 1504, 128), (13373, 224, 1024), (24000, 256, 448), (50001, 32, 64), (30112, 32, 2944),
+                                   (21342, 96, 576), (644, 288, 320), (2595, 1568, 704), (40000, 30, 200)])
+def test_tiles_of_short_and_narrow_layers(ctx, m, n, k):
+    run_and_check(ctx, m, n, k, "f16", act="silu", out="f16")
+
+
+def test_one_layer_called_at_many_sizes(ctx):
+    """Row counts and alignments in turn on one layer: each call as if it were the only one."""
+    n, k = 160, 520
+    x, w, b, _ = make(5000, n, k, "f16", 77)
+    lin = linear_of(ctx, w, b, "f16")
+    y, tol = layer64(x, w, b, "relu", None)
+    tol = tol + rounding(y.abs() + tol, "f32")
+    bufs = {pad: padded(x, k + pad, 0)[0] for pad in (0, 3)}
+    o = torch.empty(5000, n, device="cuda")
+    for m, pad in ((1, 0), (5000, 0), (5000, 3), (5000, 0), (77, 3), (77, 0), (1, 3), (300, 0), (300, 3), (1, 0)):
+        o.fill_(7.0)
+        torch.cuda.synchronize()
+        lin.run_dev(bufs[pad].data_ptr(), m, o.data_ptr(), act="relu", ldx=k + pad, out_dtype="f32")
+        ctx.sync()
+        got = o.cpu().double()
+        assert ((got[:m] - y[:m]).abs() <= tol[:m]).all() and (got[m:] == 7).all(), (m, pad)
+    lin.close()
+
+
 def test_nonfinite_values_stay_in_their_rows(ctx):
     m, n, k = 40, 64, 128
     x, w, b, r = make(m, n, k, "f16", 3, residual="f16")
