@@ -786,6 +786,21 @@ void key_tiles_add(frhot_gallery* g, const int64_t* rows, const int32_t* keys, i
     }
 }
 
+// Tiles lo .. hi into a key's list; false: the lists have grown past their limit and are dropped (`list` with them).
+bool key_tiles_add_tiles(frhot_gallery* g, std::vector<int32_t>& list, int32_t lo, int32_t hi) {
+    for (int32_t t = lo; t <= hi; ++t) {
+        if (list.empty() || list.back() < t) {
+            list.push_back(t);
+        } else {
+            const auto it = std::lower_bound(list.begin(), list.end(), t);
+            if (*it == t) continue;
+            list.insert(it, t);
+        }
+        if (++g->key_tiles_entries > g->key_tiles_limit()) { key_tiles_drop(g); return false; }
+    }
+    return true;
+}
+
 // Rebuild from the keys in device memory (after a fill that generated them there).
 int key_tiles_rebuild(frhot_gallery* g) {
     g->key_tiles.clear();
@@ -2670,11 +2685,14 @@ int page_await(frhot_ctx* c, volatile int32_t* words, size_t n) {
     return FRHOT_OK;
 }
 
-// Runs -> items of at most kPageRows rows (in page-locked memory, if they are many), moved by one launch.  A null side's `first` counts from 0 on.
+// Runs -> items of at most page_item_rows rows (in page-locked memory, if they are many), moved by one launch.  A null side's `first` counts from 0 on.
 int page_move_enqueue(frhot_ctx* c, const PageSide& src, const int64_t* src_first, const PageSide& dst, const int64_t* dst_first,
                       const int32_t* counts, const int32_t* keys, int nruns, int D) {
+    int64_t rows = 0;
+    for (int i = 0; i < nruns; ++i) rows += counts ? counts[i] : 1;
+    const int32_t most = page_item_rows(rows, D);
     size_t items = 0;
-    for (int i = 0; i < nruns; ++i) items += (size_t)((counts ? counts[i] : 1) + kPageRows - 1) / kPageRows;
+    for (int i = 0; i < nruns; ++i) items += (size_t)((counts ? counts[i] : 1) + most - 1) / most;
     if (items > 0x7fffffffu) return fail(FRHOT_ECAPACITY, "%zu row runs in one call", items);
     int rc = refuse_capture(c);
     if (rc) return rc;
@@ -2691,8 +2709,8 @@ int page_move_enqueue(frhot_ctx* c, const PageSide& src, const int64_t* src_firs
     for (int i = 0; i < nruns; ++i) {
         const int32_t n = counts ? counts[i] : 1;
         const int64_t s0 = src_first ? src_first[i] : dense, d0 = dst_first ? dst_first[i] : dense;
-        for (int32_t at = 0; at < n; at += kPageRows)
-            it[k++] = PageItem{s0 + at, d0 + at, n - at < kPageRows ? n - at : kPageRows, keys ? keys[i] : kKeepKey};
+        for (int32_t at = 0; at < n; at += most)
+            it[k++] = PageItem{s0 + at, d0 + at, n - at < most ? n - at : most, keys ? keys[i] : kKeepKey};
         dense += n;
     }
     HIP_TRY(launch_page_move(src, dst, it, (int)items, dense, D, c->stream));
@@ -2716,15 +2734,16 @@ void page_note_writes(frhot_gallery* g, const std::vector<std::pair<int64_t, int
         frhot_gallery* g; bool whole;
         ~Guard() { if (!whole) g->key_tiles_valid = false; }
     } guard{g, false};
-    auto add = [&](int64_t lo, int64_t hi, int32_t key) {
-        if (key < 0) return;
-        for (int64_t r = lo; r < hi; r = ((r >> 8) + 1) << 8) key_tiles_add(g, &r, &key, 1);
-    };
-    // one key for all runs (a fork): in ascending order every tile goes to the end of the key's list
-    if (std::all_of(keys, keys + nruns, [&](int32_t k) { return k == keys[0]; })) {
-        for (const auto& r : sorted) add(r.first, r.second, keys[0]);
-    } else {
-        for (int i = 0; i < nruns; ++i) add(first[i], first[i] + (counts ? counts[i] : 1), keys[i]);
+    if (!g->key_tiles_off && g->key_tiles_valid) {
+        // one key for all runs (a fork): in ascending order every tile goes to the end of the key's list
+        const bool one = std::all_of(keys, keys + nruns, [&](int32_t k) { return k == keys[0]; });
+        std::vector<int32_t>* list = nullptr;
+        for (int i = 0; i < nruns; ++i) {
+            if (keys[i] < 0) continue;
+            if (!list || !one) list = &g->key_tiles[keys[i]];
+            const int64_t lo = one ? sorted[i].first : first[i], hi = one ? sorted[i].second : first[i] + (counts ? counts[i] : 1);
+            if (!key_tiles_add_tiles(g, *list, (int32_t)(lo >> 8), (int32_t)((hi - 1) >> 8))) break;
+        }
     }
     guard.whole = true;
 }
@@ -2755,12 +2774,18 @@ int frhot_gallery_copy(frhot_gallery* src, const int64_t* src_rows, frhot_galler
     for (int i = 0; i < nruns; ++i) inside = inside && src_rows[i] + (counts ? counts[i] : 1) <= src->nrows;
     if (src == dst) {
         // a row that is read and written in one call would be copied before or after its change
+        int64_t first = INT64_MAX, last = 0;
         for (int i = 0; i < nruns; ++i) {
-            const int64_t lo = src_rows[i], hi = lo + (counts ? counts[i] : 1);
-            auto it = std::upper_bound(to.begin(), to.end(), std::make_pair(lo, INT64_MAX));
-            if ((it != to.begin() && std::prev(it)->second > lo) || (it != to.end() && it->first < hi))
-                return fail(FRHOT_EINVAL, "rows [%lld,%lld) are read and written by one call", (long long)lo, (long long)hi);
+            first = std::min(first, src_rows[i]);
+            last = std::max(last, src_rows[i] + (counts ? counts[i] : 1));
         }
+        if (first < to.back().second && to.front().first < last)        // (else the two ranges of rows do not touch)
+            for (int i = 0; i < nruns; ++i) {
+                const int64_t lo = src_rows[i], hi = lo + (counts ? counts[i] : 1);
+                auto it = std::upper_bound(to.begin(), to.end(), std::make_pair(lo, INT64_MAX));
+                if ((it != to.begin() && std::prev(it)->second > lo) || (it != to.end() && it->first < hi))
+                    return fail(FRHOT_EINVAL, "rows [%lld,%lld) are read and written by one call", (long long)lo, (long long)hi);
+            }
     }
     DeviceGuard dg(c->device);
     rc = page_move_enqueue(c, PageSide{src->rows, src->keys, 0}, src_rows, PageSide{dst->rows, dst->keys, 0}, dst_rows, counts, keys, nruns, src->D);

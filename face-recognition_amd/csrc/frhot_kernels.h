@@ -192,8 +192,10 @@ hipError_t linear_kernels_init();
 
 // ---- pages of a gallery (frhot_pages.hip) ----
 constexpr int32_t kKeepKey = INT32_MIN;
-struct PageItem { int64_t src, dst; int32_t n, key; };     // n <= kPageRows rows src.. -> dst..; key: the new key or kKeepKey
-constexpr int kPageRows = 64;
+struct PageItem { int64_t src, dst; int32_t n, key; };     // n <= 256 rows src.. -> dst..; key: the new key or kKeepKey
+// Rows of an item: 64 (1 M rows of 512: 404 us, 411 with 256), but 256 where a row is a few pieces of 128 bytes and the rows are many,
+// so that a block has work for the time that reading its item takes.
+inline int page_item_rows(int64_t rows, int D) { return D < 256 && rows >= 65536 ? 256 : 64; }
 struct PageSide { void* rows; int32_t* keys; int dense; };  // a gallery's rows and keys, or a dense [n, D] buffer and its keys (or null)
 // Up to kPageInline items are read here and now; a longer list is read by the kernel (page-locked host memory will do).
 constexpr int kPageInline = 64;

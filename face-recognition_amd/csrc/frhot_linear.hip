@@ -459,7 +459,8 @@ __global__ __launch_bounds__(64 * WX * WY) void linear_tile_kernel(LinearIn a, L
 // wave order, through LDS.  Weight fragments (1 KiB of consecutive bytes) are loaded straight into registers; X goes through
 // LDS by LDS-DMA, eight rows of 128 bytes an instruction: in fragment order consecutive lanes read different rows, which the
 // load path serves 16 bytes a clock (38 GB/s per CU measured, against 110-145 for whole lines).
-// GATHER: rows that LDS-DMA cannot take (not 16-byte aligned, K not a multiple of 8), by unaligned loads into registers.
+// GATHER: rows that LDS-DMA cannot take (not 16-byte aligned, K not a multiple of 8) go through registers into the stage, whole lines
+// of a row by consecutive lanes as well (41 x 429 x 3647: 7.6 us, 16 in fragment order straight into registers).
 template <int FX, int FW, int NW, int ST>
 struct WaveShape {
     static constexpr int TM = 16 * FX, TN = 16 * FW, ER = TN + 4;
@@ -480,7 +481,6 @@ __global__ __launch_bounds__(64 * NW) void linear_wave_kernel(LinearIn a, Linear
     const int z = id / tiles, t = id % tiles;
     const int m0 = (a.m_fast ? t % a.mtiles : t / a.ntiles) * TM, n0 = (a.m_fast ? t / a.mtiles : t % a.ntiles) * TN;
     const int k_lo = z * a.ksteps_per_split, k_hi = min(a.ksteps, k_lo + a.ksteps_per_split);
-    const int n = (k_hi - k_lo - wave + NW - 1) / NW;       // slices of this wave: k_lo + wave, + NW, ...
 
     const char* wp[FW];
 #pragma unroll
@@ -497,75 +497,100 @@ __global__ __launch_bounds__(64 * NW) void linear_wave_kernel(LinearIn a, Linear
 #pragma unroll
         for (int x = 0; x < FX; ++x) acc[y][x] = float4v{0.f, 0.f, 0.f, 0.f};
 
+    char* const st0 = smem + wave * ((GATHER ? 1 : ST) * Shape::XB);
+    const int c = (lane & 7) ^ (lane >> 3);             // the 16-byte chunk this lane fetches of its row
+    const char* xp[2 * FX];
+#pragma unroll
+    for (int i = 0; i < 2 * FX; ++i) xp[i] = row_at(8 * i + (lane >> 3)) + c * 16;
+    const char* const zeros = (const char*)a.zeros + c * 16;
+    uint4v bw[GATHER ? 2 : ST][2][FW], bx[2 * FX];
+    // slice i -> X stage p (GATHER: registers) and weight registers
+    auto issue = [&](int i, int p, uint4v (&vw)[2][FW]) __attribute__((always_inline)) {
+        const int ks = k_lo + wave + NW * i;
+        char* const st = st0 + p * Shape::XB;
+        if constexpr (GATHER) {
+#pragma unroll
+            for (int x = 0; x < 2 * FX; ++x) bx[x] = __builtin_bit_cast(uint4v, *(const typename vect<uint16_t, 8>::type*)(xp[x] + ks * 128));
+        } else if (ks * 64 + 64 <= a.K) {
+#pragma unroll
+            for (int x = 0; x < 2 * FX; ++x) glds16(xp[x] + (size_t)ks * a.xstep, st + x * 1024);
+        } else {                                        // chunks behind the K-th element: zeros (K is a multiple of 8 here)
+            const bool tail = ks * 64 + c * 8 >= a.K;
+#pragma unroll
+            for (int x = 0; x < 2 * FX; ++x) glds16(tail ? zeros : xp[x] + (size_t)ks * a.xstep, st + x * 1024);
+        }
+#pragma unroll
+        for (int y = 0; y < FW; ++y)
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) vw[kk][y] = *(const uint4v*)(wp[y] + (size_t)ks * wstep + kk * 1024);
+    };
+    auto mma = [&](int p, const uint4v (&vw)[2][FW]) __attribute__((always_inline)) {
+        const char* const st = st0 + p * Shape::XB;
+        uint4v vx[2][FX];
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+            for (int x = 0; x < FX; ++x)
+                vx[kk][x] = *(const uint4v*)(st + (x * 16 + l15) * 128 + (((kk * 4 + g0) ^ (lane & 7)) << 4));
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0xC07F);             // lgkmcnt(0): the stage has been read and may be refilled
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+            for (int x = 0; x < FX; ++x)
+#pragma unroll
+                for (int y = 0; y < FW; ++y) acc[y][x] = mfma<BF>(vw[kk][y], vx[kk][x], acc[y][x]);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const int slices = (k_hi - k_lo - wave + NW - 1) / NW;  // of this wave: k_lo + wave, + NW, ...
+    int i = 0;
     if constexpr (GATHER) {
-        const char* xp[FX];
+        // The slice after next comes into registers while one is multiplied; the slice that the row ends in is the last, by itself.
+        auto fence = [&]() __attribute__((always_inline)) { asm volatile("" ::: "memory"); __builtin_amdgcn_wave_barrier(); };
+        auto put = [&]() __attribute__((always_inline)) {   // (the stage is the wave's own: no other wave reads it)
 #pragma unroll
-        for (int x = 0; x < FX; ++x) xp[x] = row_at(x * 16 + l15);
-        for (int i = 0; i < n; ++i) {
-            const int ks = k_lo + wave + NW * i;
-#pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                uint4v vw[FW], vx[FX];
-#pragma unroll
-                for (int y = 0; y < FW; ++y) vw[y] = *(const uint4v*)(wp[y] + (size_t)ks * wstep + kk * 1024);
-                const int k0 = ks * 64 + kk * 32 + g0 * 8;
-#pragma unroll
-                for (int x = 0; x < FX; ++x) vx[x] = load_chunk((const uint16_t*)xp[x], k0, a.K);
-#pragma unroll
-                for (int x = 0; x < FX; ++x)
-#pragma unroll
-                    for (int y = 0; y < FW; ++y) acc[y][x] = mfma<BF>(vw[y], vx[x], acc[y][x]);
+            for (int x = 0; x < 2 * FX; ++x) *(uint4v*)(st0 + x * 1024 + lane * 16) = bx[x];
+            fence();
+        };
+        const bool cut = slices > 0 && (k_lo + wave + NW * (slices - 1)) * 64 + 64 > a.K;
+        const int n = cut ? slices - 1 : slices;
+        if (n > 0) issue(0, 0, bw[0]);
+        for (; i + 3 <= n; i += 2) {                    // nothing in here branches: the compiler can count what is in flight
+            put();
+            issue(i + 1, 0, bw[1]);
+            mma(0, bw[0]);
+            put();
+            issue(i + 2, 0, bw[0]);
+            mma(0, bw[1]);
+        }
+        if (i < n) {
+            put();
+            if (i + 1 < n) issue(i + 1, 0, bw[1]);
+            mma(0, bw[0]);
+            if (i + 1 < n) {
+                put();
+                mma(0, bw[1]);
             }
         }
-    } else {
-        char* const st0 = smem + wave * (ST * Shape::XB);
-        const int c = (lane & 7) ^ (lane >> 3);             // the 16-byte chunk this lane fetches of its row
-        const char* xp[2 * FX];
-#pragma unroll
-        for (int i = 0; i < 2 * FX; ++i) xp[i] = row_at(8 * i + (lane >> 3)) + c * 16;
-        const char* const zeros = (const char*)a.zeros + c * 16;
-        uint4v bw[ST][2][FW];
-        // slice i -> X stage and weight registers p
-        auto issue = [&](int i, int p, uint4v (&vw)[2][FW]) __attribute__((always_inline)) {
-            const int ks = k_lo + wave + NW * i;
-            char* const st = st0 + p * Shape::XB;
-            if (ks * 64 + 64 <= a.K) {
-#pragma unroll
-                for (int x = 0; x < 2 * FX; ++x) glds16(xp[x] + (size_t)ks * a.xstep, st + x * 1024);
-            } else {                                        // chunks behind the K-th element: zeros (K is a multiple of 8 here)
-                const bool tail = ks * 64 + c * 8 >= a.K;
-#pragma unroll
-                for (int x = 0; x < 2 * FX; ++x) glds16(tail ? zeros : xp[x] + (size_t)ks * a.xstep, st + x * 1024);
-            }
+        if (cut) {
+            const int ks = k_lo + wave + NW * n;
 #pragma unroll
             for (int y = 0; y < FW; ++y)
 #pragma unroll
-                for (int kk = 0; kk < 2; ++kk) vw[kk][y] = *(const uint4v*)(wp[y] + (size_t)ks * wstep + kk * 1024);
-        };
-        auto mma = [&](int p, const uint4v (&vw)[2][FW]) __attribute__((always_inline)) {
-            const char* const st = st0 + p * Shape::XB;
-            uint4v vx[2][FX];
-#pragma unroll
-            for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-                for (int x = 0; x < FX; ++x)
-                    vx[kk][x] = *(const uint4v*)(st + (x * 16 + l15) * 128 + (((kk * 4 + g0) ^ (lane & 7)) << 4));
-            __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_waitcnt(0xC07F);             // lgkmcnt(0): the stage has been read and may be refilled
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-                for (int x = 0; x < FX; ++x)
-#pragma unroll
-                    for (int y = 0; y < FW; ++y) acc[y][x] = mfma<BF>(vw[kk][y], vx[kk][x], acc[y][x]);
-            __builtin_amdgcn_sched_barrier(0);
-        };
+                for (int kk = 0; kk < 2; ++kk) bw[0][kk][y] = *(const uint4v*)(wp[y] + (size_t)ks * wstep + kk * 1024);
+#pragma unroll 1
+            for (int x = 0; x < 2 * FX; ++x)
+                *(uint4v*)(st0 + x * 1024 + lane * 16) = load_chunk((const uint16_t*)row_at(8 * x + (lane >> 3)), ks * 64 + c * 8, a.K);
+            fence();
+            mma(0, bw[0]);
+        }
+    } else {
+        const int n = slices;
 #pragma unroll
         for (int p = 0; p < ST - 1; ++p)
             if (p < n) issue(p, p, bw[p]);
-        int i = 0;
-        for (; i + 2 * ST - 1 <= n; i += ST) {              // nothing in here branches: the compiler can count what is in flight
+        for (; i + 2 * ST - 1 <= n; i += ST) {          // nothing in here branches: the compiler can count what is in flight
 #pragma unroll
             for (int p = 0; p < ST; ++p) {
                 issue(i + p + ST - 1, (p + ST - 1) % ST, bw[(p + ST - 1) % ST]);
@@ -585,8 +610,8 @@ __global__ __launch_bounds__(64 * NW) void linear_wave_kernel(LinearIn a, Linear
                 mma(q % ST, bw[q % ST]);
             }
         }
-        __syncthreads();                                    // the sums take the stages' place
     }
+    __syncthreads();                                    // the sums take the stages' place
 
     float* const part = (float*)smem;
     float* const mine = part + wave * TM * ER;
@@ -648,31 +673,40 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearIn a, LinearOut 
 // shorter than 1e-30 is divided by one.
 // L lanes a row, each R vectors of V consecutive elements (16 bytes, at any address) in registers: x is read once.  R = 0: rows too
 // long for that are read twice, the second time out of the cache.
-// TAIL: V does not divide the row, its last vector is taken element by element.
+// TAIL: V does not divide the row.  Its last vector then begins at N - V and shares elements with the one before it: they count once
+// in the sum and are stored twice, with the same value (1,375,152 rows of 22 fp16: 44 us element by element).  Rows shorter than V
+// go element by element.
 template <typename T, int V, bool TAIL>
-FR_DEV void load_row(const T* p, int n, float (&v)[V]) {
-    if (!TAIL || n >= V) {
-        const auto t = *(const typename vect<T, V>::type*)p;
+FR_DEV void load_row(const T* row, int c, int N, float (&v)[V]) {
+    if (!TAIL || N >= V) {
+        const auto t = *(const typename vect<T, V>::type*)(row + (TAIL ? min(c, N - V) : c));
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] = (float)t[j];
     } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = j < n ? (float)p[j] : 0.f;
+        for (int j = 0; j < V; ++j) v[j] = j < N ? (float)row[j] : 0.f;
     }
+}
+template <int V, bool TAIL>
+FR_DEV void add_squares(double& ss, int c, int N, const float (&v)[V]) {
+    const int shared = TAIL && N >= V ? max(0, c + V - N) : 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        if (!TAIL || j >= shared) ss += (double)v[j] * (double)v[j];
 }
 template <int V, bool TAIL>
 FR_DEV void store_unit(const UnitOut& o, int N, int m, int c, const float (&v)[V], float nrm) {
     half_t* d;
-    if (o.gallery) {
+    if (o.gallery) {                        // (N is a multiple of 64 here)
         const int64_t r = o.row0 + m;       // (the order of a gallery's rows in memory: see gal_index)
         d = (half_t*)o.out + ((((size_t)(r >> 8) * (N >> 6) + (c >> 6)) << 8) + (r & 255)) * 64 + (c & 63);
     } else {
-        d = (half_t*)o.out + (size_t)m * o.ldo + c;
+        d = (half_t*)o.out + (size_t)m * o.ldo + (TAIL && N >= V ? min(c, N - V) : c);
     }
     half_t t[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) t[j] = (half_t)__fdiv_rn(v[j], nrm);
-    if (!TAIL || c + V <= N) {
+    if (!TAIL || N >= V) {
         typename vect<half_t, V>::type u;
 #pragma unroll
         for (int j = 0; j < V; ++j) u[j] = t[j];
@@ -680,7 +714,7 @@ FR_DEV void store_unit(const UnitOut& o, int N, int m, int c, const float (&v)[V
     } else {
 #pragma unroll
         for (int j = 0; j < V; ++j)
-            if (c + j < N) d[j] = t[j];
+            if (j < N) d[j] = t[j];
     }
 }
 template <typename T, int L, int R, bool TAIL>
@@ -695,19 +729,17 @@ __global__ __launch_bounds__(256) void unit_rows_kernel(const T* __restrict__ x,
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const int c = (i * L + l) * V;
-            if (c < N) load_row<T, V, TAIL>(row + c, N - c, v[i]);
+            if (c < N) load_row<T, V, TAIL>(row, c, N, v[i]);
         }
 #pragma unroll
-        for (int i = 0; i < R; ++i)
-            if ((i * L + l) * V < N) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) ss += (double)v[i][j] * (double)v[i][j];
-            }
+        for (int i = 0; i < R; ++i) {
+            const int c = (i * L + l) * V;
+            if (c < N) add_squares<V, TAIL>(ss, c, N, v[i]);
+        }
     } else {
         for (int c = l * V; c < N; c += L * V) {
-            load_row<T, V, TAIL>(row + c, N - c, v[0]);
-#pragma unroll
-            for (int j = 0; j < V; ++j) ss += (double)v[0][j] * (double)v[0][j];
+            load_row<T, V, TAIL>(row, c, N, v[0]);
+            add_squares<V, TAIL>(ss, c, N, v[0]);
         }
     }
 #pragma unroll
@@ -722,7 +754,7 @@ __global__ __launch_bounds__(256) void unit_rows_kernel(const T* __restrict__ x,
         }
     } else {
         for (int c = l * V; c < N; c += L * V) {
-            load_row<T, V, TAIL>(row + c, N - c, v[0]);
+            load_row<T, V, TAIL>(row, c, N, v[0]);
             store_unit<V, TAIL>(o, N, m, c, v[0], nrm);
         }
     }
@@ -774,32 +806,21 @@ hipError_t launch_tile(LinearIn a, const LinearOut& o, int splits, bool gather, 
     return hipGetLastError();
 }
 
-template <bool BF, int FX, int FW, int NW, int ST, bool HAS_GATHER>
+template <bool BF, int FX, int FW, int NW, int ST>
 hipError_t launch_wave(LinearIn a, const LinearOut& o, int splits, bool gather, hipStream_t s, bool attr) {
     using Shape = WaveShape<FX, FW, NW, ST>;
-    if (gather && !HAS_GATHER) return hipErrorInvalidValue;
     const auto whole = linear_wave_kernel<BF, FX, FW, NW, ST, false>;
+    const auto pieces = linear_wave_kernel<BF, FX, FW, NW, ST, true>;
     if (attr) {
-        if constexpr (HAS_GATHER) {
-            const hipError_t e = hipFuncSetAttribute((const void*)linear_wave_kernel<BF, FX, FW, NW, ST, true>,
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, Shape::PART);
-            if (e != hipSuccess) return e;
-        }
-        return hipFuncSetAttribute((const void*)whole, hipFuncAttributeMaxDynamicSharedMemorySize, Shape::LDS);
+        const hipError_t e = hipFuncSetAttribute((const void*)whole, hipFuncAttributeMaxDynamicSharedMemorySize, Shape::LDS);
+        return e != hipSuccess ? e : hipFuncSetAttribute((const void*)pieces, hipFuncAttributeMaxDynamicSharedMemorySize, Shape::LDS);
     }
     a.mtiles = (a.M + Shape::TM - 1) / Shape::TM;
     a.ntiles = (a.npad + Shape::TN - 1) / Shape::TN;
     a.m_fast = a.mtiles < a.ntiles;
     a.splits = splits;
     a.ksteps_per_split = (a.ksteps + splits - 1) / splits;
-    const dim3 grid((unsigned)(a.mtiles * a.ntiles * splits));
-    if constexpr (HAS_GATHER) {
-        if (gather) {
-            hipLaunchKernelGGL((linear_wave_kernel<BF, FX, FW, NW, ST, true>), grid, dim3(64 * NW), Shape::PART, s, a, o);
-            return hipGetLastError();
-        }
-    }
-    hipLaunchKernelGGL(whole, grid, dim3(64 * NW), Shape::LDS, s, a, o);
+    hipLaunchKernelGGL(gather ? pieces : whole, dim3((unsigned)(a.mtiles * a.ntiles * splits)), dim3(64 * NW), Shape::LDS, s, a, o);
     return hipGetLastError();
 }
 
@@ -808,25 +829,25 @@ hipError_t launch_wave(LinearIn a, const LinearOut& o, int splits, bool gather, 
 // (7 to 15 % rms).  The wave kernel's small tiles have a batch done in one round; the tile kernel's 128-row tiles run two to a CU,
 // which hides their beginnings and ends (short K: 6533 x 1504 x 128 12.9 us, 28 with the wave kernel); per value the 256-row tiles are
 // the cheapest.
-struct Shape { int tm, tn; float first, first_step, more, more_step; bool pieces; };   // pieces: takes rows that LDS-DMA cannot
+struct Shape { int tm, tn; float first, first_step, more, more_step, slow; };   // slow: a step of rows that LDS-DMA cannot take, against this
 constexpr Shape kShapes[] = {
-    {16, 32, 4.0f, 0.040f, 2.45f, 0.059f, false},       // wave kernel, 16 waves:  256 x 512 x 4096    8.1 us
-    {32, 32, 3.6f, 0.070f, 0.82f, 0.081f, false},       // wave kernel,  8 waves:  64 x 4096 x 4096    9.8 us
-    {64, 64, 4.8f, 0.165f, 3.05f, 0.22f, false},         // wave kernel,  8 waves:  256 x 4096 x 4096  17 us
-    {64, 128, 6.0f, 0.26f, 4.8f, 0.31f, false},         // wave kernel,  4 waves:  2011 x 1024 x 4096 24 us (128 x 64, more through LDS: 27)
-    {128, 32, 3.2f, 0.33f, 0.63f, 0.57f, true},         // tile kernel, two a CU:  115728 x 32 x 2496 106 us (32 x 32 wave tiles: 121)
-    {128, 64, 3.9f, 0.36f, 1.3f, 0.27f, true},          // tile kernel, two a CU:  13373 x 224 x 1024 14 us (256 x 128: 18)
-    {256, 128, 6.7f, 0.76f, 4.9f, 0.97f, true},         // tile kernel:            16384 x 512 x 4096 70 us
-    {256, 256, 10.6f, 1.23f, 8.6f, 1.57f, true},        // tile kernel:            65536 x 512 x 4096 242 us
+    {16, 32, 4.0f, 0.040f, 2.45f, 0.059f, 1.2f},       // wave kernel, 16 waves:  256 x 512 x 4096    8.1 us
+    {32, 32, 3.6f, 0.070f, 0.82f, 0.081f, 1.3f},       // wave kernel,  8 waves:  64 x 4096 x 4096    9.8 us
+    {64, 64, 4.8f, 0.165f, 3.05f, 0.22f, 1.3f},         // wave kernel,  8 waves:  256 x 4096 x 4096  17 us
+    {64, 128, 6.0f, 0.26f, 4.8f, 0.31f, 1.3f},         // wave kernel,  4 waves:  2011 x 1024 x 4096 24 us (128 x 64, more through LDS: 27)
+    {128, 32, 3.2f, 0.33f, 0.63f, 0.57f, 1.7f},         // tile kernel, two a CU:  115728 x 32 x 2496 106 us (32 x 32 wave tiles: 121)
+    {128, 64, 3.9f, 0.36f, 1.3f, 0.27f, 1.7f},          // tile kernel, two a CU:  13373 x 224 x 1024 14 us (256 x 128: 18)
+    {256, 128, 6.7f, 0.76f, 4.9f, 0.97f, 1.7f},         // tile kernel:            16384 x 512 x 4096 70 us
+    {256, 256, 10.6f, 1.23f, 8.6f, 1.57f, 1.7f},        // tile kernel:            65536 x 512 x 4096 242 us
 };
 constexpr int kNumShapes = sizeof kShapes / sizeof kShapes[0];
 template <bool BF>
 hipError_t launch_shape(int t, const LinearIn& a, const LinearOut& o, int splits, bool gather, hipStream_t s, bool attr) {
     switch (t) {
-        case 0: return launch_wave<BF, 1, 2, 16, 3, true>(a, o, splits, gather, s, attr);
-        case 1: return launch_wave<BF, 2, 2, 8, 2, false>(a, o, splits, gather, s, attr);
-        case 2: return launch_wave<BF, 4, 4, 8, 2, false>(a, o, splits, gather, s, attr);
-        case 3: return launch_wave<BF, 4, 8, 4, 2, false>(a, o, splits, gather, s, attr);
+        case 0: return launch_wave<BF, 1, 2, 16, 3>(a, o, splits, gather, s, attr);
+        case 1: return launch_wave<BF, 2, 2, 8, 2>(a, o, splits, gather, s, attr);
+        case 2: return launch_wave<BF, 4, 4, 8, 2>(a, o, splits, gather, s, attr);
+        case 3: return launch_wave<BF, 4, 8, 4, 2>(a, o, splits, gather, s, attr);
         case 4: return launch_tile<BF, 128, 32, 4, 1, 3, 3>(a, o, splits, gather, s, attr);
         case 5: return launch_tile<BF, 128, 64, 2, 2, 3, 3>(a, o, splits, gather, s, attr);
         case 6: return launch_tile<BF, 256, 128, 4, 2, 3, 3>(a, o, splits, gather, s, attr);
@@ -836,10 +857,9 @@ hipError_t launch_shape(int t, const LinearIn& a, const LinearOut& o, int splits
 
 // What a call runs as: the shape, the number of K slices and the way unaligned rows go in, whichever an estimate of the
 // time puts first.  K slices divide the steps and add the join (a launch, and every slice's sums written and read once: 3.5 us +
-// the bytes at 4 TB/s).  Rows that LDS-DMA cannot take
-//   go through registers in the tile kernel, whose steps then take about 1.7 times as long (16384 x 512 x 4095: 106 us, 200 packed),
-//   or, for few tiles, in the smallest wave tiles (77 x 131 x 500: 4.8 us, 7.6 packed),
-//   or, if the workspace holds them, are packed by a pass of their own, 2 us + the bytes at 4.5 TB/s (394 x 512 x 4095: 18 us, 31 without).
+// the bytes at 4 TB/s).  Rows that LDS-DMA cannot take go through registers (16384 x 512 x 4095: 106 us, 200 packed) or, where
+// wide layers read them many times and the workspace holds them, are packed by a pass of their own, 2 us + the bytes at 4.5 TB/s
+// (800 x 4096 x 4095: 47 us, 60 through registers).
 LinearPlan plan_linear(int M, int npad, int ksteps, bool whole, int64_t pack_rows, size_t slab_bytes) {
     LinearPlan best;
     float best_t = 1e30f;
@@ -847,10 +867,10 @@ LinearPlan plan_linear(int M, int npad, int ksteps, bool whole, int64_t pack_row
         if (t < best_t) { best_t = t; best.shape = shape; best.splits = splits; best.gather = gather; }
     };
     const float sums = (float)M * (float)npad * 4e-6f;          // MB of a slice's sums
-    auto shapes = [&](float extra, float slow, bool gather) {
+    auto shapes = [&](float extra, bool gather) {
         for (int i = 0; i < kNumShapes; ++i) {
             const Shape& sh = kShapes[i];
-            if (gather && !sh.pieces) continue;
+            const float slow = gather ? sh.slow : 1.f;
             const int tiles = (M + sh.tm - 1) / sh.tm * ((npad + sh.tn - 1) / sh.tn);       // (at most 2^18 x 2^11)
             const float steps = (float)ksteps * slow;
             consider(extra + sh.first + steps * sh.first_step + (float)((tiles - 1) >> 8) * (sh.more + steps * sh.more_step), i, 1, gather);
@@ -863,15 +883,9 @@ LinearPlan plan_linear(int M, int npad, int ksteps, bool whole, int64_t pack_row
             }
         }
     };
-    if (whole) {
-        shapes(0.f, 1.f, false);
-        return best;
-    }
-    if (M <= pack_rows) shapes(2.f + (float)M * (float)ksteps * 256e-6f / 4.5f, 1.f, false);
-    shapes(0.f, 1.7f, true);
-    const int tiles = (M + 15) / 16 * ((npad + 31) / 32);
-    const float slices = (float)((ksteps + 15) / 16);           // of a wave
-    consider(2.8f + 1.25f * slices + (float)((tiles - 1) >> 8) * (2.6f + 1.9f * slices), 0, 1, true);
+    if (whole) shapes(0.f, false);
+    else shapes(0.f, true);
+    if (!whole && M <= pack_rows) shapes(2.f + (float)M * (float)ksteps * 256e-6f / 4.5f, false);
     return best;
 }
 

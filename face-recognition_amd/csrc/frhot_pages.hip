@@ -43,7 +43,7 @@ FR_DEV void store16(void* p, uint4v v) {
     else *(uint4v*)p = v;
 }
 
-// One item (a run of up to 64 rows) and `per` chunks of it per block; the pieces are taken chunk by chunk, rows fastest, a
+// One item (a run of up to 256 rows) and `per` chunks of it per block; the pieces are taken chunk by chunk, rows fastest, a
 // power of two of row slots per chunk so that no index needs a division.
 template <bool SD, bool DD, bool NT>
 FR_DEV void move_item(const PageSide& src, const PageSide& dst, const PageItem& it, int nk, int per) {

@@ -642,3 +642,30 @@ def test_read_refuses_keys_off_their_alignment(ctx):
     with pytest.raises(FrhotError):
         p.gal.read_dev([0], [4], buf.data_ptr(), k.data_ptr() + 2)
     p.gal.close()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 192])
+def test_many_rows_of_few_components_in_odd_runs(ctx, dim):
+    """Long items: runs of one to 3000 rows, shuffled, between and inside pages; keys kept, then given."""
+    rng = np.random.default_rng(dim)
+    n, cap = 90001, 200000
+    p, q = Pair(ctx, dim, n, n, seed=dim), Pair(ctx, dim, cap)
+    edge = np.unique(np.concatenate([[0, 1, 255, 256, 257, 600, 3600, n], rng.integers(1, n, 150)]))
+    first, counts = edge[:-1], np.diff(edge)
+    order = rng.permutation(len(first))
+    dst = np.zeros(len(first), np.int64)
+    at = 77
+    for i in order:
+        dst[i] = at
+        at += counts[i] + int(rng.integers(0, 300))
+    keys = rng.integers(0, 5, len(first)).astype(np.int32)
+    for k in (None, keys):
+        q.gal.copy(first, dst, counts, k, source=p.gal)
+        for i in range(len(first)):
+            s, d, c = first[i], dst[i], counts[i]
+            q.t[d:d + c] = p.t[s:s + c]
+            q.k[d:d + c] = p.k[s:s + c] if k is None else k[i]
+        q.check()
+        q.check_search()
+    p.gal.close()
+    q.gal.close()
