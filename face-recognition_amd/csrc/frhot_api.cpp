@@ -2636,15 +2636,29 @@ int page_check_runs(const char* what, const int64_t* first, const int32_t* count
     return FRHOT_OK;
 }
 
+// Runs by their first rows, which lie below `limit`: 11 bits at a time where they are many (3,692 shuffled runs: std::sort takes 100 us
+// of a 126 us call).
+void sort_runs(std::vector<std::pair<int64_t, int64_t>>& v, int64_t limit) {
+    if (v.size() < 256) { std::sort(v.begin(), v.end()); return; }
+    std::vector<std::pair<int64_t, int64_t>> w(v.size());
+    for (int shift = 0; (limit - 1) >> shift; shift += 11) {
+        uint32_t at[2049] = {};
+        for (const auto& r : v) ++at[((r.first >> shift) & 2047) + 1];
+        for (int i = 1; i < 2048; ++i) at[i] += at[i - 1];
+        for (const auto& r : v) w[at[(r.first >> shift) & 2047]++] = r;
+        v.swap(w);
+    }
+}
+
 // No row twice among the runs (a row written by two runs would end with either's content).
-int page_check_disjoint(const int64_t* first, const int32_t* counts, int nruns, std::vector<std::pair<int64_t, int64_t>>& sorted) {
+int page_check_disjoint(const int64_t* first, const int32_t* counts, int nruns, int64_t limit, std::vector<std::pair<int64_t, int64_t>>& sorted) {
     sorted.resize((size_t)nruns);
     bool ascending = true;
     for (int i = 0; i < nruns; ++i) {
         sorted[i] = {first[i], first[i] + (counts ? counts[i] : 1)};
         ascending = ascending && (i == 0 || sorted[i - 1].first <= sorted[i].first);
     }
-    if (!ascending) std::sort(sorted.begin(), sorted.end());
+    if (!ascending) sort_runs(sorted, limit);
     for (int i = 1; i < nruns; ++i)
         if (sorted[i].first < sorted[i - 1].second)
             return fail(FRHOT_EINVAL, "row %lld is a destination twice", (long long)sorted[i].first);
@@ -2768,7 +2782,7 @@ int frhot_gallery_copy(frhot_gallery* src, const int64_t* src_rows, frhot_galler
     int rc = page_check_runs("source", src_rows, counts, nruns, src->capacity, &total);
     if (!rc) rc = page_check_runs("destination", dst_rows, counts, nruns, dst->capacity, &total);
     std::vector<std::pair<int64_t, int64_t>> to;
-    if (!rc) rc = page_check_disjoint(dst_rows, counts, nruns, to);
+    if (!rc) rc = page_check_disjoint(dst_rows, counts, nruns, dst->capacity, to);
     if (rc) return rc;
     bool inside = true;             // every source row was written once
     for (int i = 0; i < nruns; ++i) inside = inside && src_rows[i] + (counts ? counts[i] : 1) <= src->nrows;
@@ -2826,7 +2840,7 @@ int frhot_gallery_write_dev(frhot_gallery* g, const void* rows_f16_dev, const in
     int64_t total = 0;
     int rc = page_check_runs("destination", rows, counts, nruns, g->capacity, &total);
     std::vector<std::pair<int64_t, int64_t>> to;
-    if (!rc) rc = page_check_disjoint(rows, counts, nruns, to);
+    if (!rc) rc = page_check_disjoint(rows, counts, nruns, g->capacity, to);
     if (rc) return rc;
     DeviceGuard dg(c->device);
     rc = page_move_enqueue(c, PageSide{const_cast<void*>(rows_f16_dev), nullptr, 1}, nullptr, PageSide{g->rows, g->keys, 0}, rows, counts, keys, nruns, g->D);
