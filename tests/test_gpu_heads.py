@@ -602,3 +602,66 @@ def test_more_rows_than_a_launch_has_threads(ctx):
         assert torch.equal(o[lo:lo + (1 << 28)], torch.sign(x[lo:lo + (1 << 28)])), lo
     del x, o
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("ld", [(1 << 30) + 8, (1 << 30) + 3])
+def test_rows_gigabytes_apart(ctx, ld):
+    """Row offsets past 2^32 bytes, on both sides, for rows that LDS-DMA takes and rows that it cannot."""
+    m, n, k = 4, 40, 136
+    x, w, b, r = make(m, n, k, "f16", 5, residual="f16")
+    lin = linear_of(ctx, w, b, "f16")
+    big = torch.zeros(3 * ld + 256, dtype=torch.float16, device="cuda")
+    out = torch.zeros(3 * ld + 256, dtype=torch.float16, device="cuda")
+    for i in range(m):
+        big[i * ld:i * ld + k] = x[i].cuda()
+        out[i * ld:i * ld + n] = r[i].cuda()            # (the residual, replaced by the result)
+        out[i * ld + n] = 7.0
+    torch.cuda.synchronize()
+    lin.run_dev(big.data_ptr(), m, out.data_ptr(), act="gelu", residual_dev=out.data_ptr(), ldx=ld, ldr=ld, ldo=ld)
+    ctx.sync()
+    y, tol = layer64(x, w, b, "gelu", r)
+    tol = tol + rounding(y.abs() + tol, "f16")
+    got = torch.stack([out[i * ld:i * ld + n] for i in range(m)]).cpu().double()
+    assert ((got - y).abs() <= tol).all()
+    assert all(out[i * ld + n] == 7 for i in range(m))
+    torch.cuda.synchronize()
+    ctx.unit_rows_dev(big.data_ptr(), m, k, out.data_ptr(), dtype="f16", ldx=ld, ldo=ld)
+    ctx.sync()
+    check_unit(torch.stack([out[i * ld:i * ld + k] for i in range(m)]).cpu(), x)
+    lin.close()
+    del big, out
+    torch.cuda.empty_cache()
+
+
+def test_a_layer_twice_in_a_head_and_in_a_graph(ctx):
+    """One layer used twice by a head; the head replayed from a graph where its products are split over K."""
+    from frhot.engine import Context, Head
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        c2 = Context(device=0, max_batch=1, stream=s.cuda_stream)
+        _, w, b, _ = make(1, 640, 640, "f16", 12)
+        _, w2, b2, _ = make(1, 64, 640, "f16", 13)
+        l1, l2 = linear_of(c2, w, b, "f16"), linear_of(c2, w2, b2, "f16")
+        head = Head(c2, [(l1, "silu", True), (l1, "none", True), (l2, "none", False)])
+        layers = [(w, b, "silu", True), (w, b, "none", True), (w2, b2, "none", False)]
+        m = 260
+        x = torch.randn(m, 643, generator=torch.Generator().manual_seed(2)).half()      # (odd row distance)
+        xd, o = x.cuda(), torch.zeros(m, 64, dtype=torch.float16, device="cuda")
+        e = torch.zeros_like(o)
+        head.run_dev(xd.data_ptr(), m, e.data_ptr(), ldx=643)
+        s.synchronize()
+        want, tol = head64(x[:, :640], layers)
+        assert ((e.cpu().double() - want).abs() <= tol).all()
+        g = torch.cuda.CUDAGraph()
+        g.capture_begin()
+        head.run_dev(xd.data_ptr(), m, o.data_ptr(), ldx=643)
+        g.capture_end()
+        for i in range(4):
+            xd.copy_((x * (1 + i)).cuda())
+            head.run_dev(xd.data_ptr(), m, e.data_ptr(), ldx=643)
+            o.zero_()
+            g.replay()
+            s.synchronize()
+            assert torch.equal(o, e)
+        head.close()
+        l1.close(), l2.close(), c2.close()
