@@ -464,7 +464,7 @@ __global__ __launch_bounds__(64 * WX * WY) void linear_tile_kernel(LinearIn a, L
 // LDS by LDS-DMA, eight rows of 128 bytes an instruction: in fragment order consecutive lanes read different rows, which the
 // load path serves 16 bytes a clock (38 GB/s per CU measured, against 110-145 for whole lines).
 // What bounds it is the CU's load path: 256 x 4096 x 4096 moves 1 MiB into every CU in 14 us, 74 GB/s; one row of 4096 to 512 channels
-// takes 5.2 us on 16 CUs, of which 3.4 are the launch.  Deeper rings for the weights changed neither.
+// takes 6.1 us on 16 CUs, an empty launch 3.9.  Deeper rings for the weights changed neither.
 // GATHER: rows that LDS-DMA cannot take (not 16-byte aligned, K not a multiple of 8) go through registers into the stage, whole lines
 // of a row by consecutive lanes as well (41 x 429 x 3647: 7.6 us, 16 in fragment order straight into registers).
 template <int FX, int FW, int NW, int ST>
