@@ -359,28 +359,37 @@ class Head:
         return out
 
 
+_I32, _I64 = np.dtype(np.int32), np.dtype(np.int64)
+
+
 def _list(a, dtype):
-    if type(a) is np.ndarray and a.dtype == dtype and a.ndim == 1 and a.flags.c_contiguous:
+    if type(a) is np.ndarray and a.dtype is dtype and a.ndim == 1 and a.flags.c_contiguous:
         return a
     return np.ascontiguousarray(a, dtype=dtype).reshape(-1)
 
 
 def _runs(rows, counts, keys=None):
     """Run lists as the ABI takes them; keys: one for all, one per run, or None."""
-    rows = _list(rows, np.int64)
+    rows = _list(rows, _I64)
     if counts is not None:
-        counts = _list(counts, np.int32)
+        counts = _list(counts, _I32)
         if counts.size != rows.size:
             raise ValueError(f"{counts.size} run lengths for {rows.size} runs")
     if keys is not None:
-        keys = _list(keys, np.int32)
+        keys = _list(keys, _I32)
         if keys.size != rows.size:
             keys = np.ascontiguousarray(np.broadcast_to(keys, rows.shape))
     return rows, counts, keys
 
 
 def _at(a):
-    return None if a is None else a.ctypes.data
+    """An array's address for a c_void_p argument; a.ctypes.data takes several times as long."""
+    if a is None:
+        return None
+    try:
+        return C.byref(C.c_char.from_buffer(a))
+    except (TypeError, ValueError, BufferError):        # read-only or empty
+        return a.ctypes.data
 
 
 def runs_of(rows):
@@ -511,23 +520,23 @@ class Gallery:
         if dst_rows.size != src_rows.size:
             raise ValueError(f"{src_rows.size} source runs, {dst_rows.size} destinations")
         src = self if source is None else source
-        check(self._lib.frhot_gallery_copy(src._h, src_rows.ctypes.data, self._h, dst_rows.ctypes.data, _at(counts), _at(keys), src_rows.size))
+        check(self._lib.frhot_gallery_copy(src._h, _at(src_rows), self._h, _at(dst_rows), _at(counts), _at(keys), src_rows.size))
 
     def read_dev(self, rows, counts, out_f16_dev: int, out_keys_dev: int | None = None):
         """The runs back to back as dense fp16 rows [n, D] and int32 keys, in device memory.  Enqueues only."""
         rows, counts, _ = _runs(rows, counts)
-        check(self._lib.frhot_gallery_read_dev(self._h, rows.ctypes.data, _at(counts), rows.size, out_f16_dev, out_keys_dev))
+        check(self._lib.frhot_gallery_read_dev(self._h, _at(rows), _at(counts), rows.size, out_f16_dev, out_keys_dev))
 
     def write_dev(self, rows_f16_dev: int, rows, counts, keys):
         """Dense unit fp16 rows (device) to the runs, one key per run.  Enqueues only."""
         rows, counts, keys = _runs(rows, counts, keys)
-        check(self._lib.frhot_gallery_write_dev(self._h, rows_f16_dev, rows.ctypes.data, _at(counts), keys.ctypes.data, rows.size))
+        check(self._lib.frhot_gallery_write_dev(self._h, rows_f16_dev, _at(rows), _at(counts), _at(keys), rows.size))
 
     def free_keys(self, keys) -> int:
         """Every row under one of the keys dies; returns how many did."""
-        keys = np.ascontiguousarray(keys, dtype=np.int32).reshape(-1)
+        keys = _list(keys, _I32)
         freed = C.c_int64()
-        check(self._lib.frhot_gallery_free_keys(self._h, keys.ctypes.data, keys.size, C.byref(freed)))
+        check(self._lib.frhot_gallery_free_keys(self._h, _at(keys), keys.size, C.byref(freed)))
         return freed.value
 
     def compact(self, into: "Gallery | None" = None, new_rows_dev: int | None = None) -> int:

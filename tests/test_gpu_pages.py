@@ -669,3 +669,23 @@ def test_many_rows_of_few_components_in_odd_runs(ctx, dim):
         q.check_search()
     p.gal.close()
     q.gal.close()
+
+
+def test_lists_of_any_kind(ctx):
+    """Row lists as lists, ranges, other integer types, strided, read-only: the same rows move."""
+    p = Pair(ctx, 64, 600, 300, seed=4)
+    first = np.array([0, 9, 100], np.int64)
+    ro = first.copy()
+    ro.setflags(write=False)
+    at = 300
+    for rows in (first, first.tolist(), first.astype(np.int32), first.astype(np.uint16), np.repeat(first, 2)[::2], ro, first.astype(">i8")):
+        p.gal.copy(rows, [at, at + 10, at + 20], [5, 1, 7], 2)
+        for s, d, c in zip(first, (at, at + 10, at + 20), (5, 1, 7)):
+            p.t[d:d + c], p.k[d:d + c] = p.t[s:s + c], 2
+        at += 30
+    p.check()
+    n = int((p.k == 2).sum())
+    assert p.gal.free_keys(ro[:0].tolist() + [2]) == n and p.gal.free_keys(np.array([2], ">i4")) == 0
+    p.k[p.k == 2] = DEAD
+    p.check()
+    p.gal.close()
