@@ -195,8 +195,9 @@ struct frhot_linear {
     frhot_ctx* ctx = nullptr;
     int N = 0, K = 0, dtype = 0;
     void* wt = nullptr;
+    void* wt2 = nullptr;        // the same twice in a row, from the first head on that has the layer behind another one
     float* bias = nullptr;
-    LinearPlan plan;
+    LinearPlan plan, plan2;     // of calls over wt and over wt2
     int heads = 0;              // heads that hold this layer
 };
 
@@ -207,7 +208,10 @@ struct frhot_head {
     int din = 0, dout = 0;
     int64_t rows = 0;           // rows one pass of the layers takes (longer inputs go through in runs of this many)
     void* in16 = nullptr;       // fp16 [rows, din]: gallery rows brought out for a residual of the first layer
-    void* mid[2] = {};          // fp16 [rows, widest inner layer], in turn
+    int64_t ldm = 0;            // row distance of `mid`: the widest inner layer, to whole steps
+    float* mid[2] = {};         // fp32 [rows, ldm]: the inner layers' outputs, in turn
+    void* pair = nullptr;       // fp16 [rows, 2 ldm]: one of them as the next layer's product takes it,
+    float* scale = nullptr;     // and its rows' scales
     float* y = nullptr;         // fp32 [rows, dout]: the last layer's output, in front of its norm
     void* desc = nullptr;       // fp16 [max_batch, 4096]: descriptors of an embed call, while the head is attached
 };
@@ -296,8 +300,8 @@ int upload(void** dst, const void* src, size_t n) {
 constexpr int kSplitMin = 32;   // batches from this size on run their conv stack as two halves on two streams
 
 // The layers of a head over M fp16 rows of din values (`x`: rows ldx apart, or, `tiled`, the start of a tile of a gallery of
-// dimension din), the last layer's rows brought to unit length into `o` (its row0 counts on with the runs).  Inner layers
-// round to fp16 between layers, as every activation of the library does; the last one stays fp32 up to the norm.
+// dimension din), the last layer's rows brought to unit length into `o` (its row0 counts on with the runs).  Every layer's output
+// stays fp32 (an inner one goes into the next product as pairs of fp16 numbers): the one rounding is that of the unit rows.
 int head_enqueue(frhot_head* h, const void* x, int64_t ldx, bool tiled, int64_t M, UnitOut o) {
     frhot_ctx* c = h->ctx;
     hipStream_t s = c->stream;
@@ -316,12 +320,17 @@ int head_enqueue(frhot_head* h, const void* x, int64_t ldx, bool tiled, int64_t 
             LinearCall q{};
             q.x = in; q.ldx = ld; q.tiled = t ? 1 : 0; q.bf16 = 0;
             q.wt = L.lin->wt; q.bias = L.lin->bias; q.M = n; q.N = L.lin->N; q.K = L.lin->K; q.plan = &L.lin->plan;
+            if (l > 0) {
+                HIP_TRY(launch_linear_split((const float*)in, ld, n, q.K, h->pair, h->scale, s));
+                q.x = h->pair; q.ldx = 2 * linear_kpad(q.K); q.pair = 1; q.out.scale = h->scale;
+                q.wt = L.lin->wt2; q.plan = &L.lin->plan2;
+            }
             const bool last = l == nl - 1;
-            q.out.out = last ? (void*)h->y : h->mid[l & 1];
-            q.out.ldo = q.N; q.out.otype = last ? kF32 : kF16; q.out.act = L.act;
-            if (L.residual) { q.out.res = in; q.out.ldr = ld; q.out.rtype = kF16; }
+            q.out.out = last ? h->y : h->mid[l & 1];
+            q.out.ldo = last ? q.N : h->ldm; q.out.otype = kF32; q.out.act = L.act;
+            if (L.residual) { q.out.res = in; q.out.ldr = ld; q.out.rtype = l > 0 ? kF32 : kF16; }
             HIP_TRY(launch_linear(q, c->lin, s));
-            in = q.out.out; ld = q.N; t = false;
+            in = q.out.out; ld = q.out.ldo; t = false;
         }
         UnitOut u = o;
         if (o.gallery) u.row0 = o.row0 + m0;
@@ -2397,7 +2406,7 @@ int refuse_capture(frhot_ctx* c) {
 }
 
 void head_free(frhot_head* h) {
-    void* ptrs[] = {h->in16, h->mid[0], h->mid[1], h->y, h->desc};
+    void* ptrs[] = {h->in16, h->mid[0], h->mid[1], h->pair, h->scale, h->y, h->desc};
     for (void* p : ptrs) if (p) (void)hipFree(p);
     for (auto& L : h->layers) --L.lin->heads;
     delete h;
@@ -2450,6 +2459,7 @@ int frhot_linear_destroy(frhot_linear* l) {
     DeviceGuard dg(l->ctx->device);
     (void)hipStreamSynchronize(l->ctx->stream);
     (void)hipFree(l->wt);
+    if (l->wt2) (void)hipFree(l->wt2);
     (void)hipFree(l->bias);
     delete l;
     return FRHOT_OK;
@@ -2531,13 +2541,27 @@ int frhot_head_create(frhot_ctx* c, frhot_linear* const* layers, const int32_t* 
     // As many rows a pass as fill the GPU with tiles and keep the intermediates inside the 256 MiB Infinity Cache
     // (32,768 rows of a 512-wide fp32 output: 64 MiB).
     const bool bring_out = h->layers[0].residual;
-    const size_t per_row = (size_t)dout * 4 + (size_t)widest * 2 * (n > 2 ? 2 : 1) + (bring_out ? (size_t)din * 2 : 0);
+    const size_t ldm = (size_t)linear_kpad(widest);
+    const size_t per_row = (size_t)dout * 4 + ldm * 4 * (n > 2 ? 2 : 1) + ldm * 4 + (bring_out ? (size_t)din * 2 : 0);
+    h->ldm = (int64_t)ldm;
     int64_t rows = (int64_t)((192u << 20) / per_row) / 256 * 256;
     h->rows = rows < 2048 ? 2048 : (rows > 32768 ? 32768 : rows);
     hipError_t e = hipMalloc((void**)&h->y, (size_t)h->rows * dout * 4);
-    if (e == hipSuccess && n > 1) e = hipMalloc(&h->mid[0], (size_t)h->rows * widest * 2);
-    if (e == hipSuccess && n > 2) e = hipMalloc(&h->mid[1], (size_t)h->rows * widest * 2);
+    if (e == hipSuccess && n > 1) e = hipMalloc((void**)&h->mid[0], (size_t)h->rows * ldm * 4);
+    if (e == hipSuccess && n > 2) e = hipMalloc((void**)&h->mid[1], (size_t)h->rows * ldm * 4);
+    if (e == hipSuccess && n > 1) e = hipMalloc(&h->pair, (size_t)h->rows * ldm * 4);
+    if (e == hipSuccess && n > 1) e = hipMalloc((void**)&h->scale, (size_t)h->rows * 4);
     if (e == hipSuccess && bring_out) e = hipMalloc(&h->in16, (size_t)h->rows * din * 2);
+    for (int i = 1; e == hipSuccess && i < n; ++i) {
+        frhot_linear* const l = layers[i];
+        if (l->wt2) continue;
+        const size_t bytes = linear_layout_bytes(l->N, l->K);
+        e = hipMalloc(&l->wt2, 2 * bytes);
+        for (int j = 0; e == hipSuccess && j < 2; ++j)
+            e = hipMemcpyAsync((char*)l->wt2 + j * bytes, l->wt, bytes, hipMemcpyDeviceToDevice, c->stream);
+        if (e == hipSuccess) e = hipStreamSynchronize(c->stream);
+        if (e != hipSuccess) (void)free_null(l->wt2);
+    }
     if (e != hipSuccess) return fail(FRHOT_EHIP, "head scratch for %lld rows failed: %s", (long long)h->rows, hipGetErrorString(e));
     *out = h.release();
     return FRHOT_OK;

@@ -162,16 +162,18 @@ struct LinearOut {
     void* out; int64_t ldo; int otype;
     const void* res; int64_t ldr; int rtype;        // residual added after the activation, or null
     int act, N;                                     // (N: filled in by launch_linear)
+    const float* scale;                             // the products' sum of row m counts scale[m] times (null: once)
 };
 struct LinearIn {
     const void* x; int64_t ldx; size_t xtile; int tiled, xstep;
     const void* wt; const float* bias; const void* zeros; float* slab;
     int M, K, npad, panels, ksteps, ksteps_per_split, splits, mtiles, ntiles, m_fast;
 };
-struct LinearPlan { int64_t M = 0; int whole = 0, shape = 0, splits = 0, gather = 0; };     // what calls of M rows of a layer run as
+struct LinearPlan { int64_t M = 0; int whole = 0, shape = 0, splits = 0, gather = 0; };     // what calls of M rows of a layer (or of its pairs) run as
 struct LinearCall {
     const void* x; int64_t ldx;     // [M, K] fp16 or bf16 rows ldx elements apart; tiled: rows 0.. of a gallery of dimension K (x = a tile's start)
     int tiled, bf16;
+    int pair;                       // x holds two fp16 numbers for every value (launch_linear_split's result, ldx = 2 linear_kpad(K)), wt its layout twice
     const void* wt; const float* bias;      // launch_linear_layout's result; linear_npad(N) floats
     int64_t M; int N, K;
     LinearOut out;
@@ -182,6 +184,9 @@ struct LinearWork { float* slabs; size_t slab_bytes; void* pack; size_t pack_byt
 size_t linear_layout_bytes(int N, int K);
 hipError_t launch_linear_layout(const void* w, void* wt, int N, int K, hipStream_t s);
 hipError_t launch_linear(const LinearCall& q, const LinearWork& ws, hipStream_t s);
+// fp32 rows -> pairs of fp16 numbers and the rows' scales: x[m][n] = scale[m] (out[m][n] + out[m][linear_kpad(N) + n]), zeros in
+// the padding.  ldx: a multiple of 64, at least linear_kpad(N) (what lies behind the N-th value is read and not used).
+hipError_t launch_linear_split(const float* x, int64_t ldx, int64_t M, int N, void* out, float* scale, hipStream_t s);
 struct UnitOut {
     void* out; int64_t ldo;         // fp16 rows, or
     int gallery; int64_t row0;      // rows row0 .. of a gallery of dimension N whose rows start at `out`
