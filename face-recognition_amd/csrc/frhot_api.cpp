@@ -213,7 +213,8 @@ struct frhot_head {
     void* pair = nullptr;       // fp16 [rows, 2 ldm]: one of them as the next layer's product takes it,
     float* scale = nullptr;     // and its rows' scales
     float* y = nullptr;         // fp32 [rows, dout]: the last layer's output, in front of its norm
-    void* desc = nullptr;       // fp16 [max_batch, 4096]: descriptors of an embed call, while the head is attached
+    void* desc = nullptr;       // fp16 [max_batch, 4096]: descriptors of an embed call, once the head is attached or bound
+    int galleries = 0;          // galleries that are bound to it
 };
 
 struct frhot_gallery {
@@ -246,6 +247,7 @@ struct frhot_gallery {
     bool key_tiles_off = false;
     size_t key_tiles_limit() const { return 8 * (size_t)((capacity + 255) / 256) + 65536; }
     int search_mode = FRHOT_SEARCH_AUTO;
+    frhot_head* head = nullptr;     // what makes this gallery's queries from descriptors (frhot_gallery_head)
     IndexPin idx;                   // of frhot_search (a call holds ctx->mu until its copies are done)
     int32_t* idx_dev = nullptr; size_t idx_dev_cap = 0;
     void* q16s = nullptr; size_t q16s_cap = 0;      // the queries in key order
@@ -340,6 +342,9 @@ int head_enqueue(frhot_head* h, const void* x, int64_t ldx, bool tiled, int64_t 
     return FRHOT_OK;
 }
 
+// The head that is attached to the context, if queries of Dq components are its output.
+frhot_head* attached_head(frhot_ctx* c, int Dq) { return c->head && c->head->dout == Dq ? c->head : nullptr; }
+
 // What embed_enqueue asks before it enqueues the second half of a batch: a host call whose crops
 // are still being packed and uploaded lets the first half start on the GPU meanwhile.
 struct SecondHalfGate {
@@ -351,8 +356,9 @@ constexpr int kShareLayers = 6;     // conv layers 1..6 (conv1_2 .. conv3_3) are
 constexpr int kShareMinBatch = 192, kShareMaxBatch = 320;
 
 // Enqueue the whole embed pipeline for B crops whose pixels sit at crops_dev.
+// `head`: makes out_q from the descriptors (null: their leading Dq components).
 int embed_enqueue(frhot_ctx* c, const void* crops_dev, const int64_t* offsets, const int32_t* hw,
-                  const int32_t* strides, int B, unsigned flags, float* out_f32, void* out_q, int Dq,
+                  const int32_t* strides, int B, unsigned flags, float* out_f32, void* out_q, int Dq, frhot_head* head,
                   SecondHalfGate* gate = nullptr, int first_part = 0, bool parts_start_together = true) {
     if (!c->model) return fail(FRHOT_ESTATE, "frhot_model_load has not been called");
     if (B <= 0 || B > c->max_batch) return fail(FRHOT_ECAPACITY, "batch %d outside 1..%d", B, c->max_batch);
@@ -448,10 +454,10 @@ int embed_enqueue(frhot_ctx* c, const void* crops_dev, const int64_t* offsets, c
     HIP_TRY(launch_fc_splitk(c->act[kNumConv - 1], c->w6, c->partial, B, kFcN, kFc6K, kFc6Split, s));
     HIP_TRY(launch_fc_reduce_relu(c->partial, c->b6, c->fc6_out, B, kFcN, kFc6Split, s));
     HIP_TRY(launch_fc_splitk(c->fc6_out, c->w7, c->partial, B, kFcN, kFcN, kFc7Split, s));
-    if (out_q && c->head && Dq == c->head->dout) {
-        // queries of the attached head's width: the whole descriptor in fp16, then the head
-        HIP_TRY(launch_fc_reduce_relu_l2(c->partial, c->b7, out_f32, c->head->desc, kFcN, B, kFcN, kFc7Split, s));
-        const int rc = head_enqueue(c->head, c->head->desc, kFcN, false, B, UnitOut{out_q, Dq, 0, 0, nullptr, nullptr});
+    if (out_q && head) {
+        // the whole descriptor in fp16, then the head
+        HIP_TRY(launch_fc_reduce_relu_l2(c->partial, c->b7, out_f32, head->desc, kFcN, B, kFcN, kFc7Split, s));
+        const int rc = head_enqueue(head, head->desc, kFcN, false, B, UnitOut{out_q, Dq, 0, 0, nullptr, nullptr});
         if (rc) return rc;
     } else {
         HIP_TRY(launch_fc_reduce_relu_l2(c->partial, c->b7, out_f32, out_q, out_q ? Dq : kFcN, B, kFcN, kFc7Split, s));
@@ -1255,7 +1261,7 @@ int frhot_embed_dev(frhot_ctx* c, const void* crops_dev, const int64_t* offsets,
     if (!out_f32_dev && !out_q_f16_dev) return fail(FRHOT_EINVAL, "no output requested");
     std::lock_guard<std::mutex> lk(c->mu);
     DeviceGuard dg(c->device);
-    return embed_enqueue(c, crops_dev, offsets, hw, strides, B, flags, (float*)out_f32_dev, out_q_f16_dev, Dq);
+    return embed_enqueue(c, crops_dev, offsets, hw, strides, B, flags, (float*)out_f32_dev, out_q_f16_dev, Dq, attached_head(c, Dq));
     });
 }
 
@@ -1274,7 +1280,7 @@ int frhot_embed(frhot_ctx* c, const uint8_t* const* crops, const int32_t* hw, co
     if (rc) return rc;
     rc = run_staged(c, lease.sl, st, [&]() -> int {
         int r = embed_enqueue(c, lease.sl.dev, st.offsets.data(), hw, st.packed_strides.data(), B, flags, c->emb_dev,
-                              nullptr, kFcN, &st, st.split_at, !call.alone);
+                              nullptr, kFcN, nullptr, &st, st.split_at, !call.alone);
         if (r) return r;
         HIP_TRY(hipMemcpyAsync(lease.sl.emb_pin, c->emb_dev, (size_t)B * kFcN * 4, hipMemcpyDeviceToHost, c->stream));
         return FRHOT_OK;
@@ -1380,6 +1386,7 @@ int frhot_gallery_destroy(frhot_gallery* g) {
     std::lock_guard<std::mutex> lk(g->ctx->mu);
     DeviceGuard dg(g->ctx->device);
     (void)hipStreamSynchronize(g->ctx->stream);
+    if (g->head) --g->head->galleries;
     void* ptrs[] = {g->rows, g->keys, g->part_s, g->part_r, g->qbound, g->up_vecs, g->up_keys, g->up_rows,
                     g->q16, g->q32, g->qk, g->out_s, g->out_r, g->mut_rows, g->mut_keys, g->mut_f16, g->idx_dev, g->q16s};
     for (void* p : ptrs) if (p) (void)hipFree(p);
@@ -1860,7 +1867,8 @@ static int recognise_impl(frhot_ctx* c, frhot_gallery* g, const uint8_t* const* 
     int64_t* const pin_r = (int64_t*)(sl.res_pin + (size_t)c->max_batch * 16 * 4);
     rc = run_staged(c, sl, st, [&]() -> int {
         hipStream_t s = c->stream;
-        int r = embed_enqueue(c, sl.dev, offsets.data(), hw, ps.data(), B, flags, c->emb_dev, c->q_dev, g->D, &st, st.split_at, !call.alone);
+        int r = embed_enqueue(c, sl.dev, offsets.data(), hw, ps.data(), B, flags, c->emb_dev, c->q_dev, g->D,
+                              g->head ? g->head : attached_head(c, g->D), &st, st.split_at, !call.alone);
         if (r) return r;
         r = search_keyed_enqueue(g, c->q_dev, qkeys, c->qkeys_dev, B, k, c->res_s, c->res_r, sl.idx);
         if (r) return r;
@@ -2574,6 +2582,7 @@ int frhot_head_destroy(frhot_head* h) {
     frhot_ctx* c = h->ctx;
     std::lock_guard<std::mutex> lk(c->mu);
     DeviceGuard dg(c->device);
+    if (h->galleries) return fail(FRHOT_ESTATE, "%d galler%s bound to the head", h->galleries, h->galleries == 1 ? "y is" : "ies are");
     (void)hipStreamSynchronize(c->stream);
     if (c->head == h) c->head = nullptr;
     head_free(h);
@@ -2625,16 +2634,39 @@ int frhot_head_apply(frhot_head* h, const float* x, int M, float* out) {
     });
 }
 
+// Can the head make queries of the context's descriptors?  Entered with c->mu held, in front of its attachment.
+static int head_takes_descriptors(frhot_ctx* c, frhot_head* h) {
+    if (h->ctx != c) return fail(FRHOT_EINVAL, "head belongs to another context");
+    if (h->din != kFcN) return fail(FRHOT_EINVAL, "a head of %d inputs does not take descriptors of %d", h->din, kFcN);
+    if (h->dout > kFcN) return fail(FRHOT_EINVAL, "a head of %d outputs: queries have at most %d components", h->dout, kFcN);
+    if (!h->desc) HIP_TRY(hipMalloc(&h->desc, (size_t)c->max_batch * kFcN * 2));
+    return FRHOT_OK;
+}
+
 int frhot_ctx_head(frhot_ctx* c, frhot_head* h) {
     return guarded([&]() -> int {
     if (!c) return fail(FRHOT_EINVAL, "ctx is null");
-    if (h && h->ctx != c) return fail(FRHOT_EINVAL, "head belongs to another context");
-    if (h && h->din != kFcN) return fail(FRHOT_EINVAL, "a head of %d inputs does not take descriptors of %d", h->din, kFcN);
-    if (h && h->dout > kFcN) return fail(FRHOT_EINVAL, "a head of %d outputs: queries have at most %d components", h->dout, kFcN);
     std::lock_guard<std::mutex> lk(c->mu);
     DeviceGuard dg(c->device);
-    if (h && !h->desc) HIP_TRY(hipMalloc(&h->desc, (size_t)c->max_batch * kFcN * 2));
+    const int rc = h ? head_takes_descriptors(c, h) : FRHOT_OK;
+    if (rc) return rc;
     c->head = h;
+    return FRHOT_OK;
+    });
+}
+
+int frhot_gallery_head(frhot_gallery* g, frhot_head* h) {
+    return guarded([&]() -> int {
+    if (!g) return fail(FRHOT_EINVAL, "gallery is null");
+    frhot_ctx* c = g->ctx;
+    std::lock_guard<std::mutex> lk(c->mu);
+    DeviceGuard dg(c->device);
+    if (h && h->dout != g->D) return fail(FRHOT_EINVAL, "a head of %d outputs for a gallery of dimension %d", h->dout, g->D);
+    const int rc = h ? head_takes_descriptors(c, h) : FRHOT_OK;
+    if (rc) return rc;
+    if (g->head) --g->head->galleries;
+    if (h) ++h->galleries;
+    g->head = h;
     return FRHOT_OK;
     });
 }

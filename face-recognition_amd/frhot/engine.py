@@ -240,8 +240,9 @@ class Context:
                                             n if ldo is None else ldo))
 
     def set_head(self, head: "Head | None"):
-        """Queries of head.dout components (embed_dev's dq, recognise on a gallery of that dimension) come from
-        `head` instead of the descriptor's leading components; None: as before."""
+        """Queries of head.dout components (embed_dev's dq, recognise on every gallery of that dimension that is
+        not bound to a head of its own, see Gallery.set_head) come from `head` instead of the descriptor's
+        leading components; None: as before."""
         check(self._lib.frhot_ctx_head(self._h, head.handle if head is not None else None))
         self._head = head
 
@@ -408,12 +409,14 @@ class Gallery:
         self.dim = dim
         self.capacity = capacity
         self._h = C.c_void_p()
+        self._head = None
         check(self._lib.frhot_gallery_create(ctx.handle, dim, capacity, C.byref(self._h)))
 
     def close(self):
         if getattr(self, "_h", None) and self._h.value and self.ctx.handle.value:
             self._lib.frhot_gallery_destroy(self._h)
         self._h = C.c_void_p()
+        self._head = None
 
     def __del__(self):
         try:
@@ -436,6 +439,12 @@ class Gallery:
         rows = np.ascontiguousarray(rows, dtype=np.int64).reshape(n)
         check(self._lib.frhot_gallery_upsert(self._h, _ptr(vecs, C.c_float), _ptr(keys, C.c_int32),
                                              _ptr(rows, C.c_int64), n))
+
+    def set_head(self, head: "Head | None"):
+        """Context.recognise on this gallery makes its queries with `head`, whose rows the gallery holds, whatever
+        is attached to the context; None: unbound again.  The gallery keeps the head alive."""
+        check(self._lib.frhot_gallery_head(self._h, head.handle if head is not None else None))
+        self._head = head
 
     SEARCH_AUTO, SEARCH_BY_KEY, SEARCH_WHOLE = 0, 1, 2
 

@@ -92,17 +92,24 @@ class GalleryService:
         frhot.engine.Gallery to use instead of creating one on `ctx` (tests inject a stand-in).
         `head`: a frhot.engine.Head: the gallery holds its rows (dim = head.dout), vectors of
         head.din components are taken through it on their way in and on their way to a search, and
-        it is attached to `ctx`, so that recognise_points does the same."""
+        the gallery is bound to it, so that recognise_points does the same; other services of the
+        context, with other heads or none, are not touched."""
         self.head = head
         if head is not None:
             dim = head.dout
-            if ctx is not None:
-                ctx.set_head(head)
         self.dim = dim
         self.capacity = capacity
-        if gallery is None:
+        made = gallery is None
+        if made:
             from .engine import Gallery
             gallery = Gallery(ctx, dim, capacity)
+        if head is not None and hasattr(gallery, "set_head"):       # (a stand-in has no recognise call to serve)
+            try:
+                gallery.set_head(head)
+            except Exception:
+                if made:
+                    gallery.close()
+                raise
         self.gallery = gallery
         self._lock = threading.RLock()
         self._held = threading.local()             # .depth: how often the calling thread holds _lock through _locked()

@@ -417,10 +417,14 @@ int frhot_ctx_stage_ms(frhot_ctx* ctx, float* ms5);
  * frhot_head_apply: the same for host rows (x [M,din] float32, rounded to fp16; out [M,dout] float32
  *   holding the fp16 rows), for a few descriptors at a time (M up to 2048 at least); waits, and is
  *   FRHOT_ESTATE on a stream under graph capture.
- * frhot_ctx_head: attach (or, NULL, detach) a head of 4096 inputs: frhot_embed_dev with Dq equal to
- *   its outputs and frhot_recognise* on a gallery of that dimension then use the head's rows as
- *   queries, where they take the descriptor's leading components otherwise.  Destroying an attached
- *   head detaches it.
+ * frhot_gallery_head: bind a gallery to the head of 4096 inputs whose rows it holds (or, NULL, unbind it):
+ *   frhot_recognise* on the gallery then make its queries with that head, whatever else the context
+ *   serves.  Several galleries of one context can be bound, to one head or to several.  A head cannot be
+ *   destroyed while a gallery is bound to it (FRHOT_ESTATE); destroying the gallery unbinds it.
+ * frhot_ctx_head: attach (or, NULL, detach) a head of 4096 inputs to the context: frhot_embed_dev with Dq
+ *   equal to its outputs, and frhot_recognise* on EVERY unbound gallery of that dimension, then use the
+ *   head's rows as queries, where they take the descriptor's leading components otherwise.  Destroying
+ *   an attached head detaches it.
  * All *_dev calls enqueue on the context's stream and return.  They share the context's scratch:
  * graphs captured from one context's calls must not be replayed at the same time.
  */
@@ -435,6 +439,7 @@ int frhot_head_destroy(frhot_head* head);
 int frhot_head_dev(frhot_head* head, const void* x_f16_dev, int64_t ldx, int64_t M, void* out_f16_dev, int64_t ldo);
 int frhot_head_apply(frhot_head* head, const float* x, int M, float* out);
 int frhot_ctx_head(frhot_ctx* ctx, frhot_head* head);
+int frhot_gallery_head(frhot_gallery* g, frhot_head* head);
 
 /*
  * Pages of a gallery: copying, forking, squeezing and freeing rows without a trip through host
