@@ -2610,6 +2610,9 @@ int frhot_head_apply(frhot_head* h, const float* x, int M, float* out) {
     return guarded([&]() -> int {
     if (!h || !x || !out) return fail(FRHOT_EINVAL, "null argument");
     if (M <= 0 || M > h->rows) return fail(FRHOT_EINVAL, "%d rows outside 1..%lld", M, (long long)h->rows);
+    for (size_t i = 0; i < (size_t)M * h->din; ++i)
+        if (std::isfinite(x[i]) && std::fabs(x[i]) >= 65520.f)
+            return fail(FRHOT_EINVAL, "component %zu of row %zu is %g: fp16 ends at 65504", i % h->din, i / h->din, (double)x[i]);
     frhot_ctx* c = h->ctx;
     std::lock_guard<std::mutex> lk(c->mu);
     DeviceGuard dg(c->device);

@@ -35,6 +35,13 @@ SEARCH_LIMIT = 5
 TILE = 256      # rows per gallery tile: what one scan step covers and a by-key search skips or reads
 
 
+def _unit(vec):
+    """A float32 vector at unit length; one that has it to float32's accuracy stays as it is, bit for bit, as does one
+    shorter than 1e-30."""
+    n = float(np.sqrt(np.sum(vec.astype(np.float64) ** 2)))
+    return vec if n < 1e-30 or abs(n - 1) <= 2.0 ** -20 else (vec / n).astype(np.float32)
+
+
 class _RowAllocator:
     """Gallery rows handed out so that a key's rows sit together.  The reference keeps every
     collection in storage of its own (qdrant_database_FE/app.py:108-128); here a key (collection,
@@ -91,7 +98,8 @@ class GalleryService:
         """`gallery`: an object with the upsert / tombstone / search / close methods of
         frhot.engine.Gallery to use instead of creating one on `ctx` (tests inject a stand-in).
         `head`: a frhot.engine.Head: the gallery holds its rows (dim = head.dout), vectors of
-        head.din components are taken through it on their way in and on their way to a search, and
+        head.din components are brought to unit length (as descriptors are, and as a gallery without a
+        head does) and taken through it on their way in and on their way to a search, and
         the gallery is bound to it, so that recognise_points does the same; other services of the
         context, with other heads or none, are not touched."""
         self.head = head
@@ -255,12 +263,17 @@ class GalleryService:
         self._rows.release(row)
 
     def _fits(self, vec):
-        return vec is not None and (len(vec) == self.dim or (self.head is not None and len(vec) == self.head.din))
+        if vec is None:
+            return False
+        if self.head is not None and len(vec) == self.head.din:
+            with np.errstate(over="ignore"):
+                return bool(np.isfinite(np.asarray(vec, dtype=np.float32)).all())   # (its row would match nothing)
+        return len(vec) == self.dim
 
     def _as_row(self, vec):
         vec = np.asarray(vec, dtype=np.float32).reshape(-1)
         if self.head is not None and vec.size == self.head.din:
-            vec = self.head.apply(vec)[0]
+            vec = self.head.apply(_unit(vec))[0]
         return vec
 
     def _key(self, collection, store_id) -> int:

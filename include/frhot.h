@@ -415,8 +415,8 @@ int frhot_ctx_stage_ms(frhot_ctx* ctx, float* ms5);
  *   The layers stay the caller's and must outlive the head.
  * frhot_head_dev: fp16 rows x [M,din] -> unit fp16 rows out [M,dout].
  * frhot_head_apply: the same for host rows (x [M,din] float32, rounded to fp16; out [M,dout] float32
- *   holding the fp16 rows), for a few descriptors at a time (M up to 2048 at least); waits, and is
- *   FRHOT_ESTATE on a stream under graph capture.
+ *   holding the fp16 rows), for a few descriptors at a time (M up to 2048 at least); a finite component
+ *   that fp16 does not hold is FRHOT_EINVAL.  Waits, and is FRHOT_ESTATE on a stream under graph capture.
  * frhot_gallery_head: bind a gallery to the head of 4096 inputs whose rows it holds (or, NULL, unbind it):
  *   frhot_recognise* on the gallery then make its queries with that head, whatever else the context
  *   serves.  Several galleries of one context can be bound, to one head or to several.  A head cannot be
