@@ -215,7 +215,11 @@ struct frhot_head {
     float* y = nullptr;         // fp32 [rows, dout]: the last layer's output, in front of its norm
     void* desc = nullptr;       // fp16 [max_batch, 4096]: descriptors of an embed call, once the head is attached or bound
     int galleries = 0;          // galleries that are bound to it
+    // staging of host rows, device and page-locked, kept up to kHeadStage bytes so that a vector in a request allocates nothing
+    void *io_dev = nullptr, *io_pin = nullptr;
+    size_t io_cap = 0;
 };
+constexpr size_t kHeadStage = 8u << 20;
 
 struct frhot_gallery {
     frhot_ctx* ctx = nullptr;
@@ -304,6 +308,7 @@ constexpr int kSplitMin = 32;   // batches from this size on run their conv stac
 // The layers of a head over M fp16 rows of din values (`x`: rows ldx apart, or, `tiled`, the start of a tile of a gallery of
 // dimension din), the last layer's rows brought to unit length into `o` (its row0 counts on with the runs).  Every layer's output
 // stays fp32 (an inner one goes into the next product as pairs of fp16 numbers): the one rounding is that of the unit rows.
+// o.out null: up to h->rows rows, which stay in h->y.
 int head_enqueue(frhot_head* h, const void* x, int64_t ldx, bool tiled, int64_t M, UnitOut o) {
     frhot_ctx* c = h->ctx;
     hipStream_t s = c->stream;
@@ -334,6 +339,7 @@ int head_enqueue(frhot_head* h, const void* x, int64_t ldx, bool tiled, int64_t 
             HIP_TRY(launch_linear(q, c->lin, s));
             in = q.out.out; ld = q.out.ldo; t = false;
         }
+        if (!o.out) continue;
         UnitOut u = o;
         if (o.gallery) u.row0 = o.row0 + m0;
         else u.out = (char*)o.out + (size_t)m0 * o.ldo * 2;
@@ -2414,8 +2420,9 @@ int refuse_capture(frhot_ctx* c) {
 }
 
 void head_free(frhot_head* h) {
-    void* ptrs[] = {h->in16, h->mid[0], h->mid[1], h->pair, h->scale, h->y, h->desc};
+    void* ptrs[] = {h->in16, h->mid[0], h->mid[1], h->pair, h->scale, h->y, h->desc, h->io_dev};
     for (void* p : ptrs) if (p) (void)hipFree(p);
+    if (h->io_pin) (void)hipHostFree(h->io_pin);
     for (auto& L : h->layers) --L.lin->heads;
     delete h;
 }
@@ -2606,11 +2613,12 @@ int frhot_head_dev(frhot_head* h, const void* x_f16_dev, int64_t ldx, int64_t M,
     });
 }
 
-int frhot_head_apply(frhot_head* h, const float* x, int M, float* out) {
-    return guarded([&]() -> int {
+// Host rows through a head and back: unit fp16 rows (as floats), or, `raw`, the last layer's rows in front of their norm.
+static int head_host(frhot_head* h, const float* x, int M, float* out, bool raw) {
     if (!h || !x || !out) return fail(FRHOT_EINVAL, "null argument");
     if (M <= 0 || M > h->rows) return fail(FRHOT_EINVAL, "%d rows outside 1..%lld", M, (long long)h->rows);
-    for (size_t i = 0; i < (size_t)M * h->din; ++i)
+    const size_t nx = (size_t)M * h->din, no = (size_t)M * h->dout, xb = (nx * 2 + 255) & ~(size_t)255, ob = no * (raw ? 4 : 2);
+    for (size_t i = 0; i < nx; ++i)
         if (std::isfinite(x[i]) && std::fabs(x[i]) >= 65520.f)
             return fail(FRHOT_EINVAL, "component %zu of row %zu is %g: fp16 ends at 65504", i % h->din, i / h->din, (double)x[i]);
     frhot_ctx* c = h->ctx;
@@ -2618,23 +2626,44 @@ int frhot_head_apply(frhot_head* h, const float* x, int M, float* out) {
     DeviceGuard dg(c->device);
     const int held = refuse_capture(c);
     if (held) return held;
-    const size_t nx = (size_t)M * h->din, no = (size_t)M * h->dout;
-    std::vector<_Float16> x16(nx), o16(no);
-    for (size_t i = 0; i < nx; ++i) x16[i] = (_Float16)x[i];
-    void* dev = nullptr;
-    HIP_TRY(hipMalloc(&dev, (nx + no) * 2));
-    hipError_t e = hipMemcpyAsync(dev, x16.data(), nx * 2, hipMemcpyHostToDevice, c->stream);
+    hipStream_t s = c->stream;
+    if (xb + ob > h->io_cap) {
+        h->io_cap = 0;
+        HIP_TRY(free_null(h->io_dev));                      // (every call waits: nothing reads it any more)
+        if (h->io_pin) { void* old = h->io_pin; h->io_pin = nullptr; HIP_TRY(hipHostFree(old)); }
+        HIP_TRY(hipMalloc(&h->io_dev, xb + ob));
+        HIP_TRY(hipHostMalloc(&h->io_pin, xb + ob, hipHostMallocDefault));
+        h->io_cap = xb + ob;
+    }
+    char *const dev = (char*)h->io_dev, *const pin = (char*)h->io_pin;
+    for (size_t i = 0; i < nx; ++i) ((_Float16*)pin)[i] = (_Float16)x[i];
+    hipError_t e = hipMemcpyAsync(dev, pin, nx * 2, hipMemcpyHostToDevice, s);
     int rc = FRHOT_OK;
-    if (e == hipSuccess) rc = head_enqueue(h, dev, h->din, false, M, UnitOut{(char*)dev + nx * 2, h->dout, 0, 0, nullptr, nullptr});
-    if (e == hipSuccess && rc == FRHOT_OK) e = hipMemcpyAsync(o16.data(), (char*)dev + nx * 2, no * 2, hipMemcpyDeviceToHost, c->stream);
-    const hipError_t es = hipStreamSynchronize(c->stream);
+    if (e == hipSuccess) rc = head_enqueue(h, dev, h->din, false, M, UnitOut{raw ? nullptr : dev + xb, h->dout, 0, 0, nullptr, nullptr});
+    if (e == hipSuccess && rc == FRHOT_OK) e = hipMemcpyAsync(pin + xb, raw ? (void*)h->y : dev + xb, ob, hipMemcpyDeviceToHost, s);
+    const hipError_t es = hipStreamSynchronize(s);
     if (e == hipSuccess) e = es;
-    (void)hipFree(dev);
+    if (rc == FRHOT_OK && e == hipSuccess) {
+        if (raw) memcpy(out, pin + xb, ob);
+        else for (size_t i = 0; i < no; ++i) out[i] = (float)((const _Float16*)(pin + xb))[i];
+    }
+    if (h->io_cap > kHeadStage) {
+        h->io_cap = 0;
+        (void)free_null(h->io_dev);
+        (void)hipHostFree(h->io_pin);
+        h->io_pin = nullptr;
+    }
     if (rc) return rc;
     if (e != hipSuccess) return fail(FRHOT_EHIP, "head pass failed: %s", hipGetErrorString(e));
-    for (size_t i = 0; i < no; ++i) out[i] = (float)o16[i];
     return FRHOT_OK;
-    });
+}
+
+int frhot_head_apply(frhot_head* h, const float* x, int M, float* out) {
+    return guarded([&]() -> int { return head_host(h, x, M, out, false); });
+}
+
+int frhot_head_project(frhot_head* h, const float* x, int M, float* out) {
+    return guarded([&]() -> int { return head_host(h, x, M, out, true); });
 }
 
 // Can the head make queries of the context's descriptors?  Entered with c->mu held, in front of its attachment.

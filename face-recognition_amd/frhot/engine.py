@@ -352,11 +352,18 @@ class Head:
 
     def apply(self, x: np.ndarray) -> np.ndarray:
         """Descriptors [n, din] (host floats) -> unit rows [n, dout] float32, for a few at a time."""
+        return self._host(self._lib.frhot_head_apply, x)
+
+    def project(self, x: np.ndarray) -> np.ndarray:
+        """The same in front of the norm: what Gallery.upsert and Gallery.search turn into the head's rows, bit for bit."""
+        return self._host(self._lib.frhot_head_project, x)
+
+    def _host(self, call, x):
         x = np.ascontiguousarray(x, dtype=np.float32).reshape(-1, self.din)
         out = np.empty((len(x), self.dout), dtype=np.float32)
         for lo in range(0, len(x), 2048):
             part, sub = x[lo:lo + 2048], out[lo:lo + 2048]
-            check(self._lib.frhot_head_apply(self._h, _ptr(part, C.c_float), len(part), _ptr(sub, C.c_float)))
+            check(call(self._h, _ptr(part, C.c_float), len(part), _ptr(sub, C.c_float)))
         return out
 
 

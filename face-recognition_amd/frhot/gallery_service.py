@@ -270,11 +270,17 @@ class GalleryService:
                 return bool(np.isfinite(np.asarray(vec, dtype=np.float32)).all())   # (its row would match nothing)
         return len(vec) == self.dim
 
-    def _as_row(self, vec):
-        vec = np.asarray(vec, dtype=np.float32).reshape(-1)
-        if self.head is not None and vec.size == self.head.din:
-            vec = self.head.apply(_unit(vec))[0]
-        return vec
+    def _as_rows(self, vecs):
+        """Vectors of either length -> float32 rows for the gallery's upsert and search, which bring them to unit
+        length; the descriptors among them go through the head together.  (Its rows come in front of their norm, so
+        that they are rounded once, to what recognise_points compares with; a stand-in may only have unit ones.)"""
+        vecs = [np.asarray(v, dtype=np.float32).reshape(-1) for v in vecs]
+        at = [i for i, v in enumerate(vecs) if self.head is not None and v.size == self.head.din]
+        if at:
+            project = getattr(self.head, "project", self.head.apply)
+            for i, row in zip(at, project(np.stack([_unit(vecs[i]) for i in at]))):
+                vecs[i] = row
+        return vecs
 
     def _key(self, collection, store_id) -> int:
         k = (collection, store_id)
@@ -323,7 +329,7 @@ class GalleryService:
                 print(f"Error checking face limit: {e}")
             payload = {'id': id, 'name': name, 'store_id': store_id, 'time_created': time_created}
             try:
-                vec = self._as_row(vector_embedding).reshape(1, self.dim)
+                vec = self._as_rows([vector_embedding])[0].reshape(1, self.dim)
                 if is_update_id:
                     rows = self._by_id.get((collection_name, id))
                     if not rows:
@@ -428,7 +434,7 @@ class GalleryService:
                     out[i] = (200, {"message": "Point not found", "data": []})
                     continue
                 idx.append(i)
-                vecs.append(self._as_row(vec))
+                vecs.append(self._as_rows([vec])[0])
                 keys.append(k)
             if idx or self._always_search:
                 try:

@@ -417,6 +417,9 @@ int frhot_ctx_stage_ms(frhot_ctx* ctx, float* ms5);
  * frhot_head_apply: the same for host rows (x [M,din] float32, rounded to fp16; out [M,dout] float32
  *   holding the fp16 rows), for a few descriptors at a time (M up to 2048 at least); a finite component
  *   that fp16 does not hold is FRHOT_EINVAL.  Waits, and is FRHOT_ESTATE on a stream under graph capture.
+ * frhot_head_project: the last layer's rows themselves, float32, in front of their norm.  frhot_gallery_upsert
+ *   and frhot_search bring them to unit length as the head would, bit for bit; the rows of
+ *   frhot_head_apply they would round a second time.  Otherwise as frhot_head_apply.
  * frhot_gallery_head: bind a gallery to the head of 4096 inputs whose rows it holds (or, NULL, unbind it):
  *   frhot_recognise* on the gallery then make its queries with that head, whatever else the context
  *   serves.  Several galleries of one context can be bound, to one head or to several.  A head cannot be
@@ -438,6 +441,7 @@ int frhot_head_create(frhot_ctx* ctx, frhot_linear* const* layers, const int32_t
 int frhot_head_destroy(frhot_head* head);
 int frhot_head_dev(frhot_head* head, const void* x_f16_dev, int64_t ldx, int64_t M, void* out_f16_dev, int64_t ldo);
 int frhot_head_apply(frhot_head* head, const float* x, int M, float* out);
+int frhot_head_project(frhot_head* head, const float* x, int M, float* out);
 int frhot_ctx_head(frhot_ctx* ctx, frhot_head* head);
 int frhot_gallery_head(frhot_gallery* g, frhot_head* head);
 

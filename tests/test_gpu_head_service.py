@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 import torch
 
+from test_gpu_heads import linear_of
 from test_gpu_head_binding import faces, serve, spreading_head      # noqa: F401  (faces: the fixture)
 
 pytestmark = pytest.mark.gpu
@@ -48,4 +49,62 @@ def test_apply_refuses_what_fp16_does_not_hold(gpu_ctx, faces):      # noqa: F81
     x[1, 77] = np.nan
     got = head.apply(x)
     assert np.isnan(got[1]).all() and np.isfinite(got[[0, 2]]).all()
+    head.close()
+
+
+def test_host_vectors_are_rounded_once(gpu_ctx):
+    """Rows of few large components, where rounding to fp16, bringing to unit length and rounding again is not rounding once:
+    what the service stores and asks with are the head's own rows, bit for bit."""
+    from frhot.engine import Gallery, Head
+    from frhot.gallery_service import GalleryService
+    rng = np.random.default_rng(0)
+    w = np.zeros((64, 4096), np.float16)
+    w[:4] = rng.standard_normal((4, 4096))
+
+    def unit(v):
+        v = v.astype(np.float32)
+        return (v / np.sqrt((v.astype(np.float64) ** 2).sum(1, keepdims=True)).astype(np.float32)).astype(np.float16)
+    at = np.flatnonzero((unit(w[:4].T) != unit(unit(w[:4].T))).any(1))
+    assert at.size >= 20
+    x = np.zeros((at.size, 4096), np.float32)
+    x[np.arange(at.size), at] = 1
+    head = Head(gpu_ctx, [(linear_of(gpu_ctx, torch.from_numpy(w), None, "f16"), "none", False)])
+    xd, own = torch.from_numpy(x).half().cuda(), torch.empty(at.size, 64, dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    head.run_dev(xd.data_ptr(), at.size, own.data_ptr())
+    gpu_ctx.sync()
+    want = own.cpu().numpy()
+    assert np.array_equal(head.apply(x), want.astype(np.float32))
+    assert np.array_equal(head.project(x), w[:, at].T.astype(np.float32))
+    svc = GalleryService(gpu_ctx, capacity=600, head=head)
+    svc.create_collection("7_Employees")
+    for i in range(at.size):
+        assert svc.insert_point("7_Employees", x[i], f"p{i}", "n", 7)[0] == 201
+    rows = [next(r for r, p in svc._points.items() if p["payload"]["id"] == f"p{i}") for i in range(at.size)]
+    assert np.array_equal(svc.gallery.read(rows)[0], want)
+    other = Gallery(gpu_ctx, 64, 400)
+    other.fill_synthetic(5, 0, 400)
+    s, r = torch.empty(at.size, 5, device="cuda"), torch.empty(at.size, 5, dtype=torch.int64, device="cuda")
+    other.search_dev(own.data_ptr(), None, at.size, 5, s.data_ptr(), r.data_ptr())
+    gpu_ctx.sync()
+    hs, hr = other.search(head.project(x), None, 5)
+    assert np.array_equal(hs, s.cpu().numpy()) and np.array_equal(hr, r.cpu().numpy())
+    other.close()
+    svc.close()
+    head.close()
+
+
+def test_host_rows_of_many_sizes(gpu_ctx, faces):                    # noqa: F811
+    """The staging grows and shrinks between calls; every call gives the rows of run_dev."""
+    _, emb = faces
+    head = spreading_head(gpu_ctx, emb, 256, 6)
+    x = np.random.default_rng(1).standard_normal((2000, 4096)).astype(np.float32) / 64
+    xd, own = torch.from_numpy(x).half().cuda(), torch.empty(2000, 256, dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    for n in (1, 5, 2000, 3, 700, 1):
+        own.zero_()
+        torch.cuda.synchronize()
+        head.run_dev(xd.data_ptr(), n, own.data_ptr())
+        gpu_ctx.sync()
+        assert np.array_equal(head.apply(x[:n]), own[:n].cpu().numpy().astype(np.float32))
     head.close()
