@@ -266,8 +266,11 @@ class GalleryService:
         if vec is None:
             return False
         if self.head is not None and len(vec) == self.head.din:
-            with np.errstate(over="ignore"):
-                return bool(np.isfinite(np.asarray(vec, dtype=np.float32)).all())   # (its row would match nothing)
+            try:
+                with np.errstate(over="ignore"):
+                    return bool(np.isfinite(np.asarray(vec, dtype=np.float32)).all())   # (its row would match nothing)
+            except (TypeError, ValueError):
+                return False
         return len(vec) == self.dim
 
     def _as_rows(self, vecs):
@@ -434,12 +437,13 @@ class GalleryService:
                     out[i] = (200, {"message": "Point not found", "data": []})
                     continue
                 idx.append(i)
-                vecs.append(self._as_rows([vec])[0])
+                vecs.append(vec)
                 keys.append(k)
             if idx or self._always_search:
                 try:
                     seq0, moves = self._seq, self._moves
                     with self._device_call():
+                        vecs = self._as_rows(vecs)
                         scores, rows = self._search_batch(vecs, keys)
                     if self._moves != moves:        # the rows' numbers changed meanwhile: once more, with the lock held
                         scores, rows = self._search_batch(vecs, keys)

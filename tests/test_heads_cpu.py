@@ -1,4 +1,6 @@
 """Host side of descriptor heads in a service, over stand-ins."""
+import threading
+
 import numpy as np
 
 from test_pages_cpu import PagedGallery, found, service       # noqa: F401
@@ -72,7 +74,59 @@ def test_nonfinite_vectors_are_refused():
         assert svc.insert_point("A_Employees", w, "q", "n", 1) == (404, {"message": "Embedding not found or invalid!"})
         assert svc.insert_point("A_Employees", list(w), "q", "n", 1)[0] == 404
         assert svc.search_point("A_Employees", w, 1)[0] == 404
+    assert svc.insert_point("A_Employees", ["x"] * 128, "q", "n", 1)[0] == 404 and svc.search_point("A_Employees", [None, "x"] * 64, 1)[0] == 404
     assert svc.point_count("A_Employees") == 1
+
+
+def test_a_batch_of_searches_goes_through_the_head_at_once_and_without_the_lock():
+    rng = np.random.default_rng(2)
+    head = FakeHead()
+    svc = service(head=head)
+    svc.create_collection("A_Employees")
+    vecs = rng.standard_normal((40, 128)).astype(np.float32)
+    for i, v in enumerate(vecs):
+        assert svc.insert_point("A_Employees", v, f"p{i}", "n", 1)[0] == 201
+    head.calls.clear()
+    started, go, done = threading.Event(), threading.Event(), threading.Event()
+    plain = head.apply
+
+    def slow(x):
+        started.set()
+        assert go.wait(10)
+        return plain(x)
+    head.apply = slow
+    own = plain(vecs[33])[0]                        # a row of the gallery's own length among them
+    reqs = [("A_Employees", v, 1) for v in vecs[:32]] + [("A_Employees", own, 1), ("B_Employees", vecs[0], 1), ("A_Employees", None, 1)]
+    head.calls.clear()
+    answer = {}
+    t = threading.Thread(target=lambda: answer.update(out=svc.search_points(reqs)))
+    t.start()
+    assert started.wait(10)
+    other = threading.Thread(target=lambda: (svc.delete_point("A_Employees", "p39"), done.set()))
+    other.start()
+    assert done.wait(10), "a deletion waits for the head"
+    go.set()
+    t.join(10)
+    other.join(10)
+    out = answer["out"]
+    assert head.calls == [32]
+    assert [c["data"][0][1]["id"] for _s, c in out[:33]] == [f"p{i}" for i in range(32)] + ["p33"]
+    assert [s for s, _c in out[33:]] == [404, 404]
+
+
+def test_a_failing_head_answers_404():
+    svc = service(head=FakeHead())
+    svc.create_collection("A_Employees")
+    assert svc.insert_point("A_Employees", np.ones(128, np.float32), "p", "n", 1)[0] == 201
+
+    def broken(x):
+        raise RuntimeError("device lost")
+    svc.head.apply = broken
+    v = np.ones(128, np.float32)
+    assert svc.search_points([("B_Employees", v, 1), ("A_Employees", v, 1), ("A_Employees", v, 99)]) == [
+        (404, {"message": "Collection name not found or invalid!"}), (404, {"message": "device lost"}),
+        (200, {"message": "Point not found", "data": []})]
+    assert svc.insert_point("A_Employees", v, "q", "n", 1) == (404, {"message": "device lost"})
 
 
 def test_null_gallery_is_refused():
