@@ -220,6 +220,11 @@ class GalleryService:
             except Exception as e:
                 for r in dst:
                     self._rows.release(r)
+                if dst:
+                    try:        # whatever part of the copy landed must not answer searches
+                        self.gallery.tombstone(np.asarray(dst, dtype=np.int64))
+                    except Exception:
+                        pass
                 return 404, {"message": str(e)}
             self._collections.setdefault(collection_name, None)
             # in the order the points were inserted, so that the eviction of the oldest goes on as in the source
