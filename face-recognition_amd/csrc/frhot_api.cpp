@@ -303,6 +303,14 @@ int upload(void** dst, const void* src, size_t n) {
     return FRHOT_OK;
 }
 
+// Calls that wait or that change a gallery's host-side tables (they change with the call, not with a replay).
+int refuse_capture(frhot_ctx* c) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    HIP_TRY(hipStreamIsCapturing(c->stream, &st));
+    if (st != hipStreamCaptureStatusNone) return fail(FRHOT_ESTATE, "the call cannot be captured into a graph");
+    return FRHOT_OK;
+}
+
 constexpr int kSplitMin = 32;   // batches from this size on run their conv stack as two halves on two streams
 
 // The layers of a head over M fp16 rows of din values (`x`: rows ldx apart, or, `tiled`, the start of a tile of a gallery of
@@ -1521,6 +1529,23 @@ int frhot_gallery_read(frhot_gallery* g, const int64_t* rows, int n, void* out_f
     });
 }
 
+int frhot_gallery_read_keys(frhot_gallery* g, int64_t row0, int64_t n, int32_t* out_keys) {
+    return guarded([&]() -> int {
+    if (!g || !out_keys) return fail(FRHOT_EINVAL, "null argument");
+    if (n <= 0) return fail(FRHOT_EINVAL, "n must be positive");
+    if (row0 < 0 || row0 > g->capacity - n)
+        return fail(FRHOT_ECAPACITY, "rows [%lld,%lld) outside capacity %lld", (long long)row0, (long long)(row0 + n), (long long)g->capacity);
+    frhot_ctx* c = g->ctx;
+    std::lock_guard<std::mutex> lk(c->mu);
+    DeviceGuard dg(c->device);
+    const int rc = refuse_capture(c);
+    if (rc) return rc;
+    HIP_TRY(hipMemcpyAsync(out_keys, g->keys + row0, (size_t)n * 4, hipMemcpyDeviceToHost, c->stream));
+    HIP_TRY(hipStreamSynchronize(c->stream));
+    return FRHOT_OK;
+    });
+}
+
 int frhot_gallery_write_f16(frhot_gallery* g, const void* rows_f16, const int32_t* keys, const int64_t* rows, int n) {
     return guarded([&]() -> int {
     if (!g || !rows_f16 || !keys || !rows) return fail(FRHOT_EINVAL, "null argument");
@@ -2408,14 +2433,6 @@ int check_rows_args(const char* what, const void* p, int64_t ld, int64_t M, int6
     if (ld < n) return fail(FRHOT_EINVAL, "%s: rows of %lld values are %lld apart", what, (long long)n, (long long)ld);
     if (M > 1 && ld > (int64_t)1 << 40) return fail(FRHOT_EINVAL, "%s: row distance %lld", what, (long long)ld);
     if ((uintptr_t)p % type_size(type)) return fail(FRHOT_EINVAL, "%s is not aligned to its elements", what);
-    return FRHOT_OK;
-}
-
-// Calls that wait or that change a gallery's host-side tables (they change with the call, not with a replay).
-int refuse_capture(frhot_ctx* c) {
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    HIP_TRY(hipStreamIsCapturing(c->stream, &st));
-    if (st != hipStreamCaptureStatusNone) return fail(FRHOT_ESTATE, "the call cannot be captured into a graph");
     return FRHOT_OK;
 }
 

@@ -75,6 +75,7 @@ SIGNATURES = {
     "frhot_head_apply": (C.c_int, [_p, _f32p, C.c_int, _f32p]),
     "frhot_head_project": (C.c_int, [_p, _f32p, C.c_int, _f32p]),
     "frhot_ctx_head": (C.c_int, [_p, _p]),
+    "frhot_gallery_read_keys": (C.c_int, [_p, C.c_int64, C.c_int64, _i32p]),
     "frhot_gallery_head": (C.c_int, [_p, _p]),
     "frhot_gallery_copy": (C.c_int, [_p, _p, _p, _p, _p, _p, C.c_int]),
     "frhot_gallery_read_dev": (C.c_int, [_p, _p, _p, C.c_int, _p, _p]),

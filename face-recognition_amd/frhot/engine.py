@@ -477,6 +477,14 @@ class Gallery:
                                            _ptr(keys, C.c_int32)))
         return out, keys
 
+    def read_keys(self, row0: int = 0, n: int | None = None) -> np.ndarray:
+        """Keys (int32, host) of the n rows from row0 on; by default of all up to the last written one."""
+        n = self.rows - row0 if n is None else n
+        out = np.empty(max(n, 0), dtype=np.int32)
+        if n > 0:
+            check(self._lib.frhot_gallery_read_keys(self._h, row0, n, _ptr(out, C.c_int32)))
+        return out
+
     def write_f16(self, rows_f16: np.ndarray, keys, rows):
         """Restore rows exactly as read(): fp16 unit rows [n, D], keys [n], destination rows [n]."""
         rows_f16 = np.ascontiguousarray(rows_f16, dtype=np.float16).reshape(-1, self.dim)

@@ -242,8 +242,16 @@ class GalleryService:
         with self._lock:
             try:
                 live = sorted(self._points)
-                stray = np.setdiff1d(np.arange(self.gallery.rows), np.asarray(live, dtype=np.int64))
-                if stray.size:          # rows of the table's gaps that a failed write may have left alive
+                # The rows' new numbers follow from the table only if the device holds the same rows: that is looked at
+                # before anything moves.
+                keys, at = self._device_keys(), np.asarray(live, dtype=np.int64)
+                want = np.asarray([self._point_key(r) for r in live], dtype=np.int32)
+                lost = at[at >= keys.size].tolist() if live and live[-1] >= keys.size else at[keys[at] != want].tolist()
+                if lost:
+                    raise RuntimeError(f"{len(lost)} points, the first in row {lost[0]}, are not on the device under their "
+                                       "keys; nothing was moved")
+                stray = np.setdiff1d(np.flatnonzero(keys >= 0), at)
+                if stray.size:          # rows that the table does not know, left alive by a failed write
                     self.gallery.tombstone(stray)
                 n = self.gallery.compact()
                 if n != len(live):
@@ -253,9 +261,19 @@ class GalleryService:
             place = {r: i for i, r in enumerate(live)}
             self._points = {place[r]: self._points[r] for r in live}
             self._by_id = {k: [place[r] for r in rows] for k, rows in self._by_id.items()}
-            self._rows.reset([self._keys[(p["collection"], p["payload"].get("store_id"))] for p in self._points.values()])
+            self._rows.reset([self._point_key(r) for r in self._points])
             self._moves += 1
             return 200, {"message": "Gallery compacted", "points": len(live)}
+
+    def _point_key(self, row) -> int:
+        p = self._points[row]
+        return self._keys[(p["collection"], p["payload"].get("store_id"))]
+
+    def _device_keys(self):
+        """The keys of all the gallery's rows, from the device."""
+        if hasattr(self.gallery, "read_keys"):
+            return self.gallery.read_keys()
+        return self.gallery.read(np.arange(self.gallery.rows))[1]      # (a stand-in)
 
     # ----------------------------------------------------------------- points
     def _forget(self, row):

@@ -186,6 +186,10 @@ int frhot_gallery_fill_synthetic(frhot_gallery* g, uint64_t seed, int64_t row0, 
 /* Copy n stored rows back as fp16 [n,D] plus their keys (host buffers). */
 int frhot_gallery_read(frhot_gallery* g, const int64_t* rows, int n, void* out_f16, int32_t* out_keys);
 
+/* The keys of rows row0 .. row0 + n - 1 alone (host buffer): which rows live, four bytes a row.  Waits;
+ * FRHOT_ESTATE on a stream under graph capture. */
+int frhot_gallery_read_keys(frhot_gallery* g, int64_t row0, int64_t n, int32_t* out_keys);
+
 /*
  * Write n rows exactly as given: rows_f16 [n,D] fp16 (host; must already be unit
  * length, nothing is normalised), keys[n] (FRHOT_KEY_DEAD allowed), destination
