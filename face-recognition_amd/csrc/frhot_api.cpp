@@ -32,6 +32,8 @@ namespace {
 thread_local std::string g_err;
 
 int fail(int code, const char* fmt, ...) {
+    // A HIP call that failed stays the thread's last error until it is asked for, and the next launch would report it as its own.
+    if (code == FRHOT_EHIP || code == FRHOT_ECAPACITY) (void)hipGetLastError();
     char buf[512];
     va_list ap;
     va_start(ap, fmt);
