@@ -2460,7 +2460,8 @@ int frhot_linear_create(frhot_ctx* c, const void* w, const float* bias, int N, i
     std::lock_guard<std::mutex> lk(c->mu);
     DeviceGuard dg(c->device);
     if (!dg.ok) return fail(FRHOT_EHIP, "cannot select device %d", c->device);
-    int rc = linear_scratch(c);
+    int rc = refuse_capture(c);
+    if (!rc) rc = linear_scratch(c);
     if (rc) return rc;
     std::unique_ptr<frhot_linear> l(new frhot_linear());
     l->ctx = c; l->N = N; l->K = K; l->dtype = dtype;
@@ -2491,6 +2492,8 @@ int frhot_linear_destroy(frhot_linear* l) {
     std::lock_guard<std::mutex> lk(l->ctx->mu);
     if (l->heads) return fail(FRHOT_ESTATE, "the layer belongs to %d head(s)", l->heads);
     DeviceGuard dg(l->ctx->device);
+    const int rc = refuse_capture(l->ctx);
+    if (rc) return rc;
     (void)hipStreamSynchronize(l->ctx->stream);
     (void)hipFree(l->wt);
     if (l->wt2) (void)hipFree(l->wt2);
@@ -2566,6 +2569,8 @@ int frhot_head_create(frhot_ctx* c, frhot_linear* const* layers, const int32_t* 
     if (din % 64 || dout % 64) return fail(FRHOT_EINVAL, "a head takes and gives multiples of 64 values (%d -> %d)", din, dout);
     std::lock_guard<std::mutex> lk(c->mu);
     DeviceGuard dg(c->device);
+    const int held = refuse_capture(c);
+    if (held) return held;
     std::unique_ptr<frhot_head, void (*)(frhot_head*)> h(new frhot_head(), head_free);
     h->ctx = c; h->din = din; h->dout = dout;
     for (int i = 0; i < n; ++i) {
@@ -2608,6 +2613,8 @@ int frhot_head_destroy(frhot_head* h) {
     frhot_ctx* c = h->ctx;
     std::lock_guard<std::mutex> lk(c->mu);
     DeviceGuard dg(c->device);
+    const int rc = refuse_capture(c);
+    if (rc) return rc;
     if (h->galleries) return fail(FRHOT_ESTATE, "%d galler%s bound to the head", h->galleries, h->galleries == 1 ? "y is" : "ies are");
     (void)hipStreamSynchronize(c->stream);
     if (c->head == h) c->head = nullptr;
@@ -2699,7 +2706,8 @@ int frhot_ctx_head(frhot_ctx* c, frhot_head* h) {
     if (!c) return fail(FRHOT_EINVAL, "ctx is null");
     std::lock_guard<std::mutex> lk(c->mu);
     DeviceGuard dg(c->device);
-    const int rc = h ? head_takes_descriptors(c, h) : FRHOT_OK;
+    int rc = refuse_capture(c);
+    if (!rc && h) rc = head_takes_descriptors(c, h);
     if (rc) return rc;
     c->head = h;
     return FRHOT_OK;
@@ -2713,7 +2721,8 @@ int frhot_gallery_head(frhot_gallery* g, frhot_head* h) {
     std::lock_guard<std::mutex> lk(c->mu);
     DeviceGuard dg(c->device);
     if (h && h->dout != g->D) return fail(FRHOT_EINVAL, "a head of %d outputs for a gallery of dimension %d", h->dout, g->D);
-    const int rc = h ? head_takes_descriptors(c, h) : FRHOT_OK;
+    int rc = refuse_capture(c);
+    if (!rc && h) rc = head_takes_descriptors(c, h);
     if (rc) return rc;
     if (g->head) --g->head->galleries;
     if (h) ++h->galleries;

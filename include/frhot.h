@@ -433,7 +433,10 @@ int frhot_ctx_stage_ms(frhot_ctx* ctx, float* ms5);
  *   head's rows as queries, where they take the descriptor's leading components otherwise.  Destroying
  *   an attached head detaches it.
  * All *_dev calls enqueue on the context's stream and return.  They share the context's scratch:
- * graphs captured from one context's calls must not be replayed at the same time.
+ * graphs captured from one context's calls must not be replayed at the same time.  Creating, destroying,
+ * attaching and binding allocate, wait or change what later calls do: on a stream under graph capture they
+ * are FRHOT_ESTATE and leave the capture as it was.  A graph reads the weights of its layers and writes the
+ * scratch of its heads: it must not be replayed once one of them, or the context, is destroyed.
  */
 int frhot_linear_create(frhot_ctx* ctx, const void* w, const float* bias, int N, int K, int dtype, frhot_linear** out);
 int frhot_linear_destroy(frhot_linear* layer);
