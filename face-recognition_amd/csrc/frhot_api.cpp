@@ -841,7 +841,7 @@ int key_tiles_rebuild(frhot_gallery* g) {
         HIP_TRY(hipStreamSynchronize(g->ctx->stream));
         HIP_TRY(hipMemcpy(keys.data(), g->keys, keys.size() * 4, hipMemcpyDeviceToHost));
         for (int64_t r = 0; r < g->nrows; ++r) {
-            if (keys[(size_t)r] < 0) continue;
+            if (keys[(size_t)r] < 0 || (r & 255 && keys[(size_t)r] == keys[(size_t)r - 1])) continue;     // (a run's first row of a tile)
             std::vector<int32_t>& v = g->key_tiles[keys[(size_t)r]];
             const int32_t t = (int32_t)(r >> 8);
             if (v.empty() || v.back() != t) {                    // rows ascend, so do the tiles
@@ -852,6 +852,85 @@ int key_tiles_rebuild(frhot_gallery* g) {
     }
     g->key_tiles_valid = true;
     return FRHOT_OK;
+}
+
+// The lists of `g` behind a squeeze of `src` (g itself or another gallery): the live rows of src's tile t are g's rows off[t] up to off[t + 1]
+// (`live` behind the last).  A key's rows may lie anywhere among its tile's, so a tile's keys are listed in the one or two tiles that
+// these rows touch.  Lists that were given up or must be read back (g->key_tiles_valid false) are left so, and so are lists that have
+// grown to half of what is kept: reading the keys back makes them exact again.
+void key_tiles_squeezed(const frhot_gallery* src, frhot_gallery* g, const int32_t* off, int32_t ntiles, int32_t live) {
+    size_t entries = 0;
+    std::vector<int32_t> v;
+    auto moved = [&](const std::vector<int32_t>& list) {
+        v.clear();
+        for (const int32_t t : list) {
+            if (t >= ntiles) break;
+            const int32_t lo = off[t], hi = t + 1 < ntiles ? off[t + 1] : live;
+            if (lo == hi) continue;
+            for (int32_t u = lo >> 8; u <= (hi - 1) >> 8; ++u)
+                if (v.empty() || v.back() < u) v.push_back(u);
+        }
+        entries += v.size();
+    };
+    try {
+        if (src == g) {
+            for (auto it = g->key_tiles.begin(); it != g->key_tiles.end();) {
+                moved(it->second);
+                if (v.empty()) it = g->key_tiles.erase(it);
+                else (it++)->second.assign(v.begin(), v.end());
+            }
+        } else {
+            std::unordered_map<int32_t, std::vector<int32_t>> to;
+            to.reserve(src->key_tiles.size());
+            for (const auto& kv : src->key_tiles) {
+                moved(kv.second);
+                if (!v.empty()) to.emplace(kv.first, v);
+            }
+            g->key_tiles.swap(to);
+        }
+    } catch (const std::bad_alloc&) {       // (the rows have moved all the same)
+        return;
+    }
+    g->key_tiles_entries = entries;
+    g->key_tiles_valid = entries <= g->key_tiles_limit() / 2;
+}
+
+// The lists of `g` once rows of `src` (g itself or another gallery) were copied there under their own keys: whatever src lists for the
+// tiles that a run reads is listed for the tiles that it writes.  False: too many runs or entries for that (the keys are read back).
+bool key_tiles_copied(const frhot_gallery* src, const int64_t* src_rows, frhot_gallery* g, const int64_t* dst_rows, const int32_t* counts, int nruns) {
+    struct Piece { int32_t from, to; };
+    const size_t limit = g->key_tiles_limit();
+    std::vector<Piece> pieces;
+    for (int i = 0; i < nruns; ++i) {
+        const int64_t n = counts ? counts[i] : 1, s = src_rows[i], d = dst_rows[i];
+        for (int64_t t = s >> 8; t <= (s + n - 1) >> 8; ++t) {
+            const int64_t a = std::max(s, t << 8) - s, b = std::min(s + n, (t + 1) << 8) - 1 - s;      // rows a .. b of the run
+            for (int64_t u = (d + a) >> 8; u <= (d + b) >> 8; ++u) {
+                if (!pieces.empty() && pieces.back().from == t && pieces.back().to == u) continue;
+                if (pieces.size() == limit) return false;
+                pieces.push_back({(int32_t)t, (int32_t)u});
+            }
+        }
+    }
+    const auto before = [](const Piece& a, const Piece& b) { return a.from != b.from ? a.from < b.from : a.to < b.to; };
+    std::sort(pieces.begin(), pieces.end(), before);
+    pieces.erase(std::unique(pieces.begin(), pieces.end(), [](const Piece& a, const Piece& b) { return a.from == b.from && a.to == b.to; }), pieces.end());
+    std::vector<std::pair<int32_t, int32_t>> add;       // (key, tile): collected first, src's lists may be g's own
+    for (const auto& kv : src->key_tiles)
+        for (const int32_t t : kv.second)
+            for (auto p = std::lower_bound(pieces.begin(), pieces.end(), Piece{t, 0}, before); p != pieces.end() && p->from == t; ++p) {
+                if (add.size() == limit) return false;
+                add.emplace_back(kv.first, p->to);
+            }
+    for (const auto& kt : add) {
+        std::vector<int32_t>& v = g->key_tiles[kt.first];
+        const auto it = std::lower_bound(v.begin(), v.end(), kt.second);
+        if (it != v.end() && *it == kt.second) continue;
+        if (g->key_tiles_entries == limit) return false;
+        v.insert(it, kt.second);
+        ++g->key_tiles_entries;
+    }
+    return true;
 }
 
 int index_pin_grow(IndexPin& ip, size_t n, unsigned flags = hipHostMallocDefault) {
@@ -2848,9 +2927,9 @@ int page_move_enqueue(frhot_ctx* c, const PageSide& src, const int64_t* src_firs
 }
 
 // What a gallery's host-side tables know after the runs were written: `sorted` ascending destination runs, keys per run (in the
-// caller's order, `first` / `counts`) or null: keys that only the device knows.
+// caller's order, `first` / `counts`) or null: the rows' own, copied from `src_rows` of `src`.
 void page_note_writes(frhot_gallery* g, const std::vector<std::pair<int64_t, int64_t>>& sorted, const int64_t* first, const int32_t* counts,
-                      const int32_t* keys, int nruns, bool all_live) {
+                      const int32_t* keys, int nruns, bool all_live, const frhot_gallery* src = nullptr, const int64_t* src_rows = nullptr) {
     int64_t end = g->nrows;
     bool dense = g->dense && all_live;
     for (const auto& r : sorted) {
@@ -2859,11 +2938,15 @@ void page_note_writes(frhot_gallery* g, const std::vector<std::pair<int64_t, int
     }
     g->dense = dense;
     g->nrows = end;
-    if (!keys) { g->key_tiles_valid = false; return; }
     struct Guard {                  // lists that memory ran out for are rebuilt from the device when next needed
         frhot_gallery* g; bool whole;
         ~Guard() { if (!whole) g->key_tiles_valid = false; }
     } guard{g, false};
+    if (!keys && !g->key_tiles_off) {
+        guard.whole = g->key_tiles_valid && src->key_tiles_valid && !src->key_tiles_off &&
+                      key_tiles_copied(src, src_rows, g, first, counts, nruns);
+        return;
+    }
     if (!g->key_tiles_off && g->key_tiles_valid) {
         // one key for all runs (a fork): in ascending order every tile goes to the end of the key's list
         const bool one = std::all_of(keys, keys + nruns, [&](int32_t k) { return k == keys[0]; });
@@ -2920,7 +3003,7 @@ int frhot_gallery_copy(frhot_gallery* src, const int64_t* src_rows, frhot_galler
     DeviceGuard dg(c->device);
     rc = page_move_enqueue(c, PageSide{src->rows, src->keys, 0}, src_rows, PageSide{dst->rows, dst->keys, 0}, dst_rows, counts, keys, nruns, src->D);
     if (rc) return rc;
-    page_note_writes(dst, to, dst_rows, counts, keys, nruns, keys ? true : (src->dense && inside));
+    page_note_writes(dst, to, dst_rows, counts, keys, nruns, keys ? true : (src->dense && inside), src, src_rows);
     return FRHOT_OK;
     });
 }
@@ -3047,6 +3130,8 @@ int frhot_gallery_compact(frhot_gallery* src, frhot_gallery* dst, int64_t* new_r
     hipStream_t s = c->stream;
     frhot_gallery* g = dst ? dst : src;
     int64_t live = 0;
+    int32_t* off = nullptr;
+    const int32_t tiles = (int32_t)((src->nrows + 255) / 256);
     int rc = refuse_capture(c);
     if (rc) return rc;
     if (src->nrows == 0) {
@@ -3061,13 +3146,19 @@ int frhot_gallery_compact(frhot_gallery* src, frhot_gallery* dst, int64_t* new_r
             HIP_TRY(hipMalloc((void**)&c->page_off, cap * 4));
             c->page_off_cap = cap;
         }
+        // the host's lists of keys follow the rows by the tiles' offsets
+        const bool carried = src->key_tiles_valid && !src->key_tiles_off;
         IndexPin* ip = nullptr;
-        rc = page_pin_take(c, 16, &ip);
+        rc = page_pin_take(c, 16 + (carried ? ntiles : 0), &ip);
         if (rc) return rc;
         ip->p[0] = kUntold;
+        if (carried) {
+            off = ip->p + 16;
+            std::fill(off, off + ntiles, kUntold);
+        }
         if (dst && dst->capacity < src->nrows) {
             // the rows must fit, and only the device knows how many there are: count first
-            HIP_TRY(launch_page_count(src->keys, src->nrows, c->page_off, ip->p, s));
+            HIP_TRY(launch_page_count(src->keys, src->nrows, c->page_off, nullptr, ip->p, s));
             rc = page_await(c, ip->p, 1);
             if (rc) return rc;
             if (ip->p[0] > dst->capacity)
@@ -3089,9 +3180,10 @@ int frhot_gallery_compact(frhot_gallery* src, frhot_gallery* dst, int64_t* new_r
                 return fail(FRHOT_ECAPACITY, "no room for a second copy of the gallery: %s", hipGetErrorString(e));
             }
         }
-        hipError_t e = launch_page_compact(src->rows, src->keys, src->nrows, rows, keys, dst ? dst->nrows : 0, src->D, c->page_off, new_rows_dev, ip->p, s);
+        hipError_t e = launch_page_compact(src->rows, src->keys, src->nrows, rows, keys, dst ? dst->nrows : 0, src->D, c->page_off, new_rows_dev, off, ip->p, s);
         // (the count is the first thing the kernels know; into another gallery nothing else is waited for)
         if (e == hipSuccess) rc = page_await(c, ip->p, 1);
+        if (e == hipSuccess && !rc && off) rc = page_await(c, off, ntiles);
         if (e == hipSuccess && !rc) {
             live = ip->p[0];
             if (!dst && live > 0) {
@@ -3114,13 +3206,17 @@ int frhot_gallery_compact(frhot_gallery* src, frhot_gallery* dst, int64_t* new_r
         if (rc) return rc;
         if (e != hipSuccess) return fail(FRHOT_EHIP, "compacting failed: %s", hipGetErrorString(e));
     }
+    if (live_out) *live_out = live;
     g->nrows = live;
     g->dense = true;
-    std::unordered_map<int32_t, std::vector<int32_t>>().swap(g->key_tiles);
-    g->key_tiles_entries = 0;
     g->key_tiles_off = false;
-    g->key_tiles_valid = live == 0;     // (else read back from the keys when a by-key search next needs them)
-    if (live_out) *live_out = live;
+    g->key_tiles_valid = false;         // (if nothing else: read back from the keys when a by-key search next needs them)
+    if (off) key_tiles_squeezed(src, g, off, tiles, (int32_t)live);
+    if (!g->key_tiles_valid) {
+        std::unordered_map<int32_t, std::vector<int32_t>>().swap(g->key_tiles);
+        g->key_tiles_entries = 0;
+        g->key_tiles_valid = live == 0;
+    }
     return FRHOT_OK;
     });
 }

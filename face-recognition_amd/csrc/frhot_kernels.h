@@ -211,10 +211,11 @@ struct TileRun { int32_t first, n; };
 constexpr int kFreeTiles = 16, kFreeInline = 256;
 hipError_t launch_page_free(int32_t* g_keys, const TileRun* runs, int nruns, const int32_t* keys, int nkeys, int32_t* counts, hipStream_t s);
 // Live rows of src to the front of dst in order; dst's rows behind them (up to dst_rows) die.  offsets: ntiles(src) + 1 int32 of
-// scratch, the last of which receives the number of live rows, as does *total (page-locked, stored for the host to poll).
+// scratch: the live rows in front of every tile, and their number, which *total receives as well (page-locked, stored for the host to
+// poll).  host_offsets, if not null: page-locked too, receives the ntiles(src) offsets, each polled for by itself.
 hipError_t launch_page_compact(const void* src, const int32_t* src_keys, int64_t src_rows, void* dst, int32_t* dst_keys, int64_t dst_rows,
-                               int D, int32_t* offsets, int64_t* new_rows, int32_t* total, hipStream_t s);
-hipError_t launch_page_count(const int32_t* g_keys, int64_t rows, int32_t* offsets, int32_t* total, hipStream_t s);     // the first half of it
+                               int D, int32_t* offsets, int64_t* new_rows, int32_t* host_offsets, int32_t* total, hipStream_t s);
+hipError_t launch_page_count(const int32_t* g_keys, int64_t rows, int32_t* offsets, int32_t* host_offsets, int32_t* total, hipStream_t s);     // the first half of it
 hipError_t launch_page_kill(int32_t* g_keys, int64_t lo, int64_t hi, hipStream_t s);
 // The first n rows behind a tile's start, in plain order (dense [n, D] fp16).
 hipError_t launch_page_rows(const void* tile_start, void* out, int64_t n, int D, hipStream_t s);

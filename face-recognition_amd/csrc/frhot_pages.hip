@@ -131,8 +131,8 @@ __global__ __launch_bounds__(256) void page_count_kernel(const int32_t* __restri
     if (lane == 0) counts[t] = c;
 }
 
-// counts -> exclusive sums in place, the whole in offsets[n] and *total; one block
-__global__ __launch_bounds__(1024) void page_scan_kernel(int32_t* __restrict__ offsets, int n, int32_t* __restrict__ total) {
+// counts -> exclusive sums in place (and to host_offsets, if not null), the whole in offsets[n] and *total; one block
+__global__ __launch_bounds__(1024) void page_scan_kernel(int32_t* __restrict__ offsets, int n, int32_t* host_offsets, int32_t* total) {
     __shared__ int wsum[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int carry = 0;
@@ -154,6 +154,7 @@ __global__ __launch_bounds__(1024) void page_scan_kernel(int32_t* __restrict__ o
             all += wsum[w];
         }
         if (i < n) offsets[i] = carry + before + v - c;
+        if (i < n && host_offsets) tell_host(host_offsets + i, carry + before + v - c);
         carry += all;
         __syncthreads();
     }
@@ -163,7 +164,7 @@ __global__ __launch_bounds__(1024) void page_scan_kernel(int32_t* __restrict__ o
 // Both at once for up to kSmallTiles tiles (65,536 rows): a launch less.  (The keys of a gallery fill whole tiles.)
 constexpr int kSmallTiles = 256;
 __global__ __launch_bounds__(1024) void page_count_scan_kernel(const int32_t* __restrict__ gk, int64_t rows, int ntiles, int32_t* __restrict__ offsets,
-                                                               int32_t* __restrict__ total) {
+                                                               int32_t* host_offsets, int32_t* total) {
     __shared__ int cnt[kSmallTiles];
     __shared__ int wsum[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -201,6 +202,7 @@ __global__ __launch_bounds__(1024) void page_count_scan_kernel(const int32_t* __
         all += wsum[w];
     }
     if (tid < ntiles) offsets[tid] = before + v - c;
+    if (tid < ntiles && host_offsets) tell_host(host_offsets + tid, before + v - c);
     if (tid == 0) { offsets[ntiles] = all; tell_host(total, all); }
 }
 
@@ -315,23 +317,23 @@ hipError_t launch_page_free(int32_t* gk, const TileRun* runs, int nruns, const i
     return hipGetLastError();
 }
 
-hipError_t launch_page_count(const int32_t* gk, int64_t rows, int32_t* offsets, int32_t* total, hipStream_t s) {
+hipError_t launch_page_count(const int32_t* gk, int64_t rows, int32_t* offsets, int32_t* host_offsets, int32_t* total, hipStream_t s) {
     if (!gk || !offsets || !total || rows <= 0) return hipErrorInvalidValue;
     const int ntiles = (int)((rows + 255) / 256);
     if (ntiles <= kSmallTiles) {
-        hipLaunchKernelGGL(page_count_scan_kernel, dim3(1), dim3(1024), 0, s, gk, rows, ntiles, offsets, total);
+        hipLaunchKernelGGL(page_count_scan_kernel, dim3(1), dim3(1024), 0, s, gk, rows, ntiles, offsets, host_offsets, total);
         return hipGetLastError();
     }
     hipLaunchKernelGGL(page_count_kernel, dim3((unsigned)((ntiles + 3) / 4)), dim3(256), 0, s, gk, rows, ntiles, offsets);
-    hipLaunchKernelGGL(page_scan_kernel, dim3(1), dim3(1024), 0, s, offsets, ntiles, total);
+    hipLaunchKernelGGL(page_scan_kernel, dim3(1), dim3(1024), 0, s, offsets, ntiles, host_offsets, total);
     return hipGetLastError();
 }
 
 hipError_t launch_page_compact(const void* src, const int32_t* sk, int64_t src_rows, void* dst, int32_t* dk, int64_t dst_rows, int D,
-                               int32_t* offsets, int64_t* new_rows, int32_t* total, hipStream_t s) {
+                               int32_t* offsets, int64_t* new_rows, int32_t* host_offsets, int32_t* total, hipStream_t s) {
     if (!src || !sk || !dst || !dk || !offsets || !total || src_rows <= 0 || D <= 0 || D % 64) return hipErrorInvalidValue;
     const int ntiles = (int)((src_rows + 255) / 256), dtiles = (int)((dst_rows + 255) / 256), nk = D / 64;
-    const hipError_t e = launch_page_count(sk, src_rows, offsets, total, s);
+    const hipError_t e = launch_page_count(sk, src_rows, offsets, host_offsets, total, s);
     if (e != hipSuccess) return e;
     // One chunk a block, or two or four where that brings all blocks to run at once, eight a CU (20,011 rows of 4096, 70 % of them
     // live: 47.9 us with one chunk a block, 45.6 with four; 2 M rows of 512: 587 with one, 596 with four)
