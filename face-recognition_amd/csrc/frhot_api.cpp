@@ -2610,6 +2610,20 @@ int frhot_linear_dev(frhot_linear* l, const void* x_dev, int64_t ldx, int64_t M,
     });
 }
 
+int frhot_linear_debug_plan(int N, int K, int64_t M, int aligned, int pair, int32_t* plan4) {
+    return guarded([&]() -> int {
+    if (!plan4) return fail(FRHOT_EINVAL, "null argument");
+    if (N <= 0 || K <= 0 || N > kMaxWidth || K > kMaxWidth) return fail(FRHOT_EINVAL, "layer of %d x %d outside 1..%d", N, K, kMaxWidth);
+    if (M <= 0 || M > kMaxRows) return fail(FRHOT_EINVAL, "%lld rows outside 1..%lld", (long long)M, (long long)kMaxRows);
+    LinearWork ws{};
+    ws.slab_bytes = kSlabBytes; ws.pack_bytes = kPackBytes;
+    const bool whole = pair || (aligned && K % 8 == 0);
+    const LinearPlan p = linear_plan(M, linear_npad(N), (pair ? 2 : 1) * linear_kpad(K) / 64, whole, (size_t)linear_kpad(K) * 2, ws);
+    plan4[0] = p.shape; plan4[1] = p.splits; plan4[2] = p.gather; plan4[3] = !whole && !p.gather;
+    return FRHOT_OK;
+    });
+}
+
 int frhot_unit_rows_dev(frhot_ctx* c, const void* x_dev, int dtype, int64_t ldx, int64_t M, int N, void* out_f16_dev, int64_t ldo) {
     return guarded([&]() -> int {
     if (!c) return fail(FRHOT_EINVAL, "ctx is null");

@@ -181,6 +181,8 @@ struct LinearCall {
 };
 // Device scratch of the linear kernels.  Calls that use one such scratch must be ordered among themselves.
 struct LinearWork { float* slabs; size_t slab_bytes; void* pack; size_t pack_bytes; const void* zeros; };   // zeros: 128 bytes of 0
+// row_bytes: of a packed row.  (linear_npad(N), 64-deep steps of x; whole: LDS-DMA takes the rows of x as they lie.)
+LinearPlan linear_plan(int64_t M, int npad, int ksteps, bool whole, size_t row_bytes, const LinearWork& ws);
 size_t linear_layout_bytes(int N, int K);
 hipError_t launch_linear_layout(const void* w, void* wt, int N, int K, hipStream_t s);
 hipError_t launch_linear(const LinearCall& q, const LinearWork& ws, hipStream_t s);

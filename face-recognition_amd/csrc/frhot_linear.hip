@@ -978,6 +978,15 @@ hipError_t launch_linear_layout(const void* w, void* wt, int N, int K, hipStream
     return hipGetLastError();
 }
 
+LinearPlan linear_plan(int64_t M, int npad, int ksteps, bool whole, size_t row_bytes, const LinearWork& ws) {
+    LinearPlan p = plan_linear((int)(M < kRunRows ? M : kRunRows), npad, ksteps, whole, (int64_t)(ws.pack_bytes / row_bytes), ws.slab_bytes);
+    const int per = (ksteps + p.splits - 1) / p.splits;
+    p.splits = (ksteps + per - 1) / per;                        // (no empty slice)
+    p.M = M;
+    p.whole = whole;
+    return p;
+}
+
 hipError_t launch_linear(const LinearCall& q, const LinearWork& ws, hipStream_t s) {
     if (q.M <= 0 || q.N <= 0 || q.K <= 0 || !q.x || !q.wt || !q.bias || !q.out.out || !ws.slabs || !ws.pack || !ws.zeros || !q.plan)
         return hipErrorInvalidValue;
@@ -989,12 +998,7 @@ hipError_t launch_linear(const LinearCall& q, const LinearWork& ws, hipStream_t 
     // can LDS-DMA take the rows?
     const bool whole = q.tiled || (a.K % 8 == 0 && q.ldx % 8 == 0 && (size_t)q.x % 16 == 0);
     const size_t row_bytes = (size_t)linear_kpad(q.K) * 2;
-    const int64_t pack_rows = (int64_t)(ws.pack_bytes / row_bytes);
-    if (q.plan->M != q.M || q.plan->whole != whole) {
-        *q.plan = plan_linear((int)(q.M < kRunRows ? q.M : kRunRows), a.npad, a.ksteps, whole, pack_rows, ws.slab_bytes);
-        q.plan->M = q.M;
-        q.plan->whole = whole;
-    }
+    if (q.plan->M != q.M || q.plan->whole != whole) *q.plan = linear_plan(q.M, a.npad, a.ksteps, whole, row_bytes, ws);
     const LinearPlan& plan = *q.plan;
     const bool pack = !whole && !plan.gather;
     for (int64_t m0 = 0; m0 < q.M; m0 += kRunRows) {        // (a launch has fewer than 2^32 threads)
@@ -1017,7 +1021,7 @@ hipError_t launch_linear(const LinearCall& q, const LinearWork& ws, hipStream_t 
         if (o.res) o.res = (const char*)o.res + (size_t)m0 * o.ldr * rsz;
         if (o.scale) o.scale += m0;
         o.N = q.N;
-        const int per = (a.ksteps + plan.splits - 1) / plan.splits, splits = (a.ksteps + per - 1) / per;    // (no empty slice)
+        const int splits = plan.splits;
         a.slab = splits > 1 ? ws.slabs : nullptr;
         hipError_t e = q.bf16 ? launch_shape<true>(plan.shape, a, o, splits, plan.gather, s, false)
                               : launch_shape<false>(plan.shape, a, o, splits, plan.gather, s, false);

@@ -68,6 +68,7 @@ SIGNATURES = {
     "frhot_linear_create": (C.c_int, [_p, _p, _p, C.c_int, C.c_int, C.c_int, C.POINTER(_p)]),
     "frhot_linear_destroy": (C.c_int, [_p]),
     "frhot_linear_dev": (C.c_int, [_p, _p, C.c_int64, C.c_int64, C.c_int, _p, C.c_int64, C.c_int, _p, C.c_int64, C.c_int]),
+    "frhot_linear_debug_plan": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_int, C.c_int, _i32p]),
     "frhot_unit_rows_dev": (C.c_int, [_p, _p, C.c_int, C.c_int64, C.c_int64, C.c_int, _p, C.c_int64]),
     "frhot_head_create": (C.c_int, [_p, C.POINTER(_p), _i32p, _i32p, C.c_int, C.POINTER(_p)]),
     "frhot_head_destroy": (C.c_int, [_p]),

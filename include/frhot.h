@@ -407,6 +407,9 @@ int frhot_ctx_stage_ms(frhot_ctx* ctx, float* ms5);
  *   aligned, make a large call take up to 1.7 times as long).  Nothing beyond out's N columns and M rows is written, nothing
  *   beyond K columns read.  out may be the residual itself (same address, row distance and element
  *   size) and may not overlap x or the residual otherwise.  M = 0 does nothing.
+ * frhot_linear_debug_plan: what a call of M rows of a layer of N x K runs as (no device needed; for tests):
+ *   plan4 = {tile shape, K slices, rows through registers, rows packed first}.  aligned: x and ldx are
+ *   multiples of 16 bytes; pair: the layer stands behind another one in a head.
  * frhot_unit_rows_dev: out[m] = fp16(x[m] / |x[m]|), x [M,N] of any type: norm and rounding as
  *   frhot_gallery_upsert applies them (64-bit sum of squares, float32 norm; rows shorter than 1e-30
  *   are divided by one).  out may not overlap x.
@@ -442,6 +445,7 @@ int frhot_linear_create(frhot_ctx* ctx, const void* w, const float* bias, int N,
 int frhot_linear_destroy(frhot_linear* layer);
 int frhot_linear_dev(frhot_linear* layer, const void* x_dev, int64_t ldx, int64_t M, int act, const void* residual_dev, int64_t ldr,
                      int residual_dtype, void* out_dev, int64_t ldo, int out_dtype);
+int frhot_linear_debug_plan(int N, int K, int64_t M, int aligned, int pair, int32_t* plan4);
 int frhot_unit_rows_dev(frhot_ctx* ctx, const void* x_dev, int dtype, int64_t ldx, int64_t M, int N, void* out_f16_dev, int64_t ldo);
 int frhot_head_create(frhot_ctx* ctx, frhot_linear* const* layers, const int32_t* acts, const int32_t* residuals, int n,
                       frhot_head** out);
