@@ -856,9 +856,9 @@ int key_tiles_rebuild(frhot_gallery* g) {
 
 // The lists of `g` behind a squeeze of `src` (g itself or another gallery): the live rows of src's tile t are g's rows off[t] up to off[t + 1]
 // (`live` behind the last).  A key's rows may lie anywhere among its tile's, so a tile's keys are listed in the one or two tiles that
-// these rows touch.  Lists that were given up or must be read back (g->key_tiles_valid false) are left so, and so are lists that have
-// grown to half of what is kept: reading the keys back makes them exact again.
-void key_tiles_squeezed(const frhot_gallery* src, frhot_gallery* g, const int32_t* off, int32_t ntiles, int32_t live) {
+// these rows touch.  False: there is no memory for them, or they have grown to half of what is kept, and reading the keys back makes
+// them exact again.
+bool key_tiles_squeezed(const frhot_gallery* src, frhot_gallery* g, const int32_t* off, int32_t ntiles, int32_t live) {
     size_t entries = 0;
     std::vector<int32_t> v;
     auto moved = [&](const std::vector<int32_t>& list) {
@@ -889,10 +889,10 @@ void key_tiles_squeezed(const frhot_gallery* src, frhot_gallery* g, const int32_
             g->key_tiles.swap(to);
         }
     } catch (const std::bad_alloc&) {       // (the rows have moved all the same)
-        return;
+        return false;
     }
     g->key_tiles_entries = entries;
-    g->key_tiles_valid = entries <= g->key_tiles_limit() / 2;
+    return entries <= g->key_tiles_limit() / 2;
 }
 
 // The lists of `g` once rows of `src` (g itself or another gallery) were copied there under their own keys: whatever src lists for the
@@ -3145,7 +3145,7 @@ int frhot_gallery_compact(frhot_gallery* src, frhot_gallery* dst, int64_t* new_r
     frhot_gallery* g = dst ? dst : src;
     int64_t live = 0;
     int32_t* off = nullptr;
-    const int32_t tiles = (int32_t)((src->nrows + 255) / 256);
+    bool lists = false;
     int rc = refuse_capture(c);
     if (rc) return rc;
     if (src->nrows == 0) {
@@ -3210,6 +3210,8 @@ int frhot_gallery_compact(frhot_gallery* src, frhot_gallery* dst, int64_t* new_r
                 if (e == hipSuccess) e = hipMemcpyAsync(src->keys, keys, (size_t)live * 4, hipMemcpyDeviceToDevice, s);
             }
             if (!dst && e == hipSuccess) e = launch_page_kill(src->keys, live, src->nrows, s);
+            g->key_tiles_valid = false;     // (while the rows are on their way: a failure leaves the lists to be read back)
+            if (e == hipSuccess && off) lists = key_tiles_squeezed(src, g, off, (int32_t)ntiles, (int32_t)live);
         }
         if (!dst) {
             const hipError_t es = hipStreamSynchronize(s);
@@ -3224,12 +3226,10 @@ int frhot_gallery_compact(frhot_gallery* src, frhot_gallery* dst, int64_t* new_r
     g->nrows = live;
     g->dense = true;
     g->key_tiles_off = false;
-    g->key_tiles_valid = false;         // (if nothing else: read back from the keys when a by-key search next needs them)
-    if (off) key_tiles_squeezed(src, g, off, tiles, (int32_t)live);
-    if (!g->key_tiles_valid) {
+    g->key_tiles_valid = lists || live == 0;        // (else read back from the keys when a by-key search next needs them)
+    if (!lists) {
         std::unordered_map<int32_t, std::vector<int32_t>>().swap(g->key_tiles);
         g->key_tiles_entries = 0;
-        g->key_tiles_valid = live == 0;
     }
     return FRHOT_OK;
     });
