@@ -235,14 +235,16 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const uint16_t* __rest
     *(uint4v*)(out + t * 8) = load_chunk(x + (size_t)r * ldx, k0, K);
 }
 
-// The rows between two layers of a head.  Their values are fp32 and the matrix instruction takes fp16: each value goes in as the
-// sum of two fp16 numbers, hi the value rounded and lo what that left, so the next layer is one product of twice the depth over its
-// weights, laid out twice in a row (going round in one copy inside the kernels' loops cost the call of one row 0.2 of 6.1 us) (fp32 matrix instructions run at a sixteenth of the rate).  A row is first brought by a power of two to a largest
-// finite value in 2^14 .. 2^15, which fp16 holds whatever the row's own range; the epilogue takes the power back.  Lost is half a
-// step of lo: 2^-24 of the value, or 2^-39 of the row's largest where that is more.  (The power stops at 2^100: rows smaller
-// than 2^-85 lose 2^-125 absolutely.)  Infinities and NaN stay what they are in hi, with nothing in lo.
-// A wave takes a row; rows of up to 512 R values are read once.  With fp16 inner rows 2011 x 4096 -> 1024 -> 512 took 40.5 us and was
-// 2.9e-4 off its 64-bit value (2-norm), with pairs 49.1 us and 2.1e-4, which is the unit rows' own rounding.
+// The rows between two layers of a head.  Their values are fp32 and the matrix instruction takes fp16 (its fp32 form runs at a
+// sixteenth of the rate): each value goes in as the sum of two fp16 numbers, hi the value rounded and lo what that left, so the next
+// layer is one product of twice the depth.  Its weights are laid out twice in a row for that; going round in one copy inside the
+// products' loops cost a call of one row 0.2 of 6.1 us.  A row is first brought by a power of two to a largest finite value in
+// 2^14 .. 2^15, which fp16 holds whatever the row's own range; the epilogue takes the power back.  Lost is half a step of lo: 2^-23 of
+// the value at most, or 2^-39 of the row's largest where that is more.  (The power stops at 2^126, where that is less than half of
+// fp32's smallest number.)  Infinities and NaN stay what they are in hi, with nothing in lo.
+// A wave takes a row; rows of up to 512 R values are read once.  2011 x 1024: 5.6 us, mostly the launch.  With fp16 inner rows the whole
+// of 2011 x 4096 -> 1024 -> 512 took 40.5 us and was 2.9e-4 off its 64-bit value (2-norm), with pairs 48.6 us and 2.1e-4, which is the
+// unit rows' own rounding.
 template <int R>
 __global__ __launch_bounds__(256) void linear_split_kernel(const float* __restrict__ x, int64_t ldx, int N, int kpad,
                                                            half_t* __restrict__ out, float* __restrict__ scale, int rows) {
@@ -275,7 +277,7 @@ __global__ __launch_bounds__(256) void linear_split_kernel(const float* __restri
     for (int s = 32; s > 0; s >>= 1) most = fmaxf(most, __shfl_xor(most, s));
     int e = 0;
     (void)frexpf(most, &e);                                         // most = f 2^e, f in [1/2, 1)
-    const int up = most > 0.f ? min(15 - e, 100) : 0;
+    const int up = most > 0.f ? min(15 - e, 126) : 0;
     const float by = ldexpf(1.f, up);
     if (lane == 0) scale[m] = ldexpf(1.f, -up);
     auto store = [&](int c, const float (&t)[8]) __attribute__((always_inline)) {

@@ -417,7 +417,7 @@ int frhot_ctx_stage_ms(frhot_ctx* ctx, float* ms5);
  *   activations and, where residuals[i] != 0, the layer's own input added to its output (residuals
  *   may be NULL); the last layer's rows are brought to unit length.  First input and last output are
  *   multiples of 64.  Every layer's output stays fp32: an inner one goes into the next product as two
- *   fp16 numbers a value (2^-24 of the value, or 2^-39 of its row's largest value where that is more),
+ *   fp16 numbers a value (2^-23 of the value, or 2^-39 of its row's largest value where that is more),
  *   whatever the row's range; a layer behind another one keeps its weights three times over.
  *   The layers stay the caller's and must outlive the head.
  * frhot_head_dev: fp16 rows x [M,din] -> unit fp16 rows out [M,dout].

@@ -105,3 +105,19 @@ def test_inner_rows_of_different_ranges_and_nonfinite_ones(ctx):             # n
     assert torch.equal(got[same], plain[same])
     assert (got[7] == 0).all() and torch.isnan(got[20]).all() and torch.isnan(got[[33, 34]]).all()
     head.close()
+
+
+@pytest.mark.parametrize("scale", [1.0, 1e-30, 3e37, 1e-5])
+def test_what_a_pair_of_fp16_numbers_loses(ctx, scale):  # noqa: F811
+    """Inner values that use all of fp32's bits (a bias on nothing), passed on unchanged: half a step of the second number,
+    2^-23 of the value, or 2^-39 of the row's largest, and the rounding of the two numbers' sum."""
+    g = torch.Generator().manual_seed(5)
+    b = torch.randn(1024, generator=g) * torch.rand(1024, generator=g) ** 8 * scale
+    b[:4] = torch.tensor([scale, -scale, 0.0, scale * (1 + 2.0 ** -11 + 2.0 ** -23)])
+    layers = [(torch.zeros(1024, 64, dtype=torch.float16), b, "none", False), (torch.eye(1024).half(), None, "none", False)]
+    head = head_of(ctx, layers)
+    got = torch.from_numpy(head.project(np.zeros((3, 64), np.float32))).double()
+    want = b.double().expand(3, -1)
+    tol = torch.maximum(2.0 ** -23 * want.abs(), 2.0 ** -39 * want.abs().max()) + 2.0 ** -24 * want.abs()
+    assert ((got - want).abs() <= tol).all()
+    head.close()
