@@ -113,3 +113,40 @@ def test_binding_and_attaching(gpu_ctx, faces):
     for x in (other, far, small):
         x.close()
     c2.close()
+
+
+def test_services_asked_at_the_same_time(gpu_ctx, faces):
+    """Threads on two services with heads of one width, by crop and by vector, while one of them is squeezed."""
+    import threading
+    crops, emb = faces
+    rng = np.random.default_rng(3)
+    heads = [spreading_head(gpu_ctx, emb, 256, s) for s in (3, 4)]
+    svcs = [serve(gpu_ctx, emb, rng, head=h) for h in heads]
+    errors, stop = [], threading.Event()
+
+    def ask(j):
+        svc, r = svcs[j % 2], np.random.default_rng(j)
+        try:
+            while not stop.is_set():
+                at = r.permutation(8)[:4]
+                if j < 2:
+                    got = [c["data"][0][1]["id"] for _s, c, _e in svc.recognise_points([("7_Employees", crops[i], 7) for i in at])]
+                else:
+                    got = [c["data"][0][1]["id"] for _s, c in svc.search_points([("7_Employees", emb[i] * 2, 7) for i in at])]
+                assert got == [f"p{i}" for i in at], got
+        except Exception as e:
+            errors.append(e)
+    ts = [threading.Thread(target=ask, args=(j,)) for j in range(4)]
+    [t.start() for t in ts]
+    try:
+        for i in range(0, 100, 2):
+            assert svcs[0].delete_point("7_Employees", f"s{i}")[0] == 200
+            if i % 20 == 0:
+                assert svcs[0].compact()[0] == 200
+    finally:
+        stop.set()
+        [t.join(60) for t in ts]
+    assert not errors, errors[0]
+    for svc, h in zip(svcs, heads):
+        svc.close()
+        h.close()
